@@ -8,6 +8,7 @@ import numpy as np
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # STAG_HIP_LIB selects another build of the same library (kernel ablation variants for profiling)
 LIB_PATH = os.environ.get("STAG_HIP_LIB") or os.path.join(_HERE, "lib", "libstag_hip.so")
+TRAIN_LIB_PATH = os.path.join(_HERE, "lib", "libstag_train.so")
 
 STAG_OK = 0
 SEQ_OK, SEQ_MISSING_CLASSIFIER, SEQ_STRING_CLASSIFIER, SEQ_RANKCUT_SHAPE, SEQ_EMPTY_PATH, \
@@ -78,22 +79,58 @@ EXPORTS = {
     "stag_profile_read": (ctypes.c_int, [c_p, c_p, c_p]),
 }
 
+# include/stag_train.h
+TRAIN_EXPORTS = {
+    "stag_train_last_error": (ctypes.c_char_p, []),
+    "stag_row_scores_workspace": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
+    "stag_row_scores_grad_workspace": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
+    "stag_row_scores_dev": (ctypes.c_int, [c_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, c_p, ctypes.c_int64, c_p, ctypes.c_int32,
+                                           ctypes.c_int64, c_p, ctypes.c_int32, ctypes.c_float, c_p, ctypes.c_int64, c_p, ctypes.c_int64, c_p]),
+    "stag_row_scores_grad_dev": (ctypes.c_int, [c_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, c_p, ctypes.c_int64, c_p, ctypes.c_int32,
+                                                ctypes.c_int64, ctypes.c_int32, ctypes.c_float, c_p, ctypes.c_int64, c_p, c_p, ctypes.c_int64,
+                                                c_p]),
+    "stag_sibling_loss_workspace": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int32]),
+    "stag_sibling_loss_dev": (ctypes.c_int, [c_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, c_p, c_p, c_p, ctypes.c_float, c_p, c_p,
+                                             ctypes.c_int32, ctypes.c_int64, c_p, ctypes.c_int64, c_p]),
+    "stag_adamw_dev": (ctypes.c_int, [c_p, c_p, ctypes.c_int64, ctypes.c_int32, c_p, c_p, c_p, c_p, c_p, ctypes.c_double, ctypes.c_double,
+                                      ctypes.c_double, ctypes.c_double, c_p]),
+}
+
 _lib = None
+_train = None
+
+
+def _load(path, exports):
+    if not os.path.exists(path):
+        raise StagError("%s is missing: build it with `make -C stag_amd/csrc` "
+                        "(there is no CPU fallback for this path)" % path)
+    L = ctypes.CDLL(path)
+    for name, (res, args) in exports.items():
+        fn = getattr(L, name)
+        fn.restype = res
+        fn.argtypes = args
+    return L
+
+
+def train_lib():
+    """Load libstag_train.so (include/stag_train.h)."""
+    global _train
+    if _train is None:
+        _train = _load(TRAIN_LIB_PATH, TRAIN_EXPORTS)
+    return _train
+
+
+def check_train(rc):
+    if rc != STAG_OK:
+        msg = train_lib().stag_train_last_error()
+        raise StagError("libstag_train error %d: %s" % (rc, msg.decode("utf-8", "replace") if msg else "?"))
 
 
 def lib():
     """Load libstag_hip.so (built in-tree by ``__graft_entry__.build()`` / ``make -C stag_amd/csrc``)."""
     global _lib
     if _lib is None:
-        if not os.path.exists(LIB_PATH):
-            raise StagError("%s is missing: build it with `make -C stag_amd/csrc` "
-                            "(there is no CPU fallback for this path)" % LIB_PATH)
-        L = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in EXPORTS.items():
-            fn = getattr(L, name)
-            fn.restype = res
-            fn.argtypes = args
-        _lib = L
+        _lib = _load(LIB_PATH, EXPORTS)
     return _lib
 
 

@@ -1,0 +1,367 @@
+"""Learning node classifiers on the GPU (include/stag_train.h): the counterpart of the scoring that the walk does.
+
+The reference fits one logistic regression per tree node on the CPU (stag/create_db.py:127-145).  Here the children of a
+node -- or all nodes of a level -- share a TABLE of coefficients [n_features, k]: row f belongs to token f (5 * alignment column +
+symbol), column c to classifier c, and a step of the fit is
+
+    scores        = row_scores(bits, table, bias, rows=batch)
+    loss, grad    = sibling_loss(scores, label, ...)
+    row_scores_grad(bits, grad, n_features, rows=batch, out=(table_grad, bias_grad))
+    optimizer.step()                                   # AdamW over every table and bias, with an L1 penalty
+
+``bits`` are packed one-hot rows as ``Database.encode_a2m`` / ``stag_encode_a2m_dev`` make them, on the GPU.  ``fit_siblings`` runs
+these steps for the children of one node and returns coefficients in the form ``load_db`` gives them, for
+``Database.from_dicts``.
+
+All functions take torch tensors on one GPU, enqueue their work on that GPU's current stream and return without waiting;
+they take no part in autograd.  With their outputs given (``out=``) or allocated under capture they can be recorded into a
+HIP graph.  Inputs whose rows are not contiguous are copied first; outputs have to be as documented.
+"""
+import ctypes
+import math
+
+import numpy as np
+import torch
+
+from . import _lib
+
+BLOCK, TILE = 256, 1024            # STAG_ADAMW_BLOCK, STAG_ADAMW_TILE
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_TENSOR = np.dtype([("param", "<u8"), ("grad", "<u8"), ("count", "<i8"), ("state_at", "<i8"), ("weight_decay", "<f4"), ("l1", "<f4"),
+                    ("param_type", "<i4"), ("grad_type", "<i4")])      # stag_adamw_tensor_t
+
+
+def _need(cond, msg, *args):
+    if not cond:
+        raise ValueError(msg % args)
+
+
+def _is(name, t, dtypes, dim):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch tensor" % name)
+    dtypes = dtypes if isinstance(dtypes, tuple) else (dtypes,)
+    if t.dtype not in dtypes:
+        raise TypeError("%s is %s: %s is wanted" % (name, t.dtype, " or ".join(str(d) for d in dtypes)))
+    _need(t.dim() == dim, "%s has %d dimensions: %d are wanted", name, t.dim(), dim)
+
+
+def _one_gpu(**tensors):
+    device = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        _need(t.device.type == "cuda", "%s is on %s: the operators run on the GPU", name, t.device)
+        _need(device is None or t.device == device, "%s is on %s, other tensors on %s", name, t.device, device)
+        device = t.device
+    return device
+
+
+def _rows(t):
+    """t with contiguous rows (copied if they are not), and its row stride."""
+    n, k = t.shape
+    if (k > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < k):
+        t = t.contiguous()
+    return t, (t.stride(0) if n > 1 else k)
+
+
+def _out_rows(name, t, shape, dtype):
+    _is(name, t, dtype, len(shape))
+    _need(tuple(t.shape) == tuple(shape), "%s has shape %s: %s is wanted", name, tuple(t.shape), tuple(shape))
+    if len(shape) == 1:
+        _need(shape[0] <= 1 or t.stride(0) == 1, "%s must be contiguous", name)
+        return shape[0]
+    _need((shape[1] <= 1 or t.stride(1) == 1) and (shape[0] <= 1 or t.stride(0) >= shape[1]), "%s must have contiguous rows that do not overlap", name)
+    return t.stride(0) if shape[0] > 1 else shape[1]
+
+
+def _packed(bits, n_features):
+    """bits, its row stride in words."""
+    _need(bits.shape[1] * 32 >= n_features, "bits has %d words a row: too few for %d features", bits.shape[1], n_features)
+    n, w = bits.shape
+    if (w > 1 and bits.stride(1) != 1) or (n > 1 and bits.stride(0) < w):
+        bits = bits.contiguous()
+    stride = bits.stride(0) if n > 1 else -(-w // 4) * 4
+    _need(w % 4 == 0 and stride % 4 == 0 and bits.data_ptr() % 16 == 0, "rows of bits must be whole, aligned 16-byte units (as stag_encode_a2m writes them)")
+    return bits, stride
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _work(nbytes, device):
+    if nbytes < 0:
+        _lib.check_train(int(nbytes))
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+class _on:
+    """The tensors' GPU as the current one, and its current stream."""
+
+    def __init__(self, device):
+        self.guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
+        self.stream = torch.cuda.current_stream(device).cuda_stream
+
+    def __enter__(self):
+        if self.guard:
+            self.guard.__enter__()
+        return self.stream
+
+    def __exit__(self, *a):
+        if self.guard:
+            self.guard.__exit__(*a)
+
+
+def row_scores(bits, table, bias=None, *, scale=1.0, rows=None, out=None):
+    """scores[i, c] = scale * (sum of table[f, c] over the features f of row rows[i] of bits) + bias[c], float32 [m, k]
+    (the sum of run_logistic_prediction, stag/classify.py:22-27; an embedding lookup summed over a row's tokens).
+
+    bits: int32 / uint32 [n, words]; table: float32, bfloat16 or float16 [n_features, k]; bias: float32 [k]; rows: int32 [m], any
+    order, repeats allowed, an index outside 0..n-1 is padding and scores 0 (default: all rows of bits)."""
+    _is("bits", bits, (torch.int32, torch.uint32), 2)
+    _is("table", table, tuple(_TYPES), 2)
+    n_features, k = table.shape
+    _need(n_features >= 1 and k >= 1, "table is empty: %s", tuple(table.shape))
+    if bias is not None:
+        _is("bias", bias, torch.float32, 1)
+        _need(bias.shape[0] == k, "bias has %d values, the table %d columns", bias.shape[0], k)
+        bias = bias.contiguous()
+    if rows is not None:
+        _is("rows", rows, torch.int32, 1)
+        rows = rows.contiguous()
+    m = bits.shape[0] if rows is None else rows.shape[0]
+    score_stride = k if out is None else _out_rows("out", out, (m, k), torch.float32)
+    device = _one_gpu(bits=bits, table=table, bias=bias, rows=rows, out=out)
+    bits, row_stride = _packed(bits, n_features)
+    table, table_stride = _rows(table)
+    lib = _lib.train_lib()
+    with _on(device) as stream:
+        if out is None:
+            out = torch.empty((m, k), dtype=torch.float32, device=device)
+        need = lib.stag_row_scores_workspace(m, n_features, k, _TYPES[table.dtype])
+        work = _work(need, device)
+        _lib.check_train(lib.stag_row_scores_dev(_ptr(bits), bits.shape[0], row_stride, n_features, _ptr(rows), m, _ptr(table), _TYPES[table.dtype],
+                                                 table_stride, _ptr(bias), k, float(scale), _ptr(out), score_stride, _ptr(work), need, stream))
+    return out
+
+
+def row_scores_grad(bits, grad, n_features, *, scale=1.0, rows=None, out=None):
+    """The gradient of row_scores: (table_grad float32 [n_features, k], bias_grad float32 [k]) with
+    table_grad[f, c] = scale * (sum of grad[i, c] over the i whose row has feature f), bias_grad[c] = sum of grad[i, c].
+
+    grad: float32, bfloat16 or float16 [m, k].  Padding rows (see row_scores) take part in neither, whatever grad holds for
+    them.  out: a pair of tensors to overwrite."""
+    _is("bits", bits, (torch.int32, torch.uint32), 2)
+    _is("grad", grad, tuple(_TYPES), 2)
+    n_features = int(n_features)
+    m, k = grad.shape
+    _need(n_features >= 1 and k >= 1, "no features (%d) or no classifiers (%d)", n_features, k)
+    if rows is not None:
+        _is("rows", rows, torch.int32, 1)
+        rows = rows.contiguous()
+    _need(m == (bits.shape[0] if rows is None else rows.shape[0]), "grad has %d rows, the batch %d", m, bits.shape[0] if rows is None else rows.shape[0])
+    table_grad, bias_grad = out if out is not None else (None, None)
+    stride = k
+    if out is not None:
+        stride = _out_rows("out[0]", table_grad, (n_features, k), torch.float32)
+        _out_rows("out[1]", bias_grad, (k,), torch.float32)
+    device = _one_gpu(bits=bits, grad=grad, rows=rows, table_grad=table_grad, bias_grad=bias_grad)
+    bits, row_stride = _packed(bits, n_features)
+    grad, grad_stride = _rows(grad)
+    lib = _lib.train_lib()
+    with _on(device) as stream:
+        if out is None:
+            table_grad = torch.empty((n_features, k), dtype=torch.float32, device=device)
+            bias_grad = torch.empty((k,), dtype=torch.float32, device=device)
+        need = lib.stag_row_scores_grad_workspace(m, n_features, k, _TYPES[grad.dtype])
+        work = _work(need, device)
+        _lib.check_train(lib.stag_row_scores_grad_dev(_ptr(bits), bits.shape[0], row_stride, n_features, _ptr(rows), m, _ptr(grad), _TYPES[grad.dtype],
+                                                      grad_stride, k, float(scale), _ptr(table_grad), stride, _ptr(bias_grad), _ptr(work), need, stream))
+    return table_grad, bias_grad
+
+
+def sibling_loss(scores, label, *, siblings=None, weight=None, scale=1.0, grad_dtype=None, out=None):
+    """Logistic loss of "this sibling or one of the others" and its gradient: (loss float32 [k], grad [m, k]).
+
+    Row i trains the columns siblings[i, 0] <= c < siblings[i, 1] (int32 [m, 2]; children of a node are neighbours in
+    breadth-first numbering; default: all k) with target 1 for c == label[i] (int32 [m]) and 0 for the others; a label
+    outside them makes the row a negative example for all.  loss[c] = scale * sum of weight[i] * softplus(+-score);
+    grad is d(sum of loss)/d(scores) of type grad_dtype (default float32), 0 where a row does not train, and scores are not
+    read there.  weight: float32 [m].  out: a pair of tensors to overwrite."""
+    _is("scores", scores, torch.float32, 2)
+    _is("label", label, torch.int32, 1)
+    m, k = scores.shape
+    _need(k >= 1, "no classifiers")
+    _need(label.shape[0] == m, "label has %d values, scores %d rows", label.shape[0], m)
+    label = label.contiguous()
+    if siblings is not None:
+        _is("siblings", siblings, torch.int32, 2)
+        _need(tuple(siblings.shape) == (m, 2), "siblings has shape %s: %s is wanted", tuple(siblings.shape), (m, 2))
+        siblings = siblings.contiguous()
+    if weight is not None:
+        _is("weight", weight, torch.float32, 1)
+        _need(weight.shape[0] == m, "weight has %d values, scores %d rows", weight.shape[0], m)
+        weight = weight.contiguous()
+    loss, grad = out if out is not None else (None, None)
+    dtype = grad_dtype or (grad.dtype if grad is not None else torch.float32)
+    if dtype not in _TYPES:
+        raise TypeError("grad_dtype is %s: %s is wanted" % (dtype, " or ".join(str(d) for d in _TYPES)))
+    grad_stride = k
+    if out is not None:
+        _out_rows("out[0]", loss, (k,), torch.float32)
+        grad_stride = _out_rows("out[1]", grad, (m, k), dtype)
+    device = _one_gpu(scores=scores, label=label, siblings=siblings, weight=weight, loss=loss, grad=grad)
+    scores, score_stride = _rows(scores)
+    lib = _lib.train_lib()
+    with _on(device) as stream:
+        if out is None:
+            loss = torch.empty((k,), dtype=torch.float32, device=device)
+            grad = torch.empty((m, k), dtype=dtype, device=device)
+        need = lib.stag_sibling_loss_workspace(m, k)
+        work = _work(need, device)
+        _lib.check_train(lib.stag_sibling_loss_dev(_ptr(scores), score_stride, m, k, _ptr(label), _ptr(siblings), _ptr(weight), float(scale),
+                                                   _ptr(loss), _ptr(grad), _TYPES[dtype], grad_stride, _ptr(work), need, stream))
+    return loss, grad
+
+
+class AdamW:
+    """AdamW over a list of tensors, one launch a step, with an optional L1 shrinkage (stag_adamw_dev).
+
+    params, grads: lists of contiguous tensors (float32, bfloat16 or float16) on one GPU, a gradient as large as its parameter.  The
+    optimizer holds THESE tensors: it reads the gradients from them and updates the parameters in place, at every step.
+    weight_decay, l1: a number, or one for each tensor.  state_bits 32 keeps the moments as floats; 8 keeps e4m3 codes with a
+    power-of-two scale for each 256 values (m, m_scale: the first moment; v, v_scale: the ROOT of the second), 2.03 bytes
+    a value instead of 8.  m, v and the scales are flat: tensor j's values begin at place state_at[j], a multiple of 256.
+    The step count lives on the GPU, so a captured step() counts on when it is replayed; lr and the others are the values that
+    step() was called with (attributes, may be changed between steps)."""
+
+    def __init__(self, params, grads, *, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, l1=0.0, state_bits=32):
+        params, grads = list(params), list(grads)
+        _need(len(params) >= 1, "no parameters")
+        _need(len(params) == len(grads), "%d parameters, %d gradients", len(params), len(grads))
+        _need(state_bits in (8, 32), "state_bits = %r: 8 or 32 are wanted", state_bits)
+        decay = [float(x) for x in (weight_decay if isinstance(weight_decay, (list, tuple)) else [weight_decay] * len(params))]
+        l1 = [float(x) for x in (l1 if isinstance(l1, (list, tuple)) else [l1] * len(params))]
+        _need(len(decay) == len(params) and len(l1) == len(params), "weight_decay and l1 are one number, or one for each of the %d tensors", len(params))
+        for x in decay + l1:
+            _need(math.isfinite(x) and x >= 0, "weight_decay and l1 are not negative: got %r", x)
+        self.lr, self.betas, self.eps, self.state_bits = lr, tuple(betas), eps, state_bits
+        self._check()
+        spans = []
+        for j, (p, g) in enumerate(zip(params, grads)):
+            for name, t in (("params[%d]" % j, p), ("grads[%d]" % j, g)):
+                if not isinstance(t, torch.Tensor) or t.dtype not in _TYPES:
+                    raise TypeError("%s must be a float32, bfloat16 or float16 tensor" % name)
+                _need(t.is_contiguous(), "%s is not contiguous", name)
+            _need(p.shape == g.shape, "params[%d] has shape %s, its gradient %s", j, tuple(p.shape), tuple(g.shape))
+        device = _one_gpu(**{"params[%d]" % j: p for j, p in enumerate(params)}, **{"grads[%d]" % j: g for j, g in enumerate(grads)})
+        for written, kind, tensors in ((True, "params", params), (False, "grads", grads)):
+            spans += [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), written, "%s[%d]" % (kind, j)) for j, t in enumerate(tensors) if t.numel()]
+        last, last_written = (0, 0, False, ""), (0, 0, True, "")
+        for span in sorted(spans):         # gradients may share memory with each other, what is written with nothing
+            before = last if span[2] else last_written
+            _need(before[1] <= span[0], "%s and %s share memory", before[3], span[3])
+            last = max(last, span, key=lambda x: x[1])
+            last_written = max(last_written, span, key=lambda x: x[1]) if span[2] else last_written
+        self.device, self.params, self.grads = device, params, grads
+        table = np.zeros(len(params), dtype=_TENSOR)
+        counts = np.array([p.numel() for p in params], dtype=np.int64)
+        padded = -(-counts // BLOCK) * BLOCK
+        self.state_at = [int(x) for x in np.concatenate([[0], np.cumsum(padded)[:-1]])]
+        self.state_values = int(padded.sum())
+        table["param"] = [p.data_ptr() for p in params]
+        table["grad"] = [g.data_ptr() for g in grads]
+        table["count"], table["state_at"] = counts, self.state_at
+        table["weight_decay"], table["l1"] = decay, l1
+        table["param_type"] = [_TYPES[p.dtype] for p in params]
+        table["grad_type"] = [_TYPES[g.dtype] for g in grads]
+        n_tiles = -(-counts // TILE)
+        first = np.concatenate([[0], np.cumsum(n_tiles)[:-1]])
+        tiles = np.empty((int(n_tiles.sum()), 2), dtype=np.int32)
+        tiles[:, 0] = np.repeat(np.arange(len(params)), n_tiles)
+        tiles[:, 1] = np.arange(len(tiles)) - np.repeat(first, n_tiles)
+        self._n_tiles = len(tiles)
+        self._tensors = torch.from_numpy(table.view(np.uint8)).to(device)
+        self._tiles = torch.from_numpy(tiles).to(device)
+        self._step = torch.zeros(2, dtype=torch.int32, device=device)
+        size = max(self.state_values, BLOCK)
+        kind = torch.float32 if state_bits == 32 else torch.float8_e4m3fn
+        self.m = torch.zeros(size, dtype=torch.float32, device=device).to(kind)
+        self.v = torch.zeros(size, dtype=torch.float32, device=device).to(kind)
+        self.m_scale = self.v_scale = None
+        if state_bits == 8:
+            self.m_scale = torch.ones(size // BLOCK, dtype=torch.float32, device=device)
+            self.v_scale = torch.ones(size // BLOCK, dtype=torch.float32, device=device)
+
+    def _check(self):
+        b1, b2 = self.betas
+        _need(math.isfinite(self.lr) and self.lr >= 0, "lr = %r", self.lr)
+        _need(0 < b1 < 1 and 0 < b2 < 1, "betas = %r: not inside (0, 1)", self.betas)
+        _need(math.isfinite(self.eps) and self.eps >= 0, "eps = %r", self.eps)
+
+    def step(self):
+        """One step with the gradients as they stand."""
+        self._check()
+        lib = _lib.train_lib()
+        with _on(self.device) as stream:
+            _lib.check_train(lib.stag_adamw_dev(_ptr(self._tensors), _ptr(self._tiles), self._n_tiles, self.state_bits, _ptr(self.m), _ptr(self.v),
+                                                _ptr(self.m_scale), _ptr(self.v_scale), _ptr(self._step), float(self.lr), float(self.betas[0]),
+                                                float(self.betas[1]), float(self.eps), stream))
+
+    @property
+    def steps(self):
+        """Steps done so far (waits for the GPU)."""
+        return int(self._step[0].item())
+
+    def load_state(self, steps, m, v, m_scale=None, v_scale=None):
+        """Takes up a state as .steps, .m, .v, .m_scale and .v_scale give it."""
+        _need(0 <= int(steps) < 2**31 - 1, "steps = %r", steps)
+        given = {"m": m, "v": v, "m_scale": m_scale, "v_scale": v_scale}
+        for name, t in given.items():
+            mine = getattr(self, name)
+            _need((t is None) == (mine is None), "%s: %s", name, "missing" if t is None else "states of 32 bits have none")
+            if mine is not None:
+                _is(name, t, mine.dtype, 1)
+                _need(t.shape == mine.shape, "%s has %d values: %d are wanted", name, t.shape[0], mine.shape[0])
+        for name, t in given.items():
+            if t is not None:
+                getattr(self, name).copy_(t)
+        self._step.copy_(torch.tensor([int(steps), 0], dtype=torch.int32))
+
+
+def fit_siblings(bits, label, k, n_features, *, steps=200, batch=None, lr=0.05, l1=0.0, weight_decay=0.0, weight=None, table_dtype=torch.float32,
+                 state_bits=32, seed=0, device=None):
+    """Fits the classifiers of k siblings (the children of one node, stag/create_db.py:127-145) and returns float64 [k, 1 + n_features]:
+    intercept and coefficients as load_db gives them (stag/databases.py:96-104), one row a sibling.
+
+    bits: packed rows uint32 [n, words] (NumPy, as Database.encode_a2m returns them) or a tensor; label: the sibling of each row,
+    another value = a negative example for all.  l1 penalises coefficients (not the intercept) by l1 * |w| beside the mean loss
+    of a row.  batch: rows a step (default all), drawn anew each pass by `seed`."""
+    if isinstance(bits, np.ndarray):
+        bits = torch.from_numpy(np.ascontiguousarray(bits).view(np.int32)).to(device or "cuda")
+    device = bits.device
+    n, k, n_features = bits.shape[0], int(k), int(n_features)
+    _need(n >= 1, "no rows")
+    label = torch.as_tensor(label).to(device=device, dtype=torch.int32)
+    _need(tuple(label.shape) == (n,), "label has shape %s: %s is wanted", tuple(label.shape), (n,))
+    if weight is not None:
+        weight = torch.as_tensor(weight).to(device=device, dtype=torch.float32)
+    batch = n if batch is None else max(1, min(int(batch), n))
+    table = torch.zeros((n_features, k), dtype=table_dtype, device=device)
+    bias = torch.zeros(k, device=device)
+    table_grad, bias_grad = torch.empty((n_features, k), device=device), torch.empty(k, device=device)
+    optimizer = AdamW([table, bias], [table_grad, bias_grad], lr=lr, weight_decay=[weight_decay, 0.0], l1=[l1, 0.0], state_bits=state_bits)
+    draw = torch.Generator(device="cpu").manual_seed(int(seed))
+    order, at, rows = None, 0, None
+    for _ in range(int(steps)):
+        if batch < n:
+            if order is None or at + batch > n:
+                order, at = torch.randperm(n, generator=draw).to(device=device, dtype=torch.int32), 0
+            rows, at = order[at:at + batch], at + batch
+        here = None if rows is None else rows.long()
+        scores = row_scores(bits, table, bias, rows=rows)
+        _, grad = sibling_loss(scores, label if here is None else label[here], weight=weight if here is None or weight is None else weight[here],
+                               scale=1.0 / batch)
+        row_scores_grad(bits, grad, n_features, rows=rows, out=(table_grad, bias_grad))
+        optimizer.step()
+    return torch.cat([bias[:, None], table.float().t()], 1).double().cpu().numpy()

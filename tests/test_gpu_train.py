@@ -1,0 +1,609 @@
+"""The operators that learn node classifiers (stag_amd.train, include/stag_train.h) against plain 64-bit implementations."""
+import math
+import os
+
+import numpy as np
+import pytest
+import torch
+
+from stag_amd import train
+
+if os.path.exists("/dev/kfd"):
+    torch.cuda.is_available()      # torch's copy of the HIP runtime has to be the first in a process
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+U = 2.0 ** -23                     # a 32-bit operation is off by at most half of this, whichever way it rounds by at most this
+
+
+def packed(rng, n, n_features, density=0.2, garbage=True):
+    """Random packed rows; the bits behind the last feature hold garbage, which has to be ignored."""
+    words = -(-n_features // 128) * 4
+    x = rng.random((n, words * 32)) < density
+    if not garbage:
+        x[:, n_features:] = False
+    bits = np.packbits(x, axis=1, bitorder="little").view(np.int32).reshape(n, words)
+    return torch.from_numpy(bits.copy()).to(DEV), x[:, :n_features].astype(np.float64)
+
+
+def picked(x, rows):
+    """The batch's rows of x, and which of them are no padding."""
+    if rows is None:
+        return x, np.ones(len(x), bool)
+    real = (rows >= 0) & (rows < len(x))
+    return x[np.where(real, rows, 0)] * real[:, None], real
+
+
+def half_step(t, dtype):
+    """Half a step of dtype at |t| (values below the smallest normal ones: half of the smallest step)."""
+    info = torch.finfo(dtype)
+    return np.maximum(np.abs(t), info.smallest_normal) * info.eps / 2
+
+
+def near(got, want, tol, what=""):
+    got, want = np.asarray(got, np.float64), np.asarray(want, np.float64)
+    assert got.shape == want.shape, (got.shape, want.shape)
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), "%s: %d of %d off; worst %g over its tolerance at %s" % (
+        what, bad.sum(), bad.size, np.nanmax((np.abs(got - want) / np.maximum(tol, 1e-300))[bad]), np.argwhere(bad)[0])
+
+
+# n rows held, batch (None: all rows in order), features, classifiers
+SHAPES = [
+    (1, None, 1, 1), (1, None, 145, 2), (2, None, 31, 3), (3, None, 32, 8), (5, 7, 33, 1), (16, None, 127, 31), (17, 1, 128, 32), (20, 40, 129, 33),
+    (31, None, 145, 7), (32, None, 640, 64), (33, 65, 643, 65), (64, None, 750, 13), (65, 63, 750, 100), (100, 129, 1000, 257), (300, None, 2100, 5),
+    (200, 300, 5250, 4), (1, None, 7500, 8), (4, 4, 7500, 1000), (1000, 1025, 300, 40), (700, 513, 1500, 96), (2000, 3001, 145, 10), (40, None, 20000, 12),
+    (600, 1100, 700, 300),
+]
+
+
+def batch(rng, n, m):
+    if m is None:
+        return None, None
+    rows = rng.integers(0, n, m).astype(np.int32)
+    rows[rng.random(m) < 0.1] = -1
+    if m > 2:
+        rows[[0, m - 1]] = [n, 2**31 - 1]      # past the end is padding too
+    return rows, torch.from_numpy(rows).to(DEV)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n, m, n_features, k", SHAPES)
+def test_scores(n, m, n_features, k, dtype):
+    rng = np.random.default_rng(n + 7 * n_features + k)
+    bits, x = packed(rng, n, n_features)
+    rows, d_rows = batch(rng, n, m)
+    table = torch.from_numpy(rng.normal(size=(n_features, k)).astype(np.float32)).to(DEV).to(dtype)
+    bias = torch.from_numpy(rng.normal(size=k).astype(np.float32)).to(DEV)
+    scale = 0.37
+    got = train.row_scores(bits, table, bias, scale=scale, rows=d_rows)
+    assert got.dtype == F32
+    xb, real = picked(x, rows)
+    t, b = table.double().cpu().numpy(), bias.double().cpu().numpy()
+    want = np.where(real[:, None], scale * (xb @ t) + b, 0.0)
+    # a sum of N terms in 32 bits, in any order, is off by at most N U sum|terms|; the rounding of scale, product and bias: 4 more
+    tol = (xb.sum(1)[:, None] + 4) * U * (scale * (xb @ np.abs(t)) + np.abs(b)) * real[:, None]
+    near(got.cpu(), want, tol)
+    assert torch.equal(got, train.row_scores(bits, table, bias, scale=scale, rows=d_rows))
+    near(train.row_scores(bits, table, scale=scale, rows=d_rows).cpu(), np.where(real[:, None], scale * (xb @ t), 0.0), tol)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n, m, n_features, k", SHAPES)
+def test_grad(n, m, n_features, k, dtype):
+    rng = np.random.default_rng(n + 7 * n_features + k)
+    bits, x = packed(rng, n, n_features)
+    rows, d_rows = batch(rng, n, m)
+    xb, real = picked(x, rows)
+    grad = torch.from_numpy(rng.normal(size=(len(xb), k)).astype(np.float32)).to(DEV).to(dtype)
+    g = np.where(real[:, None], grad.double().cpu().numpy(), 0.0)
+    grad[torch.from_numpy(~real).to(DEV)] = math.nan         # padding rows hold anything
+    scale = 0.37
+    table_grad, bias_grad = train.row_scores_grad(bits, grad, n_features, scale=scale, rows=d_rows)
+    assert table_grad.dtype == bias_grad.dtype == F32
+    near(table_grad.cpu(), scale * (xb.T @ g), (xb.sum(0)[:, None] + 4) * U * scale * (xb.T @ np.abs(g)), "table")
+    near(bias_grad.cpu(), g.sum(0), (real.sum() + 4) * U * np.abs(g).sum(0), "bias")
+    again = train.row_scores_grad(bits, grad, n_features, scale=scale, rows=d_rows)
+    assert torch.equal(table_grad, again[0]) and torch.equal(bias_grad, again[1])
+
+
+@pytest.mark.parametrize("n, k", [(4, 3), (80, 8), (700, 24), (2500, 200)])
+def test_32_bit_values_keep_their_24_bits(n, k):
+    """One token a row, so that nothing hides the rounding of a value: what comes back is the value."""
+    rng = np.random.default_rng(n)
+    n_features = 900
+    words = -(-n_features // 128) * 4
+    f = rng.permutation(np.arange(n) % n_features)
+    bits = np.zeros((n, words), np.uint32)
+    bits[np.arange(n), f >> 5] = np.uint32(1) << (f & 31).astype(np.uint32)
+    bits = torch.from_numpy(bits.view(np.int32)).to(DEV)
+    table = torch.from_numpy((rng.normal(size=(n_features, k)) * 10.0 ** rng.uniform(-12, 12, size=(n_features, k))).astype(np.float32)).to(DEV)
+    got = train.row_scores(bits, table).cpu().numpy()
+    want = table.cpu().numpy()[f]
+    near(got, want, 2 * U * np.abs(want))
+    grad = torch.from_numpy((rng.normal(size=(n, k)) * 10.0 ** rng.uniform(-12, 12, size=(n, k))).astype(np.float32)).to(DEV)
+    table_grad = train.row_scores_grad(bits, grad, n_features)[0].cpu().numpy()
+    want, size = np.zeros((n_features, k)), np.zeros((n_features, k))
+    np.add.at(want, f, grad.double().cpu().numpy())
+    np.add.at(size, f, grad.double().abs().cpu().numpy())
+    near(table_grad, want, (2 + n // n_features + 1) * U * size)
+
+
+@pytest.mark.parametrize("n, k", [(1, 4), (40, 5), (600, 70), (1500, 200)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_infinities_reach_only_the_rows_that_have_the_token(n, k, dtype):
+    rng = np.random.default_rng(9)
+    n_features = 333
+    bits, x = packed(rng, n, n_features)
+    table = torch.from_numpy(rng.normal(size=(n_features, k)).astype(np.float32)).to(DEV).to(dtype)
+    table[17, 0], table[200, k - 1], table[201, k // 2] = math.inf, math.nan, -math.inf
+    got = train.row_scores(bits, table).cpu().numpy()
+    t = table.double().cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        want = np.stack([t[r > 0].sum(0) for r in x])
+    fine = np.isfinite(want)
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)])
+    near(got[fine], want[fine], 400 * U * np.abs(t[np.isfinite(t)]).max() * 400)
+    grad = torch.from_numpy(rng.normal(size=(n, k)).astype(np.float32)).to(DEV).to(dtype)
+    grad[n // 2, 0], grad[n - 1, k - 1] = math.inf, math.nan
+    got = train.row_scores_grad(bits, grad, n_features)
+    g = grad.double().cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        want = np.stack([g[c > 0].sum(0) for c in x.T])
+        near_bias = g.sum(0)
+    assert np.array_equal(np.isnan(got[0].cpu().numpy()), np.isnan(want)) and np.array_equal(np.isinf(got[0].cpu().numpy()), np.isinf(want))
+    assert np.array_equal(np.isnan(got[1].cpu().numpy()), np.isnan(near_bias)) and np.array_equal(np.isinf(got[1].cpu().numpy()), np.isinf(near_bias))
+
+
+@pytest.mark.parametrize("n, k", [(3, 5), (50, 40), (700, 130)])
+def test_strided_tables_and_outputs(n, k):
+    """Tables, gradients and outputs inside larger buffers at odd places, with what lies between the rows left as it was."""
+    rng = np.random.default_rng(5)
+    n_features = 777
+    words = -(-n_features // 128) * 4
+    wide = torch.randint(-2**31, 2**31 - 1, (n, words + 8), device=DEV, dtype=torch.int32)
+    bits, x = packed(rng, n, n_features)
+    wide[:, 4:4 + words] = bits
+    inside = wide[:, 4:4 + words]
+    big = torch.from_numpy(rng.normal(size=(n_features, k + 5)).astype(np.float32)).to(DEV)
+    table = big[:, 3:3 + k]
+    out = torch.full((n, k + 7), 7.0, device=DEV)
+    got = train.row_scores(inside, table, out=out[:, 1:1 + k])
+    assert got.data_ptr() == out[:, 1:].data_ptr()
+    t = table.double().cpu().numpy()
+    near(got.cpu(), x @ t, (x.sum(1)[:, None] + 4) * U * (x @ np.abs(t)))
+    assert (out[:, 0] == 7).all() and (out[:, 1 + k:] == 7).all()
+    near(train.row_scores(bits, table.t().contiguous().t()).cpu(), x @ t, (x.sum(1)[:, None] + 4) * U * (x @ np.abs(t)))   # columns apart: copied
+    grad = torch.from_numpy(rng.normal(size=(n, k + 3)).astype(np.float32)).to(DEV)[:, 2:2 + k]
+    into = torch.full((n_features + 2, k + 1), 7.0, device=DEV)
+    bias = torch.full((k + 2,), 7.0, device=DEV)
+    train.row_scores_grad(inside, grad, n_features, out=(into[:n_features, 1:], bias[1:1 + k]))
+    g = grad.double().cpu().numpy()
+    near(into[:n_features, 1:].cpu(), x.T @ g, (x.sum(0)[:, None] + 4) * U * (x.T @ np.abs(g)))
+    assert (into[n_features:] == 7).all() and (into[:, 0] == 7).all() and bias[0] == 7 and bias[-1] == 7
+    one = torch.from_numpy(rng.normal(size=(1, k)).astype(np.float32)).to(DEV).expand(n, k)      # a broadcast gradient
+    near(train.row_scores_grad(bits, one, n_features)[0].cpu(), x.T @ one.double().cpu().numpy(), (x.sum(0)[:, None] + 4) * U * x.sum(0)[:, None] * 5)
+
+
+def test_empty_batches():
+    bits, _ = packed(np.random.default_rng(0), 5, 40)
+    none = torch.empty(0, dtype=torch.int32, device=DEV)
+    table = torch.ones(40, 3, device=DEV)
+    assert train.row_scores(bits, table, rows=none).shape == (0, 3)
+    assert train.row_scores(bits[:0], table).shape == (0, 3)
+    into = (torch.full((40, 3), 7.0, device=DEV), torch.full((3,), 7.0, device=DEV))
+    train.row_scores_grad(bits, torch.empty(0, 3, device=DEV), 40, rows=none, out=into)
+    assert (into[0] == 0).all() and (into[1] == 0).all()
+    padding = torch.full((70,), -1, dtype=torch.int32, device=DEV)
+    assert (train.row_scores(bits, table, torch.ones(3, device=DEV), rows=padding) == 0).all()
+    assert (train.row_scores(bits[:0], table, torch.ones(3, device=DEV), rows=torch.zeros_like(padding)) == 0).all()
+    got = train.row_scores_grad(bits, torch.full((70, 3), math.nan, device=DEV), 40, rows=padding)
+    assert (got[0] == 0).all() and (got[1] == 0).all()
+    loss, grad = train.sibling_loss(torch.empty(0, 3, device=DEV), none)
+    assert (loss == 0).all() and grad.shape == (0, 3)
+
+
+# ---------------------------------------------------------------------------------------------------------------- loss
+def plain_loss(z, label, lo, hi, w, scale):
+    m, k = z.shape
+    c = np.arange(k)[None, :]
+    inside = (c >= lo[:, None]) & (c < hi[:, None])
+    y = c == label[:, None]
+    with np.errstate(invalid="ignore", over="ignore"):
+        s = np.where(y, -z, z)
+        loss = np.where(s < 0, 0.0, s) + np.log1p(np.exp(-np.abs(s)))
+        p = 1.0 / (1.0 + np.exp(-s))
+    loss = np.where(inside, loss, 0.0) * w[:, None] * scale
+    return loss.sum(0), np.where(inside, np.where(y, -p, p), 0.0) * w[:, None] * scale, np.abs(loss).sum(0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("siblings", [False, True])
+@pytest.mark.parametrize("m, k", [(1, 1), (2, 3), (7, 4), (33, 8), (300, 13), (257, 257), (64, 1000), (5000, 12), (4099, 37), (100, 1025), (3, 4100), (20000, 1)])
+def test_loss(m, k, siblings, dtype):
+    rng = np.random.default_rng(m + k)
+    z = (rng.normal(size=(m, k)) * 5).astype(np.float32)
+    lo, hi = np.zeros(m, np.int64), np.full(m, k)
+    if siblings:
+        lo = rng.integers(0, k, m)
+        hi = np.minimum(lo + rng.integers(0, 9, m), k)            # some rows train nothing
+        z[(np.arange(k) < lo[:, None]) | (np.arange(k) >= hi[:, None])] = np.nan      # never read
+    label = rng.integers(-1, k, m)
+    label = np.where(rng.random(m) < 0.7, np.clip(lo + rng.integers(0, 9, m), 0, k + 1), label)
+    w = rng.random(m).astype(np.float32) + 0.1
+    scale = 2.0 / m
+    sib = torch.from_numpy(np.stack([lo, hi], 1).astype(np.int32)).to(DEV) if siblings else None
+    loss, grad = train.sibling_loss(torch.from_numpy(z).to(DEV), torch.from_numpy(label.astype(np.int32)).to(DEV), siblings=sib,
+                                    weight=torch.from_numpy(w).to(DEV), scale=scale, grad_dtype=dtype)
+    assert grad.dtype == dtype
+    want_loss, want_grad, size = plain_loss(z.astype(np.float64), label, lo, hi, w.astype(np.float64), np.float64(np.float32(scale)))
+    # exp and log1p within 2 U of their values, a handful of other operations: 8 U a term, m additions
+    near(loss.cpu(), want_loss, (m + 8) * U * size, "loss")
+    # the same for the sigmoid: 8 U, then the rounding to the type
+    near(grad.float().cpu(), want_grad, 8 * U * np.abs(want_grad) + half_step(want_grad, dtype) * (1 + 8 * U), "grad")
+    again = train.sibling_loss(torch.from_numpy(z).to(DEV), torch.from_numpy(label.astype(np.int32)).to(DEV), siblings=sib,
+                               weight=torch.from_numpy(w).to(DEV), scale=scale, grad_dtype=dtype)
+    assert torch.equal(loss, again[0]) and torch.equal(grad, again[1])
+
+
+def test_loss_at_the_ends():
+    """Scores far out: no overflow, and the small side keeps its digits; sibling ranges reaching outside are cut."""
+    z = torch.tensor([[-math.inf, -200.0, -90.0, 0.0, 90.0, 200.0, math.inf, 3.0]], device=DEV)
+    for label in (-1, 0, 3, 6, 99):
+        loss, grad = train.sibling_loss(z, torch.tensor([label], dtype=torch.int32, device=DEV), siblings=torch.tensor([[-5, 100]], dtype=torch.int32, device=DEV))
+        want = plain_loss(z.double().cpu().numpy(), np.array([label]), np.array([0]), np.array([8]), np.ones(1), 1.0)
+        fine = np.isfinite(want[0])
+        assert np.array_equal(np.isinf(loss.cpu().numpy()), ~fine)
+        near(loss.cpu().numpy()[fine], want[0][fine], 16 * U * np.abs(want[0][fine]) + 2.0 ** -149)
+        near(grad.cpu(), want[1], 16 * U * np.abs(want[1]) + 2.0 ** -126)
+    empty = torch.tensor([[5, 2]], dtype=torch.int32, device=DEV)
+    loss, grad = train.sibling_loss(torch.full((1, 8), math.nan, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV), siblings=empty)
+    assert (loss == 0).all() and (grad == 0).all()
+
+
+@pytest.mark.parametrize("k", [12, 13])
+def test_loss_strided(k):
+    rng = np.random.default_rng(k)
+    m = 50
+    z = torch.from_numpy(rng.normal(size=(m, k + 3)).astype(np.float32)).to(DEV)
+    label = torch.from_numpy(rng.integers(0, k, m).astype(np.int32)).to(DEV)
+    out = (torch.full((k,), 7.0, device=DEV), torch.full((m, k + 2), 7.0, device=DEV, dtype=BF16))
+    train.sibling_loss(z[:, 2:2 + k], label, out=(out[0], out[1][:, 1:1 + k]))
+    want = train.sibling_loss(z[:, 2:2 + k].contiguous(), label, grad_dtype=BF16)
+    assert torch.equal(out[1][:, 1:1 + k], want[1]) and (out[1][:, 0] == 7).all() and (out[1][:, -1] == 7).all()
+    near(out[0].cpu(), want[0].double().cpu(), 60 * U * want[0].double().cpu().numpy())
+
+
+# --------------------------------------------------------------------------------------------------------------- adamw
+def plain_step(p, g, m, v, t, lr, betas, eps, decay, l1):
+    m = betas[0] * m + (1 - betas[0]) * g
+    v = betas[1] * v + (1 - betas[1]) * g * g
+    d = np.sqrt(v / (1 - betas[1] ** t)) + eps
+    move = lr * m / ((1 - betas[0] ** t) * d)
+    p = p * (1 - lr * decay) - move
+    size = np.abs(p) + np.abs(move)
+    return np.sign(p) * np.maximum(np.abs(p) - lr * l1 / d, 0), m, v, size + lr * l1 / d
+
+
+SETS = [
+    [((7500, 8), F32, F32), ((8,), F32, F32)],
+    [((1,), F32, F32)],
+    [((255,), F32, F32), ((256,), F32, F32), ((257,), F32, F32), ((1023,), F32, F32), ((1024,), F32, F32), ((1025,), F32, F32)],
+    [((145, 3), BF16, F32), ((3,), F32, F32), ((33, 7), F16, F16), ((0, 4), F32, F32), ((100, 100), BF16, BF16), ((5,), F32, BF16)],
+    [((301, 3 + j % 5), [F32, BF16, F16][j % 3], [F32, F32, F16, BF16][j % 4]) for j in range(300)],
+]
+
+
+@pytest.mark.parametrize("t", [0, 1, 99, 100000])
+@pytest.mark.parametrize("which", range(len(SETS)))
+def test_adamw_32(which, t):
+    rng = np.random.default_rng(which)
+    params, grads, values, decay, l1 = [], [], [], [], []
+    for j, (shape, kind, grad_kind) in enumerate(SETS[which]):
+        params.append(torch.from_numpy(rng.normal(size=shape).astype(np.float32)).to(DEV).to(kind))
+        grads.append(torch.from_numpy((rng.normal(size=shape) * 0.01).astype(np.float32)).to(DEV).to(grad_kind))
+        decay.append(0.1 * (j % 3))
+        l1.append(0.001 * (j % 2))
+    opt = train.AdamW(params, grads, lr=0.01, weight_decay=decay, l1=l1)
+    m = torch.from_numpy((rng.normal(size=opt.m.shape) * 0.01).astype(np.float32)).to(DEV)
+    v = torch.from_numpy((rng.random(size=opt.m.shape) * 1e-4).astype(np.float32)).to(DEV)
+    if t == 0:
+        m.zero_(), v.zero_()
+    opt.load_state(t, m, v)
+    before = [p.double().cpu().numpy() for p in params]
+    opt.step()
+    assert opt.steps == t + 1
+    for j, p in enumerate(params):
+        n, a = p.numel(), opt.state_at[j]
+        g = grads[j].double().cpu().numpy().ravel()
+        mj, vj = m[a:a + n].double().cpu().numpy(), v[a:a + n].double().cpu().numpy()
+        want, wm, wv, size = plain_step(before[j].ravel(), g, mj, vj, t + 1, 0.01, (0.9, 0.999), 1e-8, decay[j], l1[j])
+        near(opt.m[a:a + n].cpu(), wm, 3 * U * (np.abs(mj) + np.abs(g)), "m of %d" % j)
+        near(opt.v[a:a + n].cpu(), wv, 4 * U * (vj + g * g), "v of %d" % j)
+        # m is the difference of what may cancel: its error against the root, times lr, joins the 24 U of the update's own operations
+        slack = 0.01 * 3 * U * (np.abs(mj) + np.abs(g)) / ((1 - 0.9 ** (t + 1)) * (np.sqrt(wv / (1 - 0.999 ** (t + 1))) + 1e-8))
+        near(p.double().cpu().numpy().ravel(), want, 24 * U * size + slack + half_step(want, p.dtype) * (1 + 1e-4), "p of %d" % j)
+
+
+def restated_rounding(x, scale, chance):
+    y = (x / scale).astype(np.float32)
+    a = np.abs(y)
+    normal = ((a.view(np.uint32) + (chance << 4 | 8).astype(np.uint32)) & np.uint32(0xfff00000)).view(np.float32)
+    small = (np.floor(a * np.float32(512) + (chance.astype(np.float32) + np.float32(0.5)) * np.float32(2.0 ** -16)) * np.float32(2.0 ** -9)).astype(np.float32)
+    return np.copysign(np.where(a < 2.0 ** -6, small, normal), y)
+
+
+def restated_scale(x):
+    top = np.maximum(np.abs(x).reshape(-1, 256).max(1), 2.0 ** -117)
+    mant, exp = np.frexp(top)
+    return np.ldexp(np.float32(1), exp - 9 + (mant > 0.875)).astype(np.float32)
+
+
+@pytest.mark.parametrize("kind, grad_kind", [(F32, F32), (BF16, BF16), (F16, F32)])
+def test_adamw_8(kind, grad_kind):
+    """The codes are a function of the inputs: a 32-bit restatement gives the same ones, over several steps."""
+    rng = np.random.default_rng(3)
+    shapes = [(300, 7), (5,), (256,), (1024, 3), (1, 1), (1023,)]
+    params = [torch.from_numpy(rng.normal(size=s).astype(np.float32)).to(DEV).to(kind) for s in shapes]
+    grads = [torch.empty(s, device=DEV, dtype=grad_kind) for s in shapes]
+    betas, lr = (0.9, 0.99), 0.01
+    opt = train.AdamW(params, grads, lr=lr, betas=betas, state_bits=8)
+    f32 = np.float32
+    total = opt.state_values
+    codes_m, codes_v = np.zeros(total, f32), np.zeros(total, f32)
+    scale_m, scale_v = np.ones(total // 256, f32), np.ones(total // 256, f32)
+    for t in range(1, 6):
+        flat = np.zeros(total, f32)
+        for j, g in enumerate(grads):
+            g.copy_(torch.from_numpy((rng.normal(size=shapes[j]) * np.exp(3 * rng.normal(size=shapes[j]))).astype(f32)))
+            flat[opt.state_at[j]:opt.state_at[j] + g.numel()] = g.float().cpu().numpy().ravel()
+        before = [p.double().cpu().numpy().ravel() for p in params]
+        opt.step()
+        m = codes_m * np.repeat(scale_m, 256)
+        v = codes_v * np.repeat(scale_v, 256)
+        v = v * v
+        m = m * f32(betas[0]) + flat * f32(1 - betas[0])
+        v = v * f32(betas[1]) + (flat * flat) * f32(1 - betas[1])
+        root = np.sqrt(v)
+        scale_m, scale_v = restated_scale(m), restated_scale(root)
+        x = (np.arange(total, dtype=np.uint64) ^ np.uint64(t * 0x9E3779B9 & 0xffffffff)) & np.uint64(0xffffffff)
+        x = (x ^ x >> np.uint64(16)) * np.uint64(0x7FEB352D) & np.uint64(0xffffffff)
+        x = (x ^ x >> np.uint64(15)) * np.uint64(0x846CA68B) & np.uint64(0xffffffff)
+        x = (x ^ x >> np.uint64(16)).astype(np.uint32)
+        codes_m = restated_rounding(m, np.repeat(scale_m, 256), x >> np.uint32(16))
+        codes_v = restated_rounding(root, np.repeat(scale_v, 256), x & np.uint32(0xffff))
+        codes_v = np.where((root > 0) & (codes_v == 0), f32(2.0 ** -9), codes_v).astype(f32)
+        assert np.array_equal(opt.m_scale.cpu().numpy(), scale_m) and np.array_equal(opt.v_scale.cpu().numpy(), scale_v), t
+        assert np.array_equal(opt.m.float().cpu().numpy(), codes_m), t
+        assert np.array_equal(opt.v.float().cpu().numpy(), codes_v), t
+        # a code is at most one step from what it stands for: 1/8 of the value, or 2^-9 of the scale
+        deq = codes_v * np.repeat(scale_v, 256)
+        assert (np.abs(deq - root) <= np.maximum(root / 8, np.repeat(scale_v, 256) * 2.0 ** -9) * 1.0001).all()
+        for j, p in enumerate(params):
+            a, n = opt.state_at[j], p.numel()
+            d = root[a:a + n] / math.sqrt(1 - betas[1] ** t) + 1e-8
+            move = lr * m[a:a + n].astype(np.float64) / ((1 - betas[0] ** t) * d)
+            want = before[j] - move
+            near(p.double().cpu().numpy().ravel(), want, 24 * U * (np.abs(want) + np.abs(move)) + half_step(want, kind) * (1 + 1e-4), "p of %d" % j)
+
+
+def test_adamw_8_moves_on_the_mean():
+    """Without gradients the root of the second moment decays by sqrt(beta2) a step on the mean, although every step is far below half a code."""
+    n = 1 << 18
+    p, g = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)
+    opt = train.AdamW([p], [g], state_bits=8)
+    root = 100.0 + 100.0 * torch.rand(n, device=DEV)
+    opt.load_state(0, torch.zeros(n, device=DEV).to(torch.float8_e4m3fn), root.to(torch.float8_e4m3fn), torch.ones(n // 256, device=DEV), torch.ones(n // 256, device=DEV))
+    start = (opt.v.float() * opt.v_scale.repeat_interleave(256)).double()
+    steps = 100
+    for _ in range(steps):
+        opt.step()
+    end = (opt.v.float() * opt.v_scale.repeat_interleave(256)).double()
+    want = 0.999 ** (steps / 2)
+    # the sum of `steps` roundings of one value, each at most one step of 2^-3, is a bounded walk: a value strays by less than
+    # sqrt(steps) / 8 of itself (one deviation), the mean of n of them by sqrt(n) less; five deviations
+    assert abs(float(end.mean() / start.mean()) - want) < 5 * math.sqrt(steps) / 8 / math.sqrt(n)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_takes_nan_and_infinities_one_by_one(bits):
+    n = 2000
+    p, g = torch.zeros(n, device=DEV), torch.ones(n, device=DEV)
+    g[700], g[1300], g[1999] = math.nan, math.inf, 0.0
+    opt = train.AdamW([p], [g], lr=0.1, state_bits=bits)
+    opt.step()
+    opt.step()
+    bad = ~torch.isfinite(p)
+    assert bad.nonzero().flatten().tolist() == [700, 1300] and p[1999] == 0
+    # 8 bits: m and the root are off by 1/8 of themselves at most in the second step
+    near(p[:700].cpu(), np.full(700, -0.2), 1e-3 if bits == 32 else 0.1 * (9 / 7 - 1) + 1e-3)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_at_odd_addresses(bits):
+    """Tensors at addresses that no vector load may use, and what lies around them."""
+    rng = np.random.default_rng(1)
+    for kind in (F32, BF16, F16):
+        buffers = [torch.full((3000,), 7.0, device=DEV).to(kind) for _ in range(2)]
+        p, g = buffers[0][1:2002], buffers[1][3:2004]
+        p.copy_(torch.from_numpy(rng.normal(size=2001).astype(np.float32)))
+        g.copy_(torch.from_numpy(rng.normal(size=2001).astype(np.float32)))
+        q, h = p.clone(), g.clone()
+        a, b = (train.AdamW([x], [y], lr=0.01, l1=0.1, state_bits=bits) for x, y in ((p, g), (q, h)))
+        for _ in range(2):
+            a.step()
+            b.step()
+        assert torch.equal(p, q) and torch.equal(a.m.view(torch.uint8), b.m.view(torch.uint8)) and torch.equal(a.v.view(torch.uint8), b.v.view(torch.uint8))
+        assert buffers[0][0] == 7 and (buffers[0][2002:] == 7).all()
+
+
+def test_adamw_refuses_shared_memory():
+    x, y = torch.zeros(100, device=DEV), torch.zeros(100, device=DEV)
+    with pytest.raises(ValueError, match=r"params\[0\] and params\[1\] share memory"):
+        train.AdamW([x[:60], x[50:]], [y[:60], y[50:]])
+    with pytest.raises(ValueError, match="share memory"):
+        train.AdamW([x[:50]], [x[20:70]])
+    train.AdamW([x[:50], x[50:]], [y[:50], y[:50]])          # gradients may be shared
+    opt = train.AdamW([x], [y])
+    with pytest.raises(ValueError, match="states of 32 bits have none"):
+        opt.load_state(0, opt.m, opt.v, opt.m, opt.v)
+    with pytest.raises(ValueError, match="values: 256 are wanted"):
+        opt.load_state(0, opt.m[:100], opt.v)
+
+
+# ------------------------------------------------------------------------------------------------------ used together
+def problem(rng, n=400, ncol=60, k=6):
+    consensus = rng.integers(1, 5, (k, ncol))
+    label = rng.integers(0, k, n).astype(np.int32)
+    sym = np.where(rng.random((n, ncol)) < 0.1, rng.integers(0, 5, (n, ncol)), consensus[label])
+    words = -(-5 * ncol // 128) * 4
+    x = np.zeros((n, words * 32), bool)
+    x[np.arange(n)[:, None], 5 * np.arange(ncol) + sym] = True
+    bits = np.packbits(x, axis=1, bitorder="little").view(np.int32).reshape(n, words)
+    return torch.from_numpy(bits.copy()).to(DEV), x[:, :5 * ncol].astype(np.float64), label
+
+
+def test_steps_equal_the_formulas():
+    """Three steps of scores, loss, gradient and AdamW on a padded batch against the same in 64 bits; the gradient also against differences."""
+    rng = np.random.default_rng(11)
+    bits, x, label = problem(rng)
+    n, (f, k) = len(x), (x.shape[1], 6)
+    rows = np.concatenate([rng.permutation(n)[:250], np.full(6, -1)]).astype(np.int32)
+    y = label[np.where(rows < 0, 0, rows)]
+    sib = np.stack([np.where(rows < 0, 0, 0), np.where(rows < 0, 0, k)], 1).astype(np.int32)       # padding trains nothing
+    table, bias = torch.from_numpy(rng.normal(size=(f, k)).astype(np.float32) * 0.1).to(DEV), torch.zeros(k, device=DEV)
+    grads = (torch.empty_like(table), torch.empty_like(bias))
+    opt = train.AdamW([table, bias], grads, lr=0.05, eps=1e-3, weight_decay=[0.01, 0.0], l1=[1e-4, 0.0])
+    xb, real = picked(x, rows)
+    T, b = table.double().cpu().numpy(), bias.double().cpu().numpy()
+    state = [[np.zeros_like(T), np.zeros_like(T)], [np.zeros_like(b), np.zeros_like(b)]]
+    d = [torch.from_numpy(a).to(DEV) for a in (rows, y.astype(np.int32), sib)]
+
+    def total(T, b):
+        return plain_loss(np.where(real[:, None], xb @ T + b, 0.0), y, sib[:, 0], sib[:, 1], np.ones(len(rows)), 1 / 250)[0].sum()
+
+    for t in range(1, 4):
+        scores = train.row_scores(bits, table, bias, rows=d[0])
+        loss, g = train.sibling_loss(scores, d[1], siblings=d[2], scale=1 / 250)
+        train.row_scores_grad(bits, g, f, rows=d[0], out=grads)
+        z = np.where(real[:, None], xb @ T + b, 0.0)
+        want_loss, want_g, _ = plain_loss(z, y, sib[:, 0], sib[:, 1], np.ones(len(rows)), 1 / 250)
+        # after a step the tables differ by the errors of the steps before, which an eps of 1e-3 keeps below 1e-5 of the update
+        near(loss.cpu(), want_loss, 1e-4 * want_loss)
+        gT, gb = xb.T @ want_g, want_g.sum(0)
+        near(grads[0].cpu(), gT, 1e-5 + 1e-4 * np.abs(gT))
+        near(grads[1].cpu(), gb, 1e-5 + 1e-4 * np.abs(gb))
+        if t == 1:
+            for _ in range(3):
+                D, e, h = rng.normal(size=T.shape), rng.normal(size=b.shape), 1e-5
+                slope = (total(T + h * D, b + h * e) - total(T - h * D, b - h * e)) / (2 * h)
+                mine = (grads[0].double().cpu().numpy() * D).sum() + (grads[1].double().cpu().numpy() * e).sum()
+                assert abs(mine - slope) <= 1e-5 * (np.abs(gT * D).sum() + np.abs(gb * e).sum())
+        opt.step()
+        T, *state[0] = plain_step(T, gT, *state[0], t, 0.05, (0.9, 0.999), 1e-3, 0.01, 1e-4)[:3]
+        b, *state[1] = plain_step(b, gb, *state[1], t, 0.05, (0.9, 0.999), 1e-3, 0.0, 0.0)[:3]
+        near(table.cpu(), T, 1e-4)
+        near(bias.cpu(), b, 1e-4)
+
+
+@pytest.mark.parametrize("bits_", [32, 8])
+def test_a_captured_training_step_counts_on(bits_):
+    """A whole step recorded into a HIP graph and replayed, with eager work of the same kind between the replays: each replay is the eager step."""
+    rng = np.random.default_rng(2)
+    bits, x, label = problem(rng, n=700, ncol=150, k=9)
+    f, k = x.shape[1], 9
+    start = torch.from_numpy(rng.normal(size=(f, k)).astype(np.float32) * 0.1).to(DEV)
+
+    def program():
+        table, bias = start.clone(), torch.zeros(k, device=DEV)
+        grads = (torch.empty_like(table), torch.empty_like(bias))
+        rows, lab = torch.zeros(600, dtype=torch.int32, device=DEV), torch.zeros(600, dtype=torch.int32, device=DEV)
+        opt = train.AdamW([table, bias], grads, lr=0.01, state_bits=bits_)
+
+        def step():
+            scores = train.row_scores(bits, table, bias, rows=rows)
+            loss, g = train.sibling_loss(scores, lab, scale=1 / 600, grad_dtype=BF16)
+            train.row_scores_grad(bits, g, f, rows=rows, out=grads)
+            opt.step()
+            return loss, scores
+
+        return table, bias, rows, lab, opt, step
+
+    eager, graphed, other = program(), program(), program()
+    program()[5]()                                           # the first call of a kernel loads its code
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    for prog in (graphed, other):                            # two graphs, each with a workspace of its own
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = prog[5]()
+        graphs.append((graph, out))
+    torch.cuda.synchronize()
+    for t in range(5):
+        pick = rng.integers(0, 700, 600).astype(np.int32)
+        for prog in (eager, graphed, other):
+            prog[2].copy_(torch.from_numpy(pick))
+            prog[3].copy_(torch.from_numpy(label[pick]))
+        loss, scores = eager[5]()
+        graphs[0][0].replay()
+        graphs[1][0].replay()
+        torch.cuda.synchronize()
+        for prog, (_, out) in zip((graphed, other), graphs):
+            assert torch.equal(out[0], loss) and torch.equal(out[1], scores), t
+            assert torch.equal(prog[0], eager[0]) and torch.equal(prog[1], eager[1]), t
+            assert torch.equal(prog[4].m.view(torch.uint8), eager[4].m.view(torch.uint8)) and prog[4].steps == t + 1
+
+
+def test_on_two_streams_at_once():
+    rng = np.random.default_rng(8)
+    bits, x = packed(rng, 900, 1500)
+    tables = [torch.from_numpy(rng.normal(size=(1500, k)).astype(np.float32)).to(DEV) for k in (9, 150)]
+    grads = [torch.from_numpy(rng.normal(size=(900, k)).astype(np.float32)).to(DEV) for k in (9, 150)]
+    want = [(train.row_scores(bits, t), train.row_scores_grad(bits, g, 1500)[0]) for t, g in zip(tables, grads)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in tables]
+    got = [[], []]
+    for _ in range(10):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[j].append((train.row_scores(bits, tables[j]), train.row_scores_grad(bits, grads[j], 1500)[0]))
+    torch.cuda.synchronize()
+    for j in range(2):
+        for a, b in got[j]:
+            assert torch.equal(a, want[j][0]) and torch.equal(b, want[j][1])
+
+
+def test_fit_siblings_feeds_the_walk():
+    """fit_siblings on rows of the package's own encoder gives coefficients that its database takes and classifies with; its first step is the formula's."""
+    from stag_amd.engine import Database
+    rng = np.random.default_rng(4)
+    ncol, k, n = 60, 4, 240
+    consensus = rng.integers(0, 4, (k, ncol))
+    label = rng.integers(0, k, n)
+    sym = np.where(rng.random((n, ncol)) < 0.05, rng.integers(0, 4, (n, ncol)), consensus[label])
+    reads = ["".join(r) for r in np.array(list("ACGT"))[sym]]
+    names = ["a", "b", "c", "d"]
+    taxonomy = {"tree_root": names, **{x: [] for x in names}}
+    rank = {"0": np.array([0.0, 1.0])}
+    with Database.from_dicts(taxonomy, rank, {x: np.zeros(1 + 5 * ncol) for x in names}, n_features=5 * ncol) as db:
+        bits = db.encode_a2m(reads)[0]
+    x = np.unpackbits(bits.view(np.uint8), axis=1, bitorder="little")[:, :5 * ncol].astype(np.float64)
+    one = train.fit_siblings(bits, label, k, 5 * ncol, steps=1, lr=0.1)
+    g = (0.5 - (label[:, None] == np.arange(k))) / n
+    full = np.concatenate([g.sum(0)[:, None], (x.T @ g).T], 1)
+    assert one.shape == (k, 1 + 5 * ncol) and one.dtype == np.float64
+    # the first step moves by lr g / (|g| + eps); a token that no row or every class has alike has a gradient of 0, or one that is rounding
+    sure = np.abs(full) > 1e-6
+    near(one[sure], (-0.1 * full / (np.abs(full) + 1e-8))[sure], 1e-3)
+    for options in (dict(steps=30, lr=0.05, l1=1e-3), dict(steps=30, batch=64, table_dtype=BF16, state_bits=8, weight=np.ones(n, np.float32))):
+        coefficients = train.fit_siblings(bits, label, k, 5 * ncol, **options)
+        assert np.isfinite(coefficients).all()
+        with Database.from_dicts(taxonomy, rank, dict(zip(names, coefficients)), n_features=5 * ncol) as db:
+            res = db.classify_a2m(reads)
+        scores = x @ coefficients[:, 1:].T + coefficients[:, 0]
+        assert (res.status == 0).all()
+        got = np.array([names.index(db.names[j]) for j in res.path_node[:, 0]])
+        assert np.array_equal(got, scores.argmax(1))           # the walk answers with what was learned
