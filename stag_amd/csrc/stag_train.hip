@@ -53,54 +53,424 @@ __device__ __forceinline__ const uint32_t *row_of(const uint32_t *bits, int64_t 
 // ------------------------------------------------------------------------------------------------------------------
 // scores and their gradient
 // ------------------------------------------------------------------------------------------------------------------
-// one thread per score
+// Both are products of a matrix of zeros and ones, held as bits, with a matrix of coefficients or gradients:
+//   scores  S[i][c] = sum_f x[i][f] T[f][c]        rows of the result: batch rows,  summed over: features
+//   grad    D[f][c] = sum_i x[i][f] G[i][c]        rows of the result: features,    summed over: batch rows
+// and run on the matrix cores although four of five bits are 0: 1,500 additions a score fed from LDS or L2 one by one take longer than
+// 7,500 multiply-adds at the matrix cores' rate.  A bit becomes a 16-bit operand by one shift and one mask: bit 14 alone is 2.0, in bf16
+// and in f16, and a mask of two such bits makes a pair; the factor 2 is taken out of the result.  A zero or one is exact
+// in 16 bits; a 32-bit coefficient is cut into three bf16 pieces of 8 bits each, which together are the coefficient,
+// and multiplied piece by piece into the same 32-bit sums.  16-bit coefficients go in as they are.
+//
+// An infinity or NaN must not meet a zero bit in a product: such values go in as 0 and, where there were any, are added
+// afterwards to the results whose rows have the bit (slow, and only then).
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+
+struct ProductArgs {
+    const uint32_t *bits;
+    int64_t n, row_stride;
+    const int32_t *rows;
+    int64_t m;
+    const void *mat;            // table or gradient
+    int64_t mat_stride;
+    const float *bias;          // scores: added
+    float *out, *bias_out;      // bias_out: grad: column sums
+    int64_t out_stride;
+    float *part;                // more than one part: raw sums [parts][result rows][k], then column sums [parts][k]
+    int32_t n_features, words, k;
+    int32_t steps, steps_per_part;      // in units of 4 K-steps (scores), 1 K-step (grad)
+    float scale;
+};
+
+template <int TYPE> struct Raw { typedef uint16_t type; };
+template <> struct Raw<STAG_F32> { typedef uint32_t type; };
+
+template <int TYPE> __device__ __forceinline__ bool not_finite(uint32_t raw) {
+    return TYPE == STAG_F32 ? (raw & 0x7f800000u) == 0x7f800000u : TYPE == STAG_BF16 ? (raw & 0x7f80u) == 0x7f80u : (raw & 0x7c00u) == 0x7c00u;
+}
+template <int TYPE> __device__ __forceinline__ float value_of(uint32_t raw) {
+    return TYPE == STAG_F32 ? __uint_as_float(raw) : TYPE == STAG_BF16 ? __uint_as_float(raw << 16) : (float)__builtin_bit_cast(f16, (uint16_t)raw);
+}
+// the larger of two magnitudes, as whole numbers: not finite if any of them is not
+template <int TYPE> __device__ __forceinline__ uint32_t magnitude(uint32_t raw) { return raw & (TYPE == STAG_F32 ? 0x7fffffffu : 0x7fffu); }
+
+__device__ __forceinline__ uint32_t high_halves(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
+
+// the 8 operands of K-step part s: bits 4s .. 4s+3 and 4s+16 .. 4s+19 of x, as 2.0 or 0
+__device__ __forceinline__ u32x4 operands(uint32_t x, int s) {
+    u32x4 a;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] = __builtin_amdgcn_alignbit(x, x, (4 * s + j + 18) & 31) & 0x40004000u;
+    return a;
+}
+
+// 32 x 32 bits in each half of the wave: lane r held row r, lane f comes to hold column f (bit r = row r)
+__device__ __forceinline__ uint32_t transposed(uint32_t x, int lane) {
+#define STAG_EXCHANGE(J, LOW)                                                                    \
+    {                                                                                            \
+        const uint32_t y = (uint32_t)__builtin_amdgcn_ds_swizzle((int)x, (J) << 10 | 0x1f);      \
+        const uint32_t keep = lane & (J) ? ~(LOW) : (LOW);                                       \
+        const uint32_t z = __builtin_amdgcn_alignbit(y, y, lane & (J) ? (J) : 32 - (J));         \
+        x = (x & keep) | (z & ~keep);                                                            \
+    }
+    STAG_EXCHANGE(16, 0x0000ffffu)
+    STAG_EXCHANGE(8, 0x00ff00ffu)
+    STAG_EXCHANGE(4, 0x0f0f0f0fu)
+    STAG_EXCHANGE(2, 0x33333333u)
+    STAG_EXCHANGE(1, 0x55555555u)
+#undef STAG_EXCHANGE
+    return x;
+}
+
+// A workgroup of four waves makes 4 MT x 32 rows of the result by NT x 32 columns; a wave its own MT row tiles.  A K-step
+// is 64 terms of the sum: two words of bits, one for each half of the wave (the matrix instruction takes 8 terms from
+// each half), in four instructions of 16 terms.  The workgroup loads the K-step's 64 x 32 NT coefficients, cuts them into pieces and
+// stores them to LDS in operand order; two buffers, the next one's loads in flight while the matrix cores work on this one.
+template <int TYPE, bool GRAD, int MT, int NT>
+__global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
+    typedef typename Raw<TYPE>::type raw_t;
+    constexpr int P = TYPE == STAG_F32 ? 3 : 1, COLS = 32 * NT, PASSES = NT, GROUPS = 256 / COLS;
+    __shared__ u32x4 lds[2][P][8][COLS];
+    __shared__ float sums[GRAD ? 256 : 1];
+    __shared__ int found;
+    __shared__ uint8_t padding[GRAD ? 1 : 128 * MT];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int64_t tile0 = ((int64_t)blockIdx.x * 4 + wave) * MT;           // this wave's first row tile
+    const int col = threadIdx.x % COLS, group = threadIdx.x / COLS;
+    const int c0 = blockIdx.y * COLS, c = c0 + col < a.k ? c0 + col : a.k - 1;
+    const bool c_ok = c0 + col < a.k;
+    const int64_t limit = GRAD ? a.m : a.n_features;                       // terms of the sum
+    const int first = blockIdx.z * a.steps_per_part;
+    const int last = min(first + a.steps_per_part, a.steps);
+    const raw_t *mat = (const raw_t *)a.mat + c;
+    if (threadIdx.x == 0) found = 0;
+    __syncthreads();
+
+    // the term that stands at place r (0..63) of K-step ks
+    auto term = [&](int ks, int r) -> int64_t {
+        if constexpr (GRAD) return (int64_t)ks * 64 + r;
+        return 32 * ((int64_t)(ks >> 2) * 8 + (r >> 5) * 4 + (ks & 3)) + (r & 31);
+    };
+
+    f32x16 acc[MT][NT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[t][n] = (f32x16)(0.f);
+    float column_sum = 0.f;
+
+    raw_t b[PASSES][8];
+    // `real`: which of the K-step's terms there are; the others are zeros, whatever the memory holds
+    auto load_b = [&](int ks, uint64_t real) {
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int g = group + i * GROUPS, r0 = 32 * (g & 1) + 4 * (g >> 1);
+            if (real == ~0ull) {
+                const raw_t *p = mat + term(ks, r0) * a.mat_stride;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) b[i][q] = p[((q >> 1) + 16 * (q & 1)) * a.mat_stride];
+            } else {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const int r = r0 + (q >> 1) + 16 * (q & 1);
+                    const int64_t at = term(ks, r);
+                    b[i][q] = mat[(at < limit ? at : limit - 1) * a.mat_stride];
+                    if (!(real >> r & 1)) b[i][q] = 0;
+                }
+            }
+        }
+    };
+    auto store_b = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int g = group + i * GROUPS;
+            if (!c_ok) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) b[i][q] = 0;
+            }
+            if constexpr (GRAD) {
+                if (blockIdx.x == 0) {
+                    float s = 0.f;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) s += value_of<TYPE>(b[i][q]);
+                    column_sum += s;
+                }
+            }
+            uint32_t top = 0;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) top = max(top, magnitude<TYPE>(b[i][q]));
+            if (not_finite<TYPE>(top)) {
+                found = 1;
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (not_finite<TYPE>(b[i][q])) b[i][q] = 0;
+            }
+            if constexpr (TYPE == STAG_F32) {
+                uint32_t x[8], y[8], z[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    x[q] = b[i][q];
+                    const float left = __uint_as_float(x[q]) - __uint_as_float(x[q] & 0xffff0000u);        // exact: the low 16 bits
+                    y[q] = __float_as_uint(left);
+                    z[q] = __float_as_uint(left - __uint_as_float(y[q] & 0xffff0000u));                    // exact: the low 8 bits
+                }
+                u32x4 p0, p1, p2;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    p0[j] = high_halves(x[2 * j], x[2 * j + 1]);
+                    p1[j] = high_halves(y[2 * j], y[2 * j + 1]);
+                    p2[j] = high_halves(z[2 * j], z[2 * j + 1]);
+                }
+                lds[buf][0][g][col] = p0;
+                lds[buf][P > 1 ? 1 : 0][g][col] = p1;
+                lds[buf][P > 2 ? 2 : 0][g][col] = p2;
+            } else {
+                u32x4 p0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) p0[j] = (uint32_t)b[i][2 * j] | (uint32_t)b[i][2 * j + 1] << 16;
+                lds[buf][0][g][col] = p0;
+            }
+        }
+    };
+    auto multiply = [&](int buf, const uint32_t *x) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            u32x4 w[MT];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) w[t] = operands(x[t], s);
+#pragma unroll
+            for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const u32x4 v = lds[buf][p][2 * s + half][32 * n + (lane & 31)];
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        if constexpr (TYPE == STAG_F16)
+                            acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, w[t]), __builtin_bit_cast(f16x8, v), acc[t][n], 0, 0, 0);
+                        else
+                            acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w[t]), __builtin_bit_cast(bf16x8, v), acc[t][n], 0, 0, 0);
+                    }
+                }
+        }
+    };
+
+    if constexpr (!GRAD) {
+        const uint32_t *row[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int64_t i = (tile0 + t) * 32 + (lane & 31);
+            row[t] = i < a.m ? row_of(a.bits, a.n, a.row_stride, a.rows, i) : nullptr;
+        }
+        auto load_x = [&](int sb, u32x4 *x) {
+            const int w = sb * 8 + half * 4;
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                x[t] = (u32x4)(0u);
+                if (row[t] && w < a.words) x[t] = *(const u32x4 *)(row[t] + w);
+            }
+        };
+        auto real_of = [&](int ks) -> uint64_t {
+            uint64_t mask = 0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int64_t there = limit - term(ks, 32 * h);
+                mask |= (there >= 32 ? 0xffffffffull : there > 0 ? (1ull << there) - 1 : 0ull) << (32 * h);
+            }
+            return mask;
+        };
+        u32x4 x[MT], next[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+            if (half == 0) padding[(wave * MT + t) * 32 + lane] = row[t] == nullptr;
+        load_x(first, x);
+        load_b(first * 4, real_of(first * 4));
+        store_b(0);
+        __syncthreads();
+#pragma unroll 1
+        for (int ks = first * 4; ks < last * 4; ++ks) {
+            const bool more = ks + 1 < last * 4;
+            if ((ks & 3) == 0 && ks + 4 < last * 4) load_x((ks >> 2) + 1, next);
+            if (more) load_b(ks + 1, real_of(ks + 1));
+            uint32_t w[MT];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                w[t] = x[t][0];
+                x[t] = (ks & 3) == 3 ? next[t] : __builtin_shufflevector(x[t], x[t], 1, 2, 3, 0);
+            }
+            multiply(ks & 1, w);
+            if (more) store_b((ks & 1) ^ 1);
+            __syncthreads();
+        }
+    } else {
+        static_assert(!GRAD || MT == 4, "a lane loads the words of its wave's row tiles at once");
+        const int64_t w0 = tile0 < a.words ? tile0 : a.words - 4;
+        auto load_row = [&](int ks) -> const uint32_t * {
+            const int64_t i = (int64_t)ks * 64 + lane;
+            return i < a.m ? row_of(a.bits, a.n, a.row_stride, a.rows, i) : nullptr;
+        };
+        auto load_x = [&](const uint32_t *r) { return r ? *(const u32x4 *)(r + w0) : (u32x4)(0u); };
+        const uint32_t *row = load_row(first);
+        u32x4 x = load_x(row), next = (u32x4)(0u);
+        load_b(first, __ballot(row != nullptr));
+        const uint32_t *ahead = first + 1 < last ? load_row(first + 1) : nullptr;
+        store_b(0);
+        __syncthreads();
+#pragma unroll 1
+        for (int ks = first; ks < last; ++ks) {
+            const bool more = ks + 1 < last;
+            if (more) {
+                next = load_x(ahead);
+                load_b(ks + 1, __ballot(ahead != nullptr));
+                if (ks + 2 < last) ahead = load_row(ks + 2);
+            }
+            uint32_t w[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) w[t] = transposed(x[t], lane);
+            multiply((ks - first) & 1, w);
+            if (more) store_b(((ks - first) & 1) ^ 1);
+            __syncthreads();
+            x = next;
+        }
+    }
+
+    const int64_t out_rows = GRAD ? a.n_features : a.m;
+    auto row_at = [&](int t, int i) -> int64_t { return (tile0 + t) * 32 + 8 * (i >> 2) + 4 * half + (i & 3); };
+    const bool whole = gridDim.z == 1;
+    const float scale = 0.5f * a.scale;
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int64_t r = row_at(t, i);
+            if (r >= out_rows) continue;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int cc = c0 + 32 * n + (lane & 31);
+                if (cc >= a.k) continue;
+                if (!whole)
+                    a.part[((int64_t)blockIdx.z * out_rows + r) * a.k + cc] = acc[t][n][i];
+                else if (a.out)
+                    a.out[r * a.out_stride + cc] =
+                        !GRAD && padding[(wave * MT + t) * 32 + 8 * (i >> 2) + 4 * half + (i & 3)] ? 0.f : acc[t][n][i] * scale + (!GRAD && a.bias ? a.bias[cc] : 0.f);
+            }
+        }
+    if (found) {       // the terms left out above, to the results whose rows have the bit
+        __syncthreads();
+        for (int e = threadIdx.x; e < 128 * MT * COLS; e += 256) {
+            const int64_t r = (int64_t)blockIdx.x * 128 * MT + e / COLS;
+            const int cc = c0 + e % COLS;
+            if (r >= out_rows || cc >= a.k || (whole && !a.out)) continue;
+            float *to = whole ? a.out + r * a.out_stride + cc : a.part + ((int64_t)blockIdx.z * out_rows + r) * a.k + cc;
+            const int64_t end = min(limit, term(last * (GRAD ? 1 : 4), 0));
+            float s = 0.f;
+            for (int64_t at = term(first * (GRAD ? 1 : 4), 0); at < end; ++at) {
+                const raw_t v = ((const raw_t *)a.mat)[at * a.mat_stride + cc];
+                if (!not_finite<TYPE>(v)) continue;
+                const int64_t bit = GRAD ? r : at;
+                const uint32_t *words = row_of(a.bits, a.n, a.row_stride, a.rows, GRAD ? at : r);
+                if (words && (words[bit >> 5] >> (bit & 31) & 1u)) s += value_of<TYPE>(v);
+            }
+            if (!(s == 0.f)) *to += whole ? s * a.scale : s;
+        }
+    }
+    if constexpr (GRAD) {
+        if (blockIdx.x == 0) {
+            sums[threadIdx.x] = column_sum;
+            __syncthreads();
+            if (group == 0 && c_ok) {
+                float s = 0.f;
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g) s += sums[g * COLS + col];
+                if (!whole)
+                    a.part[(int64_t)gridDim.z * out_rows * a.k + (int64_t)blockIdx.z * a.k + c] = s;
+                else if (a.bias_out)
+                    a.bias_out[c] = s;
+            }
+        }
+    }
+}
+
+// adds up the parts, in order
+template <bool GRAD>
+__global__ __launch_bounds__(256) void k_join(ProductArgs a, int parts, int64_t out_rows) {
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, all = out_rows * a.k;
+    if (at < all) {
+        float s = 0.f;
+        for (int p = 0; p < parts; ++p) s += a.part[p * all + at];
+        const int64_t r = at / a.k;
+        const int c = (int)(at - r * a.k);
+        const bool padding = !GRAD && a.rows && !row_of(a.bits, a.n, a.row_stride, a.rows, r);
+        if (a.out) a.out[r * a.out_stride + c] = padding ? 0.f : s * (0.5f * a.scale) + (!GRAD && a.bias ? a.bias[c] : 0.f);
+    } else if (GRAD && at < all + a.k && a.bias_out) {
+        float s = 0.f;
+        for (int p = 0; p < parts; ++p) s += a.part[parts * all + (int64_t)p * a.k + (at - all)];
+        a.bias_out[at - all] = s;
+    }
+}
+
+// Few rows: the lookups themselves.  A workgroup makes one row of scores, `cw` columns of it (a power of two up to 64): it
+// lists the row's tokens in LDS, 256 words at a time, and its 1024 / cw column groups take the tokens in turn.
+constexpr int LOOKUP_WORDS = 256;
 template <typename T>
-__global__ __launch_bounds__(256) void k_scores(const uint32_t *bits, int64_t n, int64_t row_stride, int n_features, const int32_t *rows,
-                                                int64_t m, const T *table, int64_t table_stride, const float *bias, int k,
-                                                float scale, float *scores, int64_t score_stride) {
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= m * k) return;
-    const int64_t i = at / k;
-    const int c = (int)(at - i * k);
+__global__ __launch_bounds__(1024) void k_lookup(const uint32_t *bits, int64_t n, int64_t row_stride, int n_features, const int32_t *rows, const T *table,
+                                                 int64_t table_stride, const float *bias, int k, float scale, float *scores, int64_t score_stride,
+                                                 int cw_log) {
+    __shared__ uint16_t token[LOOKUP_WORDS * 32];
+    __shared__ int before[5];
+    __shared__ float part[1024];
+    const int64_t i = blockIdx.x;
+    const int cw = 1 << cw_log, c = blockIdx.y * cw + (threadIdx.x & (cw - 1)), slot = threadIdx.x >> cw_log, slots = 1024 >> cw_log;
     const uint32_t *row = row_of(bits, n, row_stride, rows, i);
     float s = 0.f;
     if (row) {
-        for (int w = 0; 32 * w < n_features; ++w) {
-            float part = 0.f;
-            for (uint32_t x = row[w]; x; x &= x - 1) {
-                const int f = 32 * w + __builtin_ctz(x);
-                if (f < n_features) part += (float)table[(int64_t)f * table_stride + c];
+        const int words = (n_features + 31) / 32;
+        for (int w0 = 0; w0 < words; w0 += LOOKUP_WORDS) {
+            __syncthreads();
+            uint32_t x = 0;
+            int count = 0, inside = 0;
+            if (threadIdx.x < LOOKUP_WORDS) {
+                const int w = w0 + threadIdx.x;
+                if (w < words) x = row[w];
+                if (32 * (w + 1) > n_features) x &= w < words ? 0xffffffffu >> (32 * words - n_features) : 0u;
+                count = __builtin_popcount(x);
+                inside = count;
+#pragma unroll
+                for (int o = 1; o < 64; o <<= 1) {
+                    const int y = __shfl_up(inside, o);
+                    if ((threadIdx.x & 63) >= o) inside += y;
+                }
+                if ((threadIdx.x & 63) == 63) before[threadIdx.x >> 6] = inside;
             }
-            s += part;
-        }
-        s = s * scale + (bias ? bias[c] : 0.f);
-    }
-    scores[i * score_stride + c] = s;
-}
-
-// one thread per coefficient; feature n_features stands for the bias, which every row has
-template <typename T>
-__global__ __launch_bounds__(256) void k_grad(const uint32_t *bits, int64_t n, int64_t row_stride, int n_features, const int32_t *rows,
-                                              int64_t m, const T *grad, int64_t grad_stride, int k, float scale, float *table_grad,
-                                              int64_t table_grad_stride, float *bias_grad) {
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= ((int64_t)n_features + 1) * k) return;
-    const int f = (int)(at / k), c = (int)(at - (int64_t)f * k);
-    float s = 0.f, part = 0.f;
-    for (int64_t i = 0; i < m; ++i) {
-        const uint32_t *row = row_of(bits, n, row_stride, rows, i);
-        if (row && (f == n_features || (row[f >> 5] >> (f & 31) & 1u))) part += (float)grad[i * grad_stride + c];
-        if ((i & 31) == 31) {
-            s += part;
-            part = 0.f;
+            __syncthreads();
+            const int b0 = before[0], b1 = before[1], b2 = before[2], total = b0 + b1 + b2 + before[3];
+            if (threadIdx.x < LOOKUP_WORDS) {
+                const int wv = threadIdx.x >> 6;
+                int at = inside - count + (wv > 0 ? b0 : 0) + (wv > 1 ? b1 : 0) + (wv > 2 ? b2 : 0);
+                for (; x; x &= x - 1) token[at++] = (uint16_t)(threadIdx.x * 32 + __builtin_ctz(x));
+            }
+            __syncthreads();
+            if (c < k) {
+                const T *from = table + (int64_t)w0 * 32 * table_stride + c;
+                int t = slot;
+                for (; t + 3 * slots < total; t += 4 * slots) {
+                    float v[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) v[u] = (float)from[(int64_t)token[t + u * slots] * table_stride];
+                    s += (v[0] + v[1]) + (v[2] + v[3]);
+                }
+                for (; t < total; t += slots) s += (float)from[(int64_t)token[t] * table_stride];
+            }
         }
     }
-    s += part;
-    if (f < n_features) {
-        if (table_grad) table_grad[(int64_t)f * table_grad_stride + c] = s * scale;
-    } else if (bias_grad) {
-        bias_grad[c] = s;
+    part[threadIdx.x] = s;
+    for (int half = slots / 2; half; half >>= 1) {
+        __syncthreads();
+        if (slot < half) part[threadIdx.x] += part[threadIdx.x + (half << cw_log)];
     }
+    if (slot == 0 && c < k) scores[i * score_stride + c] = row ? part[threadIdx.x] * scale + (bias ? bias[c] : 0.f) : 0.f;
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -398,23 +768,65 @@ int check_matrix(const char *name, const void *p, int type, int64_t stride, int3
         if (rc_ != STAG_OK) return rc_; \
     } while (0)
 
-template <typename T>
-int scores_typed(const uint32_t *d_bits, int64_t n, int64_t row_stride, int32_t n_features, const int32_t *d_rows, int64_t m, const void *d_table,
-                 int64_t table_stride, const float *d_bias, int32_t k, float scale, float *d_scores, int64_t score_stride, hipStream_t st) {
-    REQUIRE(m * k < (int64_t)1 << 39, "m * k is too large");
-    k_scores<T><<<(unsigned)ceil_div(m * k, 256), 256, 0, st>>>(d_bits, n, row_stride, n_features, d_rows, m, (const T *)d_table, table_stride, d_bias, k,
-                                                               scale, d_scores, score_stride);
-    HIP_TRY(hipGetLastError());
+// how a product is cut up
+struct Plan {
+    bool lookup;
+    int mt, nt, steps, per_part, parts;
+    int64_t row_blocks, col_blocks, out_rows, work_bytes;
+};
+
+Plan product_plan(bool grad, int64_t m, int32_t n_features, int32_t k) {
+    Plan p = {};
+    p.out_rows = grad ? n_features : m;
+    if (m == 0) return p;
+    p.lookup = !grad && m <= 64;
+    p.nt = k <= 32 ? 1 : 2;
+    p.mt = grad || ceil_div(m, 512) * ceil_div(k, 32 * p.nt) >= 128 ? 4 : 1;
+    p.row_blocks = ceil_div(p.out_rows, 128 * p.mt);
+    p.col_blocks = ceil_div(k, 32 * p.nt);
+    p.steps = (int)(grad ? ceil_div(m, 64) : ceil_div(n_features, 256));
+    const int64_t blocks = p.row_blocks * p.col_blocks, wanted = blocks < 512 ? 512 / blocks : 1, most = grad ? ceil_div(p.steps, 2) : p.steps;
+    const int64_t parts = wanted < most ? wanted : most;
+    p.per_part = p.steps ? (int)ceil_div(p.steps, parts) : 0;
+    p.parts = p.steps ? (int)ceil_div(p.steps, p.per_part) : 0;
+    if (p.parts > 1 && !p.lookup) p.work_bytes = ((int64_t)p.parts * (p.out_rows + (grad ? 1 : 0)) * k) * 4;
+    return p;
+}
+
+template <int TYPE, bool GRAD>
+int product(const Plan &p, ProductArgs a, hipStream_t st) {
+    a.words = (int32_t)ceil_div(a.n_features, 128) * 4;
+    a.steps = p.steps;
+    a.steps_per_part = p.per_part;
+    REQUIRE(p.row_blocks < (int64_t)1 << 31 && ceil_div((p.out_rows + 1) * a.k, 256) < (int64_t)1 << 31, "%lld rows of %d columns are too many",
+            (long long)p.out_rows, a.k);
+    if (p.parts) {
+        const dim3 grid((unsigned)p.row_blocks, (unsigned)p.col_blocks, (unsigned)p.parts);
+        if (p.mt == 4 && p.nt == 2)
+            k_product<TYPE, GRAD, 4, 2><<<grid, 256, 0, st>>>(a);
+        else if (p.mt == 4)
+            k_product<TYPE, GRAD, 4, 1><<<grid, 256, 0, st>>>(a);
+        else if constexpr (!GRAD) {
+            if (p.nt == 2)
+                k_product<TYPE, GRAD, 1, 2><<<grid, 256, 0, st>>>(a);
+            else
+                k_product<TYPE, GRAD, 1, 1><<<grid, 256, 0, st>>>(a);
+        }
+        HIP_TRY(hipGetLastError());
+    }
+    if (p.parts != 1) {      // an empty sum has no parts
+        k_join<GRAD><<<(unsigned)ceil_div((p.out_rows + (GRAD ? 1 : 0)) * a.k, 256), 256, 0, st>>>(a, p.parts, p.out_rows);
+        HIP_TRY(hipGetLastError());
+    }
     return STAG_OK;
 }
 
 template <typename T>
-int grad_typed(const uint32_t *d_bits, int64_t n, int64_t row_stride, int32_t n_features, const int32_t *d_rows, int64_t m, const void *d_grad,
-               int64_t grad_stride, int32_t k, float scale, float *d_table_grad, int64_t table_grad_stride, float *d_bias_grad, hipStream_t st) {
-    const int64_t blocks = ceil_div(((int64_t)n_features + 1) * k, 256);
-    REQUIRE(blocks < (int64_t)1 << 31, "n_features * k is too large");
-    k_grad<T><<<(unsigned)blocks, 256, 0, st>>>(d_bits, n, row_stride, n_features, d_rows, m, (const T *)d_grad, grad_stride, k, scale, d_table_grad,
-                                               table_grad_stride, d_bias_grad);
+int lookup(const ProductArgs &a, hipStream_t st) {
+    int cw_log = 0;
+    while (cw_log < 6 && (1 << cw_log) < a.k) ++cw_log;
+    k_lookup<T><<<dim3((unsigned)a.m, (unsigned)ceil_div(a.k, 1 << cw_log)), 1024, 0, st>>>(a.bits, a.n, a.row_stride, a.n_features, a.rows, (const T *)a.mat,
+                                                                                          a.mat_stride, a.bias, a.k, a.scale, a.out, a.out_stride, cw_log);
     HIP_TRY(hipGetLastError());
     return STAG_OK;
 }
@@ -462,12 +874,12 @@ const char *stag_train_last_error(void) { return g_err; }
 
 int64_t stag_row_scores_workspace(int64_t m, int32_t n_features, int32_t k, int32_t type) {
     TRY(check_rows(nullptr, 0, (((int64_t)n_features + 127) / 128) * 4, n_features, (const int32_t *)16, m, k, type));
-    return 0;
+    return product_plan(false, m, n_features, k).work_bytes;
 }
 
 int64_t stag_row_scores_grad_workspace(int64_t m, int32_t n_features, int32_t k, int32_t type) {
     TRY(check_rows(nullptr, 0, (((int64_t)n_features + 127) / 128) * 4, n_features, (const int32_t *)16, m, k, type));
-    return 0;
+    return product_plan(true, m, n_features, k).work_bytes;
 }
 
 int stag_row_scores_dev(const uint32_t *d_bits, int64_t n, int64_t row_stride, int32_t n_features, const int32_t *d_rows, int64_t m, const void *d_table,
@@ -478,16 +890,21 @@ int stag_row_scores_dev(const uint32_t *d_bits, int64_t n, int64_t row_stride, i
     if (m == 0) return STAG_OK;
     TRY(check_matrix("d_scores", d_scores, STAG_F32, score_stride, k));
     REQUIRE(aligned(d_bias, 4), "d_bias is not aligned to its type");
-    const int64_t need = stag_row_scores_workspace(m, n_features, k, type);
-    REQUIRE(work_bytes >= need && (need == 0 || (d_work && aligned(d_work, 256))), "d_work: %lld bytes, 256-byte aligned, are wanted", (long long)need);
+    const Plan p = product_plan(false, m, n_features, k);
+    REQUIRE(work_bytes >= p.work_bytes && (p.work_bytes == 0 || (d_work && aligned(d_work, 256))), "d_work: %lld bytes, 256-byte aligned, are wanted",
+            (long long)p.work_bytes);
+    ProductArgs a = {};
+    a.bits = d_bits, a.n = n, a.row_stride = row_stride, a.rows = d_rows, a.m = m, a.n_features = n_features;
+    a.mat = d_table, a.mat_stride = table_stride, a.bias = d_bias, a.k = k, a.scale = scale, a.out = d_scores, a.out_stride = score_stride;
+    a.part = (float *)d_work;
     hipStream_t st = (hipStream_t)stream;
     switch (type) {
     case STAG_F32:
-        return scores_typed<float>(d_bits, n, row_stride, n_features, d_rows, m, d_table, table_stride, d_bias, k, scale, d_scores, score_stride, st);
+        return p.lookup ? lookup<float>(a, st) : product<STAG_F32, false>(p, a, st);
     case STAG_BF16:
-        return scores_typed<bf16>(d_bits, n, row_stride, n_features, d_rows, m, d_table, table_stride, d_bias, k, scale, d_scores, score_stride, st);
+        return p.lookup ? lookup<bf16>(a, st) : product<STAG_BF16, false>(p, a, st);
     default:
-        return scores_typed<f16>(d_bits, n, row_stride, n_features, d_rows, m, d_table, table_stride, d_bias, k, scale, d_scores, score_stride, st);
+        return p.lookup ? lookup<f16>(a, st) : product<STAG_F16, false>(p, a, st);
     }
 }
 
@@ -499,16 +916,21 @@ int stag_row_scores_grad_dev(const uint32_t *d_bits, int64_t n, int64_t row_stri
     if (d_table_grad) TRY(check_matrix("d_table_grad", d_table_grad, STAG_F32, table_grad_stride, k));
     REQUIRE(aligned(d_bias_grad, 4), "d_bias_grad is not aligned to its type");
     if (!d_table_grad && !d_bias_grad) return STAG_OK;
-    const int64_t need = stag_row_scores_grad_workspace(m, n_features, k, type);
-    REQUIRE(work_bytes >= need && (need == 0 || (d_work && aligned(d_work, 256))), "d_work: %lld bytes, 256-byte aligned, are wanted", (long long)need);
+    const Plan p = product_plan(true, m, n_features, k);
+    REQUIRE(work_bytes >= p.work_bytes && (p.work_bytes == 0 || (d_work && aligned(d_work, 256))), "d_work: %lld bytes, 256-byte aligned, are wanted",
+            (long long)p.work_bytes);
+    ProductArgs a = {};
+    a.bits = d_bits, a.n = n, a.row_stride = row_stride, a.rows = d_rows, a.m = m, a.n_features = n_features;
+    a.mat = d_grad, a.mat_stride = grad_stride, a.k = k, a.scale = scale, a.out = d_table_grad, a.out_stride = table_grad_stride, a.bias_out = d_bias_grad;
+    a.part = (float *)d_work;
     hipStream_t st = (hipStream_t)stream;
     switch (type) {
     case STAG_F32:
-        return grad_typed<float>(d_bits, n, row_stride, n_features, d_rows, m, d_grad, grad_stride, k, scale, d_table_grad, table_grad_stride, d_bias_grad, st);
+        return product<STAG_F32, true>(p, a, st);
     case STAG_BF16:
-        return grad_typed<bf16>(d_bits, n, row_stride, n_features, d_rows, m, d_grad, grad_stride, k, scale, d_table_grad, table_grad_stride, d_bias_grad, st);
+        return product<STAG_BF16, true>(p, a, st);
     default:
-        return grad_typed<f16>(d_bits, n, row_stride, n_features, d_rows, m, d_grad, grad_stride, k, scale, d_table_grad, table_grad_stride, d_bias_grad, st);
+        return product<STAG_F16, true>(p, a, st);
     }
 }
 

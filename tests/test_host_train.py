@@ -29,6 +29,17 @@ def test_descriptors_have_the_layout_of_the_header():
         [0, 8, 16, 24, 32, 36, 40, 44]
 
 
+def test_workspaces_of_every_size():
+    L = _lib.train_lib()
+    for m in (0, 1, 63, 64, 65, 1000, 100000, 2**31 - 1):
+        for f in (1, 31, 7500, 157500, 1 << 27):
+            for k in (1, 13, 64, 1000, 1 << 20):
+                for kind in range(3):
+                    assert L.stag_row_scores_workspace(m, f, k, kind) >= 0
+                    assert L.stag_row_scores_grad_workspace(m, f, k, kind) >= 0
+            assert L.stag_sibling_loss_workspace(m, k) >= 0
+
+
 SCORES = dict(bits=P, n=10, row_stride=4, n_features=100, rows=None, m=10, table=P, type=0, table_stride=3, bias=None, k=3, scale=1.0, scores=P,
               score_stride=3, work=P, work_bytes=1 << 40, stream=None)
 
