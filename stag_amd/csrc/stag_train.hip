@@ -79,8 +79,9 @@ struct ProductArgs {
     const float *bias;          // scores: added
     float *out, *bias_out;      // bias_out: grad: column sums
     int64_t out_stride;
+    const uint32_t *turned;     // TURNED: the bits by feature, see k_turn
     float *part;                // more than one part: raw sums [parts][result rows][k], then column sums [parts][k]
-    int32_t n_features, words, k;
+    int32_t n_features, words, k;       // words of a row of bits (TURNED: of a turned row)
     int32_t steps, steps_per_part;      // in units of 4 K-steps (scores), 1 K-step (grad)
     float scale;
 };
@@ -125,26 +126,33 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x, int lane) {
     return x;
 }
 
+// Where the bits of a result row come from: ROWS: a batch row (scores); TURN: a feature, whose bits in 64 batch rows the wave
+// turns out of their packed rows as it goes; TURNED: a feature, from bits that k_turn has laid out by feature before.
+enum Source { ROWS, TURN, TURNED };
+
 // A workgroup of four waves makes 4 MT x 32 rows of the result by NT x 32 columns; a wave its own MT row tiles.  A K-step
 // is 64 terms of the sum: two words of bits, one for each half of the wave (the matrix instruction takes 8 terms from
-// each half), in four instructions of 16 terms.  The workgroup loads the K-step's 64 x 32 NT coefficients, cuts them into pieces and
-// stores them to LDS in operand order; two buffers, the next one's loads in flight while the matrix cores work on this one.
-template <int TYPE, bool GRAD, int MT, int NT>
+// each half), in four instructions of 16 terms.  The workgroup loads the coefficients of U K-steps, 64 U x 32 NT, cuts them into pieces
+// and stores them to LDS in operand order; the next ones are in flight while the matrix cores work on these.
+template <int TYPE, Source SRC, int MT, int NT, int U>
 __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
     typedef typename Raw<TYPE>::type raw_t;
-    constexpr int P = TYPE == STAG_F32 ? 3 : 1, COLS = 32 * NT, PASSES = NT, GROUPS = 256 / COLS;
-    __shared__ u32x4 lds[2][P][8][COLS];
+    constexpr bool GRAD = SRC != ROWS;
+    constexpr int P = TYPE == STAG_F32 ? 3 : 1, COLS = 32 * NT, GROUPS = 256 / COLS, BUFFERS = U == 1 ? 2 : 1;
+    static_assert(SRC != TURN || MT == 4, "a lane loads the words of its wave's row tiles at once");
+    __shared__ u32x4 lds[BUFFERS][U][P][8][COLS];
     __shared__ float sums[GRAD ? 256 : 1];
-    __shared__ int found;
     __shared__ uint8_t padding[GRAD ? 1 : 128 * MT];
+    __shared__ int found;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int64_t tile0 = ((int64_t)blockIdx.x * 4 + wave) * MT;           // this wave's first row tile
+    const int64_t out_rows = GRAD ? a.n_features : a.m;
     const int col = threadIdx.x % COLS, group = threadIdx.x / COLS;
     const int c0 = blockIdx.y * COLS, c = c0 + col < a.k ? c0 + col : a.k - 1;
     const bool c_ok = c0 + col < a.k;
     const int64_t limit = GRAD ? a.m : a.n_features;                       // terms of the sum
-    const int first = blockIdx.z * a.steps_per_part;
-    const int last = min(first + a.steps_per_part, a.steps);
+    constexpr int UNIT = SRC == TURN ? 1 : 4;                              // K-steps of a step of the plan
+    const int first = blockIdx.z * a.steps_per_part * UNIT, last = min((int)(blockIdx.z + 1) * a.steps_per_part, a.steps) * UNIT;
     const raw_t *mat = (const raw_t *)a.mat + c;
     if (threadIdx.x == 0) found = 0;
     __syncthreads();
@@ -162,80 +170,80 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
         for (int n = 0; n < NT; ++n) acc[t][n] = (f32x16)(0.f);
     float column_sum = 0.f;
 
-    raw_t b[PASSES][8];
-    // `real`: which of the K-step's terms there are; the others are zeros, whatever the memory holds
-    auto load_b = [&](int ks, uint64_t real) {
+    raw_t b[U][NT][8];
+    auto load_b = [&](int u, int ks) {
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
+        for (int i = 0; i < NT; ++i) {
             const int g = group + i * GROUPS, r0 = 32 * (g & 1) + 4 * (g >> 1);
-            if (real == ~0ull) {
+            if (term(ks, 63) < limit) {
                 const raw_t *p = mat + term(ks, r0) * a.mat_stride;
 #pragma unroll
-                for (int q = 0; q < 8; ++q) b[i][q] = p[((q >> 1) + 16 * (q & 1)) * a.mat_stride];
+                for (int q = 0; q < 8; ++q) b[u][i][q] = p[((q >> 1) + 16 * (q & 1)) * a.mat_stride];
             } else {
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
-                    const int r = r0 + (q >> 1) + 16 * (q & 1);
-                    const int64_t at = term(ks, r);
-                    b[i][q] = mat[(at < limit ? at : limit - 1) * a.mat_stride];
-                    if (!(real >> r & 1)) b[i][q] = 0;
+                    const int64_t at = term(ks, r0 + (q >> 1) + 16 * (q & 1));
+                    b[u][i][q] = mat[(at < limit ? at : limit - 1) * a.mat_stride];
                 }
             }
         }
     };
-    auto store_b = [&](int buf) {
+    // `real`: which of the K-step's terms there are; the others are zeros, whatever the memory held
+    auto store_b = [&](int buf, int u, uint64_t real) {
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
+        for (int i = 0; i < NT; ++i) {
             const int g = group + i * GROUPS;
-            if (!c_ok) {
+            raw_t(&v)[8] = b[u][i];
+            if (real != ~0ull || !c_ok) {
+                const uint32_t there = c_ok ? (uint32_t)(real >> (32 * (g & 1) + 4 * (g >> 1))) : 0u;
 #pragma unroll
-                for (int q = 0; q < 8; ++q) b[i][q] = 0;
+                for (int q = 0; q < 8; ++q)
+                    if (!(there >> ((q >> 1) + 16 * (q & 1)) & 1u)) v[q] = 0;
             }
             if constexpr (GRAD) {
                 if (blockIdx.x == 0) {
                     float s = 0.f;
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) s += value_of<TYPE>(b[i][q]);
+                    for (int q = 0; q < 8; ++q) s += value_of<TYPE>(v[q]);
                     column_sum += s;
                 }
             }
             uint32_t top = 0;
 #pragma unroll
-            for (int q = 0; q < 8; ++q) top = max(top, magnitude<TYPE>(b[i][q]));
+            for (int q = 0; q < 8; ++q) top = max(top, magnitude<TYPE>(v[q]));
             if (not_finite<TYPE>(top)) {
                 found = 1;
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
-                    if (not_finite<TYPE>(b[i][q])) b[i][q] = 0;
+                    if (not_finite<TYPE>(v[q])) v[q] = 0;
             }
             if constexpr (TYPE == STAG_F32) {
-                uint32_t x[8], y[8], z[8];
+                uint32_t y[8], z[8];
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
-                    x[q] = b[i][q];
-                    const float left = __uint_as_float(x[q]) - __uint_as_float(x[q] & 0xffff0000u);        // exact: the low 16 bits
+                    const float left = __uint_as_float(v[q]) - __uint_as_float(v[q] & 0xffff0000u);        // exact: the low 16 bits
                     y[q] = __float_as_uint(left);
                     z[q] = __float_as_uint(left - __uint_as_float(y[q] & 0xffff0000u));                    // exact: the low 8 bits
                 }
                 u32x4 p0, p1, p2;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    p0[j] = high_halves(x[2 * j], x[2 * j + 1]);
+                    p0[j] = high_halves(v[2 * j], v[2 * j + 1]);
                     p1[j] = high_halves(y[2 * j], y[2 * j + 1]);
                     p2[j] = high_halves(z[2 * j], z[2 * j + 1]);
                 }
-                lds[buf][0][g][col] = p0;
-                lds[buf][P > 1 ? 1 : 0][g][col] = p1;
-                lds[buf][P > 2 ? 2 : 0][g][col] = p2;
+                lds[buf][u][0][g][col] = p0;
+                lds[buf][u][P > 1 ? 1 : 0][g][col] = p1;
+                lds[buf][u][P > 2 ? 2 : 0][g][col] = p2;
             } else {
                 u32x4 p0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) p0[j] = (uint32_t)b[i][2 * j] | (uint32_t)b[i][2 * j + 1] << 16;
-                lds[buf][0][g][col] = p0;
+                for (int j = 0; j < 4; ++j) p0[j] = (uint32_t)v[2 * j] | (uint32_t)v[2 * j + 1] << 16;
+                lds[buf][u][0][g][col] = p0;
             }
         }
     };
-    auto multiply = [&](int buf, const uint32_t *x) {
+    auto multiply = [&](int buf, int u, const uint32_t *x) {
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             u32x4 w[MT];
@@ -245,7 +253,7 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
             for (int p = P - 1; p >= 0; --p)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const u32x4 v = lds[buf][p][2 * s + half][32 * n + (lane & 31)];
+                    const u32x4 v = lds[buf][u][p][2 * s + half][32 * n + (lane & 31)];
 #pragma unroll
                     for (int t = 0; t < MT; ++t) {
                         if constexpr (TYPE == STAG_F16)
@@ -257,13 +265,19 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
         }
     };
 
-    if constexpr (!GRAD) {
+    if constexpr (SRC != TURN) {
         const uint32_t *row[MT];
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             const int64_t i = (tile0 + t) * 32 + (lane & 31);
-            row[t] = i < a.m ? row_of(a.bits, a.n, a.row_stride, a.rows, i) : nullptr;
+            if constexpr (SRC == ROWS) {
+                row[t] = i < a.m ? row_of(a.bits, a.n, a.row_stride, a.rows, i) : nullptr;
+                if (half == 0) padding[(wave * MT + t) * 32 + lane] = row[t] == nullptr;
+            } else {
+                row[t] = i < out_rows ? a.turned + i * a.words : nullptr;
+            }
         }
+        const uint32_t *valid = SRC == TURNED ? a.turned + out_rows * a.words : nullptr;
         auto load_x = [&](int sb, u32x4 *x) {
             const int w = sb * 8 + half * 4;
 #pragma unroll
@@ -273,6 +287,7 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
             }
         };
         auto real_of = [&](int ks) -> uint64_t {
+            if constexpr (SRC == TURNED) return valid[(ks >> 2) * 8 + (ks & 3)] | (uint64_t)valid[(ks >> 2) * 8 + (ks & 3) + 4] << 32;
             uint64_t mask = 0;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -282,98 +297,118 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
             return mask;
         };
         u32x4 x[MT], next[MT];
+        load_x(first >> 2, x);
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
-            if (half == 0) padding[(wave * MT + t) * 32 + lane] = row[t] == nullptr;
-        load_x(first, x);
-        load_b(first * 4, real_of(first * 4));
-        store_b(0);
-        __syncthreads();
+        for (int u = 0; u < U; ++u) load_b(u, first + u);
+        if constexpr (U == 1) store_b(0, 0, real_of(first));
 #pragma unroll 1
-        for (int ks = first * 4; ks < last * 4; ++ks) {
-            const bool more = ks + 1 < last * 4;
-            if ((ks & 3) == 0 && ks + 4 < last * 4) load_x((ks >> 2) + 1, next);
-            if (more) load_b(ks + 1, real_of(ks + 1));
-            uint32_t w[MT];
+        for (int ks = first; ks < last; ks += U) {
+            const bool more = ks + U < last, turn = ((ks + U) & 3) == 0;
+            if constexpr (U > 1) {
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                w[t] = x[t][0];
-                x[t] = (ks & 3) == 3 ? next[t] : __builtin_shufflevector(x[t], x[t], 1, 2, 3, 0);
+                for (int u = 0; u < U; ++u) store_b(0, u, real_of(ks + u));
             }
-            multiply(ks & 1, w);
-            if (more) store_b((ks & 1) ^ 1);
             __syncthreads();
+            if ((U == 4 || (ks & 3) == 0) && ks + 4 < last) load_x((ks >> 2) + 1, next);
+            if (more) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) load_b(u, ks + U + u);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                uint32_t w[MT];
+#pragma unroll
+                for (int t = 0; t < MT; ++t) w[t] = x[t][u];
+                multiply(U == 1 ? ks & 1 : 0, u, w);
+            }
+#pragma unroll
+            for (int t = 0; t < MT; ++t) x[t] = U == 4 || turn ? next[t] : U == 2 ? __builtin_shufflevector(x[t], x[t], 2, 3, 0, 1) : __builtin_shufflevector(x[t], x[t], 1, 2, 3, 0);
+            if constexpr (U == 1) {
+                if (more) store_b((ks & 1) ^ 1, 0, real_of(ks + 1));
+            } else {
+                __syncthreads();
+            }
         }
     } else {
-        static_assert(!GRAD || MT == 4, "a lane loads the words of its wave's row tiles at once");
         const int64_t w0 = tile0 < a.words ? tile0 : a.words - 4;
-        auto load_row = [&](int ks) -> const uint32_t * {
+        const uint32_t *row[U];
+        u32x4 x[U];
+        uint64_t real[U];
+        auto load_row = [&](int u, int ks) {
             const int64_t i = (int64_t)ks * 64 + lane;
-            return i < a.m ? row_of(a.bits, a.n, a.row_stride, a.rows, i) : nullptr;
+            row[u] = ks < last && i < a.m ? row_of(a.bits, a.n, a.row_stride, a.rows, i) : nullptr;
         };
-        auto load_x = [&](const uint32_t *r) { return r ? *(const u32x4 *)(r + w0) : (u32x4)(0u); };
-        const uint32_t *row = load_row(first);
-        u32x4 x = load_x(row), next = (u32x4)(0u);
-        load_b(first, __ballot(row != nullptr));
-        const uint32_t *ahead = first + 1 < last ? load_row(first + 1) : nullptr;
-        store_b(0);
-        __syncthreads();
-#pragma unroll 1
-        for (int ks = first; ks < last; ++ks) {
-            const bool more = ks + 1 < last;
-            if (more) {
-                next = load_x(ahead);
-                load_b(ks + 1, __ballot(ahead != nullptr));
-                if (ks + 2 < last) ahead = load_row(ks + 2);
-            }
-            uint32_t w[4];
+        auto load_x = [&](int u) {
+            real[u] = __ballot(row[u] != nullptr);
+            x[u] = row[u] ? *(const u32x4 *)(row[u] + w0) : (u32x4)(0u);
+        };
 #pragma unroll
-            for (int t = 0; t < 4; ++t) w[t] = transposed(x[t], lane);
-            multiply((ks - first) & 1, w);
-            if (more) store_b(((ks - first) & 1) ^ 1);
+        for (int u = 0; u < U; ++u) {
+            load_row(u, first + u);
+            load_b(u, first + u);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_x(u);
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_row(u, first + U + u);
+        if constexpr (U == 1) store_b(0, 0, real[0]);
+#pragma unroll 1
+        for (int ks = first; ks < last; ks += U) {
+            const bool more = ks + U < last;
+            if constexpr (U > 1) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) store_b(0, u, real[u]);
+            }
             __syncthreads();
-            x = next;
+            u32x4 now[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) now[u] = x[u];
+            if (more) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    load_b(u, ks + U + u);
+                    load_x(u);
+                    load_row(u, ks + 2 * U + u);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                uint32_t w[4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) w[t] = transposed(now[u][t], lane);
+                multiply(U == 1 ? (ks - first) & 1 : 0, u, w);
+            }
+            if constexpr (U == 1) {
+                if (more) store_b(((ks - first) & 1) ^ 1, 0, real[0]);
+            } else {
+                __syncthreads();
+            }
         }
     }
+    __syncthreads();
 
-    const int64_t out_rows = GRAD ? a.n_features : a.m;
-    auto row_at = [&](int t, int i) -> int64_t { return (tile0 + t) * 32 + 8 * (i >> 2) + 4 * half + (i & 3); };
     const bool whole = gridDim.z == 1;
-    const float scale = 0.5f * a.scale;
+    float *to = whole ? a.out : a.part + (int64_t)blockIdx.z * out_rows * a.k;
+    const int64_t stride = whole ? a.out_stride : a.k;
+    const float scale = whole ? 0.5f * a.scale : 1.f;
+    if (to) {
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
+        for (int n = 0; n < NT; ++n) {
+            const int cc = c0 + 32 * n + (lane & 31);
+            if (cc >= a.k) continue;
+            const float bias = !GRAD && whole && a.bias ? a.bias[cc] : 0.f;
+            const int64_t r0 = tile0 * 32 + 4 * half;
+            float *p = to + r0 * stride + cc;
+            const int64_t left = out_rows - r0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int64_t r = row_at(t, i);
-            if (r >= out_rows) continue;
+            for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const int cc = c0 + 32 * n + (lane & 31);
-                if (cc >= a.k) continue;
-                if (!whole)
-                    a.part[((int64_t)blockIdx.z * out_rows + r) * a.k + cc] = acc[t][n][i];
-                else if (a.out)
-                    a.out[r * a.out_stride + cc] =
-                        !GRAD && padding[(wave * MT + t) * 32 + 8 * (i >> 2) + 4 * half + (i & 3)] ? 0.f : acc[t][n][i] * scale + (!GRAD && a.bias ? a.bias[cc] : 0.f);
-            }
-        }
-    if (found) {       // the terms left out above, to the results whose rows have the bit
-        __syncthreads();
-        for (int e = threadIdx.x; e < 128 * MT * COLS; e += 256) {
-            const int64_t r = (int64_t)blockIdx.x * 128 * MT + e / COLS;
-            const int cc = c0 + e % COLS;
-            if (r >= out_rows || cc >= a.k || (whole && !a.out)) continue;
-            float *to = whole ? a.out + r * a.out_stride + cc : a.part + ((int64_t)blockIdx.z * out_rows + r) * a.k + cc;
-            const int64_t end = min(limit, term(last * (GRAD ? 1 : 4), 0));
-            float s = 0.f;
-            for (int64_t at = term(first * (GRAD ? 1 : 4), 0); at < end; ++at) {
-                const raw_t v = ((const raw_t *)a.mat)[at * a.mat_stride + cc];
-                if (!not_finite<TYPE>(v)) continue;
-                const int64_t bit = GRAD ? r : at;
-                const uint32_t *words = row_of(a.bits, a.n, a.row_stride, a.rows, GRAD ? at : r);
-                if (words && (words[bit >> 5] >> (bit & 31) & 1u)) s += value_of<TYPE>(v);
-            }
-            if (!(s == 0.f)) *to += whole ? s * a.scale : s;
+                for (int i = 0; i < 16; ++i) {
+                    const int r = 32 * t + 8 * (i >> 2) + (i & 3);
+                    float v = acc[t][n][i] * scale;
+                    if constexpr (!GRAD) v += padding[wave * MT * 32 + 4 * half + r] ? 0.f : bias;
+                    if (r < left) p[r * stride] = v;
+                }
         }
     }
     if constexpr (GRAD) {
@@ -391,24 +426,80 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
             }
         }
     }
+    if (found && to) {       // the terms left out above, to the results whose rows have the bit
+        __syncthreads();
+        for (int e = threadIdx.x; e < 128 * MT * COLS; e += 256) {
+            const int64_t r = (int64_t)blockIdx.x * 128 * MT + e / COLS;
+            const int cc = c0 + e % COLS;
+            if (r >= out_rows || cc >= a.k) continue;
+            const int64_t end = min(limit, term(last, 0));
+            float s = 0.f;
+            for (int64_t at = term(first, 0); at < end; ++at) {
+                const raw_t v = ((const raw_t *)a.mat)[at * a.mat_stride + cc];
+                if (!not_finite<TYPE>(v)) continue;
+                const int64_t bit = GRAD ? r : at;
+                const uint32_t *words = row_of(a.bits, a.n, a.row_stride, a.rows, GRAD ? at : r);
+                if (words && (words[bit >> 5] >> (bit & 31) & 1u)) s += value_of<TYPE>(v);
+            }
+            if (!(s == 0.f)) to[r * stride + cc] += whole ? s * a.scale : s;
+        }
+    }
+}
+
+// The batch's bits by feature: turned[f][w], w < words = 8 * ceil(m / 256), with the words in the order in which k_product
+// takes them: word 8 s + 4 h + q holds batch rows 64 (4 s + q) + 32 h + (0..31).  Row n_features says which batch rows are no padding.
+// A wave turns 256 rows by 4 words of features; a lane loads 16 bytes of four rows and stores 16 bytes of four features.
+__global__ __launch_bounds__(256) void k_turn(ProductArgs a, uint32_t *turned, int row_words) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int64_t s = blockIdx.x;
+    const int w0 = (blockIdx.y * 4 + wave) * 4;
+    if (w0 >= row_words) return;
+    u32x4 x[4], real;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int64_t i = 64 * (4 * s + q) + lane;
+        const uint32_t *row = i < a.m ? row_of(a.bits, a.n, a.row_stride, a.rows, i) : nullptr;
+        x[q] = row ? *(const u32x4 *)(row + w0) : (u32x4)(0u);
+        const uint64_t mask = __ballot(row != nullptr);
+        real[q] = half ? (uint32_t)(mask >> 32) : (uint32_t)mask;
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        u32x4 y;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) y[q] = transposed(x[q][t], lane);
+        const int64_t f = (int64_t)(w0 + t) * 32 + (lane & 31);
+        if (f < a.n_features) *(u32x4 *)(turned + f * a.words + 8 * s + 4 * half) = y;
+    }
+    if (w0 == 0 && (lane & 31) == 0) *(u32x4 *)(turned + (int64_t)a.n_features * a.words + 8 * s + 4 * half) = real;
 }
 
 // adds up the parts, in order
 template <bool GRAD>
 __global__ __launch_bounds__(256) void k_join(ProductArgs a, int parts, int64_t out_rows) {
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, all = out_rows * a.k;
-    if (at < all) {
-        float s = 0.f;
-        for (int p = 0; p < parts; ++p) s += a.part[p * all + at];
-        const int64_t r = at / a.k;
-        const int c = (int)(at - r * a.k);
-        const bool padding = !GRAD && a.rows && !row_of(a.bits, a.n, a.row_stride, a.rows, r);
-        if (a.out) a.out[r * a.out_stride + c] = padding ? 0.f : s * (0.5f * a.scale) + (!GRAD && a.bias ? a.bias[c] : 0.f);
-    } else if (GRAD && at < all + a.k && a.bias_out) {
-        float s = 0.f;
-        for (int p = 0; p < parts; ++p) s += a.part[parts * all + (int64_t)p * a.k + (at - all)];
-        a.bias_out[at - all] = s;
+    const bool bias = GRAD && at >= all;
+    if (at >= all + (GRAD ? a.k : 0)) return;
+    const float *part = bias ? a.part + parts * all + (at - all) : a.part + at;
+    const int64_t step = bias ? a.k : all;
+    float s = 0.f;
+    int p = 0;
+    for (; p + 8 <= parts; p += 8) {
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = part[(p + u) * step];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) s += v[u];
     }
+    for (; p < parts; ++p) s += part[p * step];
+    if (bias) {
+        if (a.bias_out) a.bias_out[at - all] = s;
+        return;
+    }
+    const int64_t r = at / a.k;
+    const int c = (int)(at - r * a.k);
+    const bool padding = !GRAD && a.rows && !row_of(a.bits, a.n, a.row_stride, a.rows, r);
+    if (a.out) a.out[r * a.out_stride + c] = padding ? 0.f : s * (0.5f * a.scale) + (!GRAD && a.bias ? a.bias[c] : 0.f);
 }
 
 // Few rows: the lookups themselves.  A workgroup makes one row of scores, `cw` columns of it (a power of two up to 64): it
@@ -545,12 +636,21 @@ __global__ __launch_bounds__(256) void k_loss(const float *scores, int64_t score
     }
 }
 
+// adds up the partial rows: 32 columns a workgroup, every eighth row to a thread, then the eight sums in order
 __global__ __launch_bounds__(256) void k_loss_join(const float *part, int n_parts, int k, float *loss) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= k) return;
+    __shared__ double sums[8][32];
+    const int col = threadIdx.x & 31, g = threadIdx.x >> 5, c = blockIdx.x * 32 + col;
     double s = 0.0;
-    for (int p = 0; p < n_parts; ++p) s += part[(int64_t)p * k + c];
-    loss[c] = (float)s;
+    if (c < k) {
+#pragma unroll 8
+        for (int p = g; p < n_parts; p += 8) s += part[(int64_t)p * k + c];
+    }
+    sums[g][col] = s;
+    __syncthreads();
+    if (g == 0 && c < k) {
+        for (int q = 1; q < 8; ++q) s += sums[q][col];
+        loss[c] = (float)s;
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -771,8 +871,9 @@ int check_matrix(const char *name, const void *p, int type, int64_t stride, int3
 // how a product is cut up
 struct Plan {
     bool lookup;
+    Source src;
     int mt, nt, steps, per_part, parts;
-    int64_t row_blocks, col_blocks, out_rows, work_bytes;
+    int64_t row_blocks, col_blocks, out_rows, turned_words, turned_bytes, work_bytes;
 };
 
 Plan product_plan(bool grad, int64_t m, int32_t n_features, int32_t k) {
@@ -780,37 +881,56 @@ Plan product_plan(bool grad, int64_t m, int32_t n_features, int32_t k) {
     p.out_rows = grad ? n_features : m;
     if (m == 0) return p;
     p.lookup = !grad && m <= 64;
+    if (p.lookup) return p;
     p.nt = k <= 32 ? 1 : 2;
-    p.mt = grad || ceil_div(m, 512) * ceil_div(k, 32 * p.nt) >= 128 ? 4 : 1;
-    p.row_blocks = ceil_div(p.out_rows, 128 * p.mt);
     p.col_blocks = ceil_div(k, 32 * p.nt);
-    p.steps = (int)(grad ? ceil_div(m, 64) : ceil_div(n_features, 256));
-    const int64_t blocks = p.row_blocks * p.col_blocks, wanted = blocks < 512 ? 512 / blocks : 1, most = grad ? ceil_div(p.steps, 2) : p.steps;
+    p.src = !grad ? ROWS : p.col_blocks > 2 && m > 256 ? TURNED : TURN;
+    if (p.src == TURNED) {
+        p.turned_words = 8 * ceil_div(m, 256);
+        p.turned_bytes = ceil_div(((int64_t)n_features + 1) * p.turned_words * 4, 256) * 256;
+    }
+    p.mt = grad || m > 1024 ? 4 : 1;
+    p.row_blocks = ceil_div(p.out_rows, 128 * p.mt);
+    p.steps = (int)(p.src == ROWS ? ceil_div(n_features, 256) : p.src == TURN ? ceil_div(m, 64) : ceil_div(m, 256));
+    const int64_t blocks = p.row_blocks * p.col_blocks, wanted = blocks < 512 ? 512 / blocks : 1, most = p.src == TURN ? ceil_div(p.steps, 2) : p.steps;
     const int64_t parts = wanted < most ? wanted : most;
-    p.per_part = p.steps ? (int)ceil_div(p.steps, parts) : 0;
-    p.parts = p.steps ? (int)ceil_div(p.steps, p.per_part) : 0;
-    if (p.parts > 1 && !p.lookup) p.work_bytes = ((int64_t)p.parts * (p.out_rows + (grad ? 1 : 0)) * k) * 4;
+    p.per_part = (int)ceil_div(p.steps, parts);
+    p.parts = (int)ceil_div(p.steps, p.per_part);
+    p.work_bytes = p.turned_bytes + (p.parts > 1 ? ((int64_t)p.parts * (p.out_rows + (grad ? 1 : 0)) * k) * 4 : 0);
     return p;
 }
 
 template <int TYPE, bool GRAD>
-int product(const Plan &p, ProductArgs a, hipStream_t st) {
+int product(const Plan &p, ProductArgs a, void *work, hipStream_t st) {
     a.words = (int32_t)ceil_div(a.n_features, 128) * 4;
     a.steps = p.steps;
     a.steps_per_part = p.per_part;
+    a.part = (float *)((char *)work + p.turned_bytes);
     REQUIRE(p.row_blocks < (int64_t)1 << 31 && ceil_div((p.out_rows + 1) * a.k, 256) < (int64_t)1 << 31, "%lld rows of %d columns are too many",
             (long long)p.out_rows, a.k);
     if (p.parts) {
         const dim3 grid((unsigned)p.row_blocks, (unsigned)p.col_blocks, (unsigned)p.parts);
-        if (p.mt == 4 && p.nt == 2)
-            k_product<TYPE, GRAD, 4, 2><<<grid, 256, 0, st>>>(a);
-        else if (p.mt == 4)
-            k_product<TYPE, GRAD, 4, 1><<<grid, 256, 0, st>>>(a);
-        else if constexpr (!GRAD) {
-            if (p.nt == 2)
-                k_product<TYPE, GRAD, 1, 2><<<grid, 256, 0, st>>>(a);
+        if constexpr (GRAD) {
+            if (p.src == TURNED) {
+                const int row_words = a.words;
+                a.turned = (const uint32_t *)work;
+                a.words = (int32_t)p.turned_words;
+                k_turn<<<dim3((unsigned)ceil_div(a.m, 256), (unsigned)ceil_div(row_words, 16)), 256, 0, st>>>(a, (uint32_t *)work, row_words);
+                k_product<TYPE, TURNED, 4, 2, 1><<<grid, 256, 0, st>>>(a);
+            } else if (p.nt == 2) {
+                k_product<TYPE, TURN, 4, 2, 1><<<grid, 256, 0, st>>>(a);
+            } else {
+                k_product<TYPE, TURN, 4, 1, 2><<<grid, 256, 0, st>>>(a);
+            }
+        } else {
+            if (p.mt == 4 && p.nt == 2)
+                k_product<TYPE, ROWS, 4, 2, 1><<<grid, 256, 0, st>>>(a);
+            else if (p.mt == 4)
+                k_product<TYPE, ROWS, 4, 1, 2><<<grid, 256, 0, st>>>(a);
+            else if (p.nt == 2)
+                k_product<TYPE, ROWS, 1, 2, 2><<<grid, 256, 0, st>>>(a);
             else
-                k_product<TYPE, GRAD, 1, 1><<<grid, 256, 0, st>>>(a);
+                k_product<TYPE, ROWS, 1, 1, 4><<<grid, 256, 0, st>>>(a);
         }
         HIP_TRY(hipGetLastError());
     }
@@ -843,7 +963,7 @@ LossPlan loss_plan(int64_t m, int32_t k, bool vectors) {
     const int64_t cols = ceil_div(k, p.v);
     p.ct = (int)(cols < 256 ? cols : 256);
     p.gy = (unsigned)ceil_div(cols, p.ct);
-    const int64_t passes = ceil_div(m, 256 / p.ct), wanted = 2048 / p.gy > 0 ? 2048 / p.gy : 1;
+    const int64_t passes = ceil_div(m, 256 / p.ct), wanted = 1024 / p.gy > 0 ? 1024 / p.gy : 1;
     // few values: one workgroup a column tile, whose sums are the result without a second launch
     p.gx = (unsigned)(m * (int64_t)k <= 16384 ? 1 : passes < wanted ? passes : wanted);
     return p;
@@ -860,7 +980,7 @@ int loss_typed(const LossPlan &p, const float *d_scores, int64_t score_stride, i
         k_loss<T, 1><<<grid, 256, 0, st>>>(d_scores, score_stride, m, k, d_label, d_siblings, d_weight, scale, to, (T *)d_grad, grad_stride, p.ct);
     HIP_TRY(hipGetLastError());
     if (d_loss && p.gx > 1) {
-        k_loss_join<<<(unsigned)ceil_div(k, 256), 256, 0, st>>>(parts, (int)p.gx, k, d_loss);
+        k_loss_join<<<(unsigned)ceil_div(k, 32), 256, 0, st>>>(parts, (int)p.gx, k, d_loss);
         HIP_TRY(hipGetLastError());
     }
     return STAG_OK;
@@ -896,15 +1016,14 @@ int stag_row_scores_dev(const uint32_t *d_bits, int64_t n, int64_t row_stride, i
     ProductArgs a = {};
     a.bits = d_bits, a.n = n, a.row_stride = row_stride, a.rows = d_rows, a.m = m, a.n_features = n_features;
     a.mat = d_table, a.mat_stride = table_stride, a.bias = d_bias, a.k = k, a.scale = scale, a.out = d_scores, a.out_stride = score_stride;
-    a.part = (float *)d_work;
     hipStream_t st = (hipStream_t)stream;
     switch (type) {
     case STAG_F32:
-        return p.lookup ? lookup<float>(a, st) : product<STAG_F32, false>(p, a, st);
+        return p.lookup ? lookup<float>(a, st) : product<STAG_F32, false>(p, a, d_work, st);
     case STAG_BF16:
-        return p.lookup ? lookup<bf16>(a, st) : product<STAG_BF16, false>(p, a, st);
+        return p.lookup ? lookup<bf16>(a, st) : product<STAG_BF16, false>(p, a, d_work, st);
     default:
-        return p.lookup ? lookup<f16>(a, st) : product<STAG_F16, false>(p, a, st);
+        return p.lookup ? lookup<f16>(a, st) : product<STAG_F16, false>(p, a, d_work, st);
     }
 }
 
@@ -922,15 +1041,14 @@ int stag_row_scores_grad_dev(const uint32_t *d_bits, int64_t n, int64_t row_stri
     ProductArgs a = {};
     a.bits = d_bits, a.n = n, a.row_stride = row_stride, a.rows = d_rows, a.m = m, a.n_features = n_features;
     a.mat = d_grad, a.mat_stride = grad_stride, a.k = k, a.scale = scale, a.out = d_table_grad, a.out_stride = table_grad_stride, a.bias_out = d_bias_grad;
-    a.part = (float *)d_work;
     hipStream_t st = (hipStream_t)stream;
     switch (type) {
     case STAG_F32:
-        return product<STAG_F32, true>(p, a, st);
+        return product<STAG_F32, true>(p, a, d_work, st);
     case STAG_BF16:
-        return product<STAG_BF16, true>(p, a, st);
+        return product<STAG_BF16, true>(p, a, d_work, st);
     default:
-        return product<STAG_F16, true>(p, a, st);
+        return product<STAG_F16, true>(p, a, d_work, st);
     }
 }
 
