@@ -7,6 +7,9 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#ifdef STAG_TUNE
+#include <cstdlib>
+#endif
 
 namespace {
 
@@ -95,8 +98,18 @@ template <int TYPE> __device__ __forceinline__ bool not_finite(uint32_t raw) {
 template <int TYPE> __device__ __forceinline__ float value_of(uint32_t raw) {
     return TYPE == STAG_F32 ? __uint_as_float(raw) : TYPE == STAG_BF16 ? __uint_as_float(raw << 16) : (float)__builtin_bit_cast(f16, (uint16_t)raw);
 }
-// the larger of two magnitudes, as whole numbers: not finite if any of them is not
-template <int TYPE> __device__ __forceinline__ uint32_t magnitude(uint32_t raw) { return raw & (TYPE == STAG_F32 ? 0x7fffffffu : 0x7fffu); }
+
+// A buffer of up to 2^31 - 1 bytes: loads behind its end give zero, stores there are dropped.
+constexpr uint32_t NOWHERE = 0x80000000u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void *p, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, (int)(bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : bytes), 0x00020000);
+}
+template <typename raw_t> __device__ __forceinline__ raw_t load_raw(__amdgpu_buffer_rsrc_t from, uint32_t at) {
+    if constexpr (sizeof(raw_t) == 4)
+        return __builtin_amdgcn_raw_buffer_load_b32(from, at, 0, 0);
+    else
+        return __builtin_amdgcn_raw_buffer_load_b16(from, at, 0, 0);
+}
 
 __device__ __forceinline__ uint32_t high_halves(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
 
@@ -139,21 +152,19 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
     typedef typename Raw<TYPE>::type raw_t;
     constexpr bool GRAD = SRC != ROWS;
     constexpr int P = TYPE == STAG_F32 ? 3 : 1, COLS = 32 * NT, GROUPS = 256 / COLS, BUFFERS = U == 1 ? 2 : 1;
-    static_assert(SRC != TURN || MT == 4, "a lane loads the words of its wave's row tiles at once");
+    typedef __attribute__((ext_vector_type(MT))) uint32_t words_t;          // TURN: a lane loads the words of its wave's row tiles at once
     __shared__ u32x4 lds[BUFFERS][U][P][8][COLS];
     __shared__ float sums[GRAD ? 256 : 1];
-    __shared__ uint8_t padding[GRAD ? 1 : 128 * MT];
     __shared__ int found;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int64_t tile0 = ((int64_t)blockIdx.x * 4 + wave) * MT;           // this wave's first row tile
     const int64_t out_rows = GRAD ? a.n_features : a.m;
-    const int col = threadIdx.x % COLS, group = threadIdx.x / COLS;
-    const int c0 = blockIdx.y * COLS, c = c0 + col < a.k ? c0 + col : a.k - 1;
-    const bool c_ok = c0 + col < a.k;
+    const int col = threadIdx.x % COLS, group = threadIdx.x / COLS, c0 = blockIdx.y * COLS, c = c0 + col;
+    const bool c_ok = c < a.k;
     const int64_t limit = GRAD ? a.m : a.n_features;                       // terms of the sum
     constexpr int UNIT = SRC == TURN ? 1 : 4;                              // K-steps of a step of the plan
     const int first = blockIdx.z * a.steps_per_part * UNIT, last = min((int)(blockIdx.z + 1) * a.steps_per_part, a.steps) * UNIT;
-    const raw_t *mat = (const raw_t *)a.mat + c;
+    uint32_t padding[MT] = {}, any_padding = 0;                             // ROWS: which rows of a tile are padding
     if (threadIdx.x == 0) found = 0;
     __syncthreads();
 
@@ -170,35 +181,36 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
         for (int n = 0; n < NT; ++n) acc[t][n] = (f32x16)(0.f);
     float column_sum = 0.f;
 
+    // Buffer loads: one 32-bit offset a lane, and what lies behind the last term or column reads as zero.
     raw_t b[U][NT][8];
+    uint32_t at_b[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const int g = group + i * GROUPS, r0 = 4 * (g >> 1) + (g & 1) * (GRAD ? 32 : 128);
+        at_b[i] = c_ok ? (uint32_t)((r0 * (int)a.mat_stride + c) * (int)sizeof(raw_t)) : NOWHERE;
+    }
+    const uint32_t row_b = (uint32_t)a.mat_stride * sizeof(raw_t);
     auto load_b = [&](int u, int ks) {
+        const int64_t t0 = term(ks, 0);
+        const auto from = buffer((const raw_t *)a.mat + t0 * a.mat_stride, (limit - t0) * row_b);
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const int g = group + i * GROUPS, r0 = 32 * (g & 1) + 4 * (g >> 1);
-            if (term(ks, 63) < limit) {
-                const raw_t *p = mat + term(ks, r0) * a.mat_stride;
+        for (int i = 0; i < NT; ++i)
 #pragma unroll
-                for (int q = 0; q < 8; ++q) b[u][i][q] = p[((q >> 1) + 16 * (q & 1)) * a.mat_stride];
-            } else {
-#pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    const int64_t at = term(ks, r0 + (q >> 1) + 16 * (q & 1));
-                    b[u][i][q] = mat[(at < limit ? at : limit - 1) * a.mat_stride];
-                }
-            }
-        }
+            for (int q = 0; q < 8; ++q) b[u][i][q] = load_raw<raw_t>(from, at_b[i] + ((q >> 1) + 16 * (q & 1)) * row_b);
     };
-    // `real`: which of the K-step's terms there are; the others are zeros, whatever the memory held
+    // `real`: which of the K-step's rows are no padding (GRAD); the others are zeros, whatever the memory holds
     auto store_b = [&](int buf, int u, uint64_t real) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             const int g = group + i * GROUPS;
             raw_t(&v)[8] = b[u][i];
-            if (real != ~0ull || !c_ok) {
-                const uint32_t there = c_ok ? (uint32_t)(real >> (32 * (g & 1) + 4 * (g >> 1))) : 0u;
+            if constexpr (GRAD) {
+                if (a.rows && real != ~0ull) {
+                    const uint32_t there = (uint32_t)(real >> (32 * (g & 1) + 4 * (g >> 1)));
 #pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    if (!(there >> ((q >> 1) + 16 * (q & 1)) & 1u)) v[q] = 0;
+                    for (int q = 0; q < 8; ++q)
+                        if (!(there >> ((q >> 1) + 16 * (q & 1)) & 1u)) v[q] = 0;
+                }
             }
             if constexpr (GRAD) {
                 if (blockIdx.x == 0) {
@@ -208,22 +220,28 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
                     column_sum += s;
                 }
             }
-            uint32_t top = 0;
-#pragma unroll
-            for (int q = 0; q < 8; ++q) top = max(top, magnitude<TYPE>(v[q]));
-            if (not_finite<TYPE>(top)) {
-                found = 1;
-#pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    if (not_finite<TYPE>(v[q])) v[q] = 0;
-            }
             if constexpr (TYPE == STAG_F32) {
-                uint32_t y[8], z[8];
+                // an infinity or NaN makes NaN of the remainder, whatever the others are
+                auto cut = [&](uint32_t *y, uint32_t *z) -> float {
+                    float sum = 0.f;
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    const float left = __uint_as_float(v[q]) - __uint_as_float(v[q] & 0xffff0000u);        // exact: the low 16 bits
-                    y[q] = __float_as_uint(left);
-                    z[q] = __float_as_uint(left - __uint_as_float(y[q] & 0xffff0000u));                    // exact: the low 8 bits
+                    for (int q = 0; q < 8; ++q) {
+                        const float left = __uint_as_float(v[q]) - __uint_as_float(v[q] & 0xffff0000u);        // exact: the low 16 bits
+                        const float rest = left - __uint_as_float(__float_as_uint(left) & 0xffff0000u);        // exact: the low 8 bits
+                        y[q] = __float_as_uint(left);
+                        z[q] = __float_as_uint(rest);
+                        sum += rest;
+                    }
+                    return sum;
+                };
+                uint32_t y[8], z[8];
+                const float sum = cut(y, z);
+                if (!(sum == sum)) {
+                    found = 1;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        if (not_finite<TYPE>(v[q])) v[q] = 0;
+                    cut(y, z);
                 }
                 u32x4 p0, p1, p2;
 #pragma unroll
@@ -236,9 +254,22 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
                 lds[buf][u][P > 1 ? 1 : 0][g][col] = p1;
                 lds[buf][u][P > 2 ? 2 : 0][g][col] = p2;
             } else {
+                constexpr uint32_t EXPONENT = TYPE == STAG_BF16 ? 0x7f807f80u : 0x7c007c00u, ONE = TYPE == STAG_BF16 ? 0x00800080u : 0x04000400u;
                 u32x4 p0;
+                uint32_t over = 0;       // bit 15 and bit 31: an exponent of ones came by
 #pragma unroll
-                for (int j = 0; j < 4; ++j) p0[j] = (uint32_t)v[2 * j] | (uint32_t)v[2 * j + 1] << 16;
+                for (int j = 0; j < 4; ++j) {
+                    p0[j] = (uint32_t)v[2 * j] | (uint32_t)v[2 * j + 1] << 16;
+                    over |= (p0[j] & EXPONENT) + ONE;
+                }
+                if (over & 0x80008000u) {
+                    found = 1;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (not_finite<TYPE>(p0[j] & 0xffffu)) p0[j] &= 0xffff0000u;
+                        if (not_finite<TYPE>(p0[j] >> 16)) p0[j] &= 0x0000ffffu;
+                    }
+                }
                 lds[buf][u][0][g][col] = p0;
             }
         }
@@ -272,7 +303,8 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
             const int64_t i = (tile0 + t) * 32 + (lane & 31);
             if constexpr (SRC == ROWS) {
                 row[t] = i < a.m ? row_of(a.bits, a.n, a.row_stride, a.rows, i) : nullptr;
-                if (half == 0) padding[(wave * MT + t) * 32 + lane] = row[t] == nullptr;
+                padding[t] = (uint32_t)__ballot(row[t] == nullptr);
+                any_padding |= padding[t];
             } else {
                 row[t] = i < out_rows ? a.turned + i * a.words : nullptr;
             }
@@ -288,13 +320,7 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
         };
         auto real_of = [&](int ks) -> uint64_t {
             if constexpr (SRC == TURNED) return valid[(ks >> 2) * 8 + (ks & 3)] | (uint64_t)valid[(ks >> 2) * 8 + (ks & 3) + 4] << 32;
-            uint64_t mask = 0;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int64_t there = limit - term(ks, 32 * h);
-                mask |= (there >= 32 ? 0xffffffffull : there > 0 ? (1ull << there) - 1 : 0ull) << (32 * h);
-            }
-            return mask;
+            return ~0ull;
         };
         u32x4 x[MT], next[MT];
         load_x(first >> 2, x);
@@ -330,9 +356,9 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
             }
         }
     } else {
-        const int64_t w0 = tile0 < a.words ? tile0 : a.words - 4;
+        const int64_t w0 = tile0 < a.words ? tile0 : a.words - MT;
         const uint32_t *row[U];
-        u32x4 x[U];
+        words_t x[U];
         uint64_t real[U];
         auto load_row = [&](int u, int ks) {
             const int64_t i = (int64_t)ks * 64 + lane;
@@ -340,7 +366,7 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
         };
         auto load_x = [&](int u) {
             real[u] = __ballot(row[u] != nullptr);
-            x[u] = row[u] ? *(const u32x4 *)(row[u] + w0) : (u32x4)(0u);
+            x[u] = row[u] ? *(const words_t *)(row[u] + w0) : (words_t)(0u);
         };
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -360,7 +386,7 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
                 for (int u = 0; u < U; ++u) store_b(0, u, real[u]);
             }
             __syncthreads();
-            u32x4 now[U];
+            words_t now[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) now[u] = x[u];
             if (more) {
@@ -373,9 +399,9 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                uint32_t w[4];
+                uint32_t w[MT];
 #pragma unroll
-                for (int t = 0; t < 4; ++t) w[t] = transposed(now[u][t], lane);
+                for (int t = 0; t < MT; ++t) w[t] = transposed(now[u][t], lane);
                 multiply(U == 1 ? (ks - first) & 1 : 0, u, w);
             }
             if constexpr (U == 1) {
@@ -391,24 +417,28 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
     float *to = whole ? a.out : a.part + (int64_t)blockIdx.z * out_rows * a.k;
     const int64_t stride = whole ? a.out_stride : a.k;
     const float scale = whole ? 0.5f * a.scale : 1.f;
-    if (to) {
+    const auto into = buffer(to + tile0 * 32 * stride, to ? (out_rows - tile0 * 32) * stride * 4 : 0);
+    const uint32_t row_to = (uint32_t)stride * 4;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int cc = c0 + 32 * n + (lane & 31);
-            if (cc >= a.k) continue;
-            const float bias = !GRAD && whole && a.bias ? a.bias[cc] : 0.f;
-            const int64_t r0 = tile0 * 32 + 4 * half;
-            float *p = to + r0 * stride + cc;
-            const int64_t left = out_rows - r0;
+    for (int n = 0; n < NT; ++n) {
+        const int cc = c0 + 32 * n + (lane & 31);
+        const uint32_t at = cc < a.k ? (uint32_t)(4 * half * (int)stride + cc) * 4 : NOWHERE;
+        const float bias = !GRAD && whole && a.bias && cc < a.k ? a.bias[cc] : 0.f;
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+        for (int t = 0; t < MT; ++t) {
+            const uint32_t pad = padding[t] >> (4 * half);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int r = 32 * t + 8 * (i >> 2) + (i & 3);
-                    float v = acc[t][n][i] * scale;
-                    if constexpr (!GRAD) v += padding[wave * MT * 32 + 4 * half + r] ? 0.f : bias;
-                    if (r < left) p[r * stride] = v;
+            for (int i = 0; i < 16; ++i) {
+                const int r = 8 * (i >> 2) + (i & 3);
+                float v = acc[t][n][i] * scale;
+                if constexpr (!GRAD) {
+                    if (any_padding)
+                        v += pad >> r & 1u ? 0.f : bias;
+                    else
+                        v += bias;
                 }
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), into, at + (32 * t + r) * row_to, 0, 0);
+            }
         }
     }
     if constexpr (GRAD) {
@@ -841,6 +871,7 @@ __global__ __launch_bounds__(256) void k_adamw(AdamwArgs a) {
 constexpr int64_t MAX_M = (int64_t)1 << 31;      // rows of a batch
 constexpr int32_t MAX_K = 1 << 20;               // classifiers of a table
 constexpr int32_t MAX_FEATURES = 1 << 27;
+constexpr int64_t MAX_STRIDE = 1 << 21;          // 160 rows of it stay under 2^31 bytes, a buffer's reach
 
 int check_rows(const uint32_t *d_bits, int64_t n, int64_t row_stride, int32_t n_features, const int32_t *d_rows, int64_t m, int32_t k, int type) {
     REQUIRE(type_known(type), "unknown type %d", type);
@@ -859,6 +890,7 @@ int check_rows(const uint32_t *d_bits, int64_t n, int64_t row_stride, int32_t n_
 int check_matrix(const char *name, const void *p, int type, int64_t stride, int32_t k) {
     REQUIRE(p && aligned(p, type_bytes(type)), "%s is null or not aligned to its type", name);
     REQUIRE(stride >= k, "%s's stride %lld is less than its %d columns", name, (long long)stride, k);
+    REQUIRE(stride <= MAX_STRIDE, "%s's stride %lld is over %lld", name, (long long)stride, (long long)MAX_STRIDE);
     return STAG_OK;
 }
 
@@ -893,7 +925,10 @@ Plan product_plan(bool grad, int64_t m, int32_t n_features, int32_t k) {
     p.row_blocks = ceil_div(p.out_rows, 128 * p.mt);
     p.steps = (int)(p.src == ROWS ? ceil_div(n_features, 256) : p.src == TURN ? ceil_div(m, 64) : ceil_div(m, 256));
     const int64_t blocks = p.row_blocks * p.col_blocks, wanted = blocks < 512 ? 512 / blocks : 1, most = p.src == TURN ? ceil_div(p.steps, 2) : p.steps;
-    const int64_t parts = wanted < most ? wanted : most;
+    int64_t parts = wanted < most ? wanted : most;
+#ifdef STAG_TUNE
+    if (const char *e = getenv("STAG_TUNE")) { int mt, pp; sscanf(e, "%d,%d", &mt, &pp); if (p.src != TURNED) { p.mt = mt; p.row_blocks = ceil_div(p.out_rows, 128 * p.mt);} parts = pp < p.steps ? pp : p.steps; }
+#endif
     p.per_part = (int)ceil_div(p.steps, parts);
     p.parts = (int)ceil_div(p.steps, p.per_part);
     p.work_bytes = p.turned_bytes + (p.parts > 1 ? ((int64_t)p.parts * (p.out_rows + (grad ? 1 : 0)) * k) * 4 : 0);
@@ -917,10 +952,14 @@ int product(const Plan &p, ProductArgs a, void *work, hipStream_t st) {
                 a.words = (int32_t)p.turned_words;
                 k_turn<<<dim3((unsigned)ceil_div(a.m, 256), (unsigned)ceil_div(row_words, 16)), 256, 0, st>>>(a, (uint32_t *)work, row_words);
                 k_product<TYPE, TURNED, 4, 2, 1><<<grid, 256, 0, st>>>(a);
-            } else if (p.nt == 2) {
+            } else if (p.nt == 2 && p.mt == 4) {
                 k_product<TYPE, TURN, 4, 2, 1><<<grid, 256, 0, st>>>(a);
-            } else {
+            } else if (p.nt == 2) {
+                k_product<TYPE, TURN, 1, 2, 2><<<grid, 256, 0, st>>>(a);
+            } else if (p.mt == 4) {
                 k_product<TYPE, TURN, 4, 1, 2><<<grid, 256, 0, st>>>(a);
+            } else {
+                k_product<TYPE, TURN, 1, 1, 4><<<grid, 256, 0, st>>>(a);
             }
         } else {
             if (p.mt == 4 && p.nt == 2)
