@@ -102,10 +102,12 @@ int stag_sibling_loss_dev(const float *d_scores, int64_t score_stride, int64_t m
  * 1/2000 of itself, which rounding to nearest would lose every time.
  *
  * d_tensors: n descriptors in device memory; d_tiles: for each STAG_ADAMW_TILE values of each tensor (the last tile
- * of a tensor may be shorter) its tensor and its number in the tensor.  d_step: {t, 0}.
+ * of a tensor may be shorter) its tensor and its number in the tensor.  d_step: STAG_ADAMW_STEP_WORDS words, t and then
+ * zeros, which the call leaves zero.
  */
 #define STAG_ADAMW_BLOCK 256
 #define STAG_ADAMW_TILE 1024
+#define STAG_ADAMW_STEP_WORDS 1088
 typedef struct {
     void *param;
     const void *grad;

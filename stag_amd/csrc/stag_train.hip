@@ -71,6 +71,8 @@ typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
 
 struct ProductArgs {
     const uint32_t *bits;
@@ -597,59 +599,93 @@ __global__ __launch_bounds__(1024) void k_lookup(const uint32_t *bits, int64_t n
 // ------------------------------------------------------------------------------------------------------------------
 // loss of siblings
 // ------------------------------------------------------------------------------------------------------------------
-// A thread owns V neighbouring columns and goes down the rows of its workgroup; loss sums stay in its registers until the
-// workgroup adds them up in a fixed order and stores one partial row of K sums.  Scores are read only where the row
-// trains (a place of the tree has a handful of siblings among the thousands of a level); the rest of the gradient is
-// zeros, so what bounds a level's loss is writing the gradient.
+// e = exp(-|s|): 2^t with the rounding of t = -|s| log2(e) put back in; below 2^-126 by way of 2^(t + 64)
+__device__ __forceinline__ float exp_minus_abs(float s) {
+#pragma clang fp contract(off)
+    float x = fabsf(s);
+    x = x > 110.f ? 110.f : x;
+    const float t = -x * 0x1.715476p+0f, lost = fmaf(-x, 0x1.715476p+0f, -t) - x * 0x1.4ae0bep-26f;
+    const bool low = t < -120.f;
+    const float y = __builtin_amdgcn_exp2f(low ? t + 64.f : t);
+    return fmaf(y, lost * 0x1.62e430p-1f, y) * (low ? 0x1p-64f : 1.f);
+}
+
+// log(1 + e) for 0 <= e <= 1: 2 artanh(z), z = e / (2 + e) <= 1/3, by its series; what is left out is below 2^-26 of it.  For
+// small e it is e, whose halves may not be numbers of 32 bits.
+__device__ __forceinline__ float log_one_plus(float e) {
+    const float d = 2.f + e, r = __builtin_amdgcn_rcpf(d), z0 = e * r, z = fmaf(fmaf(-z0, d, e), r, z0), q = z * z;
+    float p = 1.f / 15.f;
+    p = fmaf(p, q, 1.f / 13.f);
+    p = fmaf(p, q, 1.f / 11.f);
+    p = fmaf(p, q, 1.f / 9.f);
+    p = fmaf(p, q, 1.f / 7.f);
+    p = fmaf(p, q, 1.f / 5.f);
+    p = fmaf(p, q, 1.f / 3.f);
+    return e < 0x1p-26f ? e : 2.f * fmaf(p * q, z, z);
+}
+
+// A thread owns V neighbouring columns and goes down the rows of its workgroup, four at a time so that their loads are in
+// flight together; loss sums stay in its registers until the workgroup adds them up in a fixed order and stores one
+// partial row of K sums.  Scores are read only where the row trains (a place of the tree has a handful of siblings among
+// the thousands of a level); the rest of the gradient is zeros, so what bounds a level's loss is writing the gradient.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void k_loss(const float *scores, int64_t score_stride, int64_t m, int k, const int32_t *label,
                                               const int32_t *siblings, const float *weight, float scale, float *loss, T *grad,
                                               int64_t grad_stride, int ct) {
+    constexpr int ROWS_AT_ONCE = 4;
+    typedef __attribute__((ext_vector_type(V))) T out_t;
     __shared__ float part[256 * V];
     const int cv = threadIdx.x % ct, r = threadIdx.x / ct, rp = 256 / ct;
     const int c0 = (blockIdx.y * ct + cv) * V;
     float sum[V] = {};
     if (r < rp && c0 < k) {
-        for (int64_t i = (int64_t)blockIdx.x * rp + r; i < m; i += (int64_t)gridDim.x * rp) {
-            int lo = 0, hi = k;
-            if (siblings) {
-                lo = siblings[2 * i];
-                hi = siblings[2 * i + 1];
-            }
-            float g[V] = {};
-            if (c0 + V > lo && c0 < hi) {
-                const int lab = label[i];
-                const float w = scale * (weight ? weight[i] : 1.f);
-                const float *src = scores + i * score_stride + c0;
-                float z[V];
-                if constexpr (V == 4) {
-                    const float4 q = *(const float4 *)src;
-                    z[0] = q.x, z[1] = q.y, z[2] = q.z, z[3] = q.w;
-                } else {
-                    z[0] = src[0];
-                }
+        const int64_t step = (int64_t)gridDim.x * rp;
+        for (int64_t i0 = (int64_t)blockIdx.x * rp + r; i0 < m; i0 += ROWS_AT_ONCE * step) {
+            int lo[ROWS_AT_ONCE], hi[ROWS_AT_ONCE], lab[ROWS_AT_ONCE];
+            float w[ROWS_AT_ONCE], z[ROWS_AT_ONCE][V];
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const int c = c0 + j;
-                    if (c < lo || c >= hi) continue;
-                    const float s = c == lab ? -z[j] : z[j];
-                    const float e = expf(-fabsf(s));
-                    sum[j] += w * ((s < 0.f ? 0.f : s) + log1pf(e));      // softplus(s); NaN stays NaN
-                    const float p = (s >= 0.f ? 1.f : e) / (1.f + e) * w;  // sigmoid(s)
-                    g[j] = c == lab ? -p : p;
+            for (int u = 0; u < ROWS_AT_ONCE; ++u) {
+                const int64_t i = i0 + u * step < m ? i0 + u * step : m - 1;
+                lo[u] = siblings ? siblings[2 * i] : 0;
+                hi[u] = siblings ? siblings[2 * i + 1] : k;
+                lab[u] = label[i];
+                w[u] = weight ? weight[i] : 1.f;
+            }
+#pragma unroll
+            for (int u = 0; u < ROWS_AT_ONCE; ++u) {
+                const int64_t i = i0 + u * step;
+                if (i < m && c0 + V > lo[u] && c0 < hi[u]) {
+                    const float *src = scores + i * score_stride + c0;
+                    if constexpr (V == 1) {
+                        z[u][0] = src[0];
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < V; q += 4) {
+                            const float4 f = *(const float4 *)(src + q);
+                            z[u][q] = f.x, z[u][q + 1] = f.y, z[u][q + 2] = f.z, z[u][q + 3] = f.w;
+                        }
+                    }
                 }
             }
-            if (grad) {
-                T *dst = grad + i * grad_stride + c0;
-                if constexpr (V == 4) {
-                    T out[4] = {(T)g[0], (T)g[1], (T)g[2], (T)g[3]};
-                    if constexpr (sizeof(T) == 4)
-                        *(float4 *)dst = *(const float4 *)out;
-                    else
-                        *(uint2 *)dst = *(const uint2 *)out;
-                } else {
-                    dst[0] = (T)g[0];
+#pragma unroll
+            for (int u = 0; u < ROWS_AT_ONCE; ++u) {
+                const int64_t i = i0 + u * step;
+                if (i >= m) break;
+                out_t g = (out_t)(T)0.f;
+                if (c0 + V > lo[u] && c0 < hi[u]) {
+                    const float wu = scale * w[u];
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        const int c = c0 + j;
+                        if (c < lo[u] || c >= hi[u]) continue;
+                        const float s = c == lab[u] ? -z[u][j] : z[u][j];
+                        const float e = exp_minus_abs(s), d = 1.f + e, r = __builtin_amdgcn_rcpf(d);
+                        sum[j] += wu * ((s < 0.f ? 0.f : s) + log_one_plus(e));        // softplus(s); NaN stays NaN
+                        const float p = (s >= 0.f ? 1.f : e) * fmaf(fmaf(-d, r, 1.f), r, r) * wu;   // sigmoid(s)
+                        g[j] = (T)(c == lab[u] ? -p : p);
+                    }
                 }
+                if (grad) *(out_t *)(grad + i * grad_stride + c0) = g;
             }
         }
     }
@@ -686,6 +722,9 @@ __global__ __launch_bounds__(256) void k_loss_join(const float *part, int n_part
 // ------------------------------------------------------------------------------------------------------------------
 // AdamW over many tensors
 // ------------------------------------------------------------------------------------------------------------------
+constexpr int STEP_COUNTERS = 32, STEP_LINE = 32;
+static_assert(STAG_ADAMW_STEP_WORDS == STEP_LINE * (2 + STEP_COUNTERS), "the words of d_step");
+
 struct AdamwArgs {
     const stag_adamw_tensor_t *tensors;
     const stag_adamw_tile_t *tiles;
@@ -696,46 +735,74 @@ struct AdamwArgs {
     float lr, beta1, beta2, one_minus_beta1, one_minus_beta2, log_beta1, log_beta2, eps;
 };
 
-__device__ __forceinline__ float4 load4(const void *p, int type, int64_t at, int64_t count, bool whole) {
-    float x[4];
+// Four neighbouring values as they lie in memory (16-bit ones in the first two words), past the caches: a step touches each once.
+// `whole`: all there and aligned; otherwise one by one up to `count`, zeros behind it.
+__device__ __forceinline__ u32x4 load4(const void *p, int type, int64_t at, int64_t count, bool whole) {
+    u32x4 x = (u32x4)(0u);
     if (whole) {
-        if (type == STAG_F32) return *(const float4 *)((const float *)p + at);
-        const uint2 q = *(const uint2 *)((const uint16_t *)p + at);
-        const uint32_t h[4] = {q.x & 0xffffu, q.x >> 16, q.y & 0xffffu, q.y >> 16};
+        if (type == STAG_F32) return __builtin_nontemporal_load((const u32x4 *)((const uint32_t *)p + at));
+        const u32x2 q = __builtin_nontemporal_load((const u32x2 *)((const uint16_t *)p + at));
+        x[0] = q[0], x[1] = q[1];
+        return x;
+    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            x[j] = type == STAG_BF16 ? __uint_as_float(h[j] << 16) : (float)__builtin_bit_cast(f16, (uint16_t)h[j]);
+    for (int j = 0; j < 4; ++j)
+        if (at + j < count) {
+            if (type == STAG_F32)
+                x[j] = ((const uint32_t *)p)[at + j];
+            else
+                x[j >> 1] |= (uint32_t)((const uint16_t *)p)[at + j] << (16 * (j & 1));
+        }
+    return x;
+}
+
+__device__ __forceinline__ void values4(u32x4 raw, int type, float *x) {
+    if (type == STAG_F32) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(raw[j]);
+    } else if (type == STAG_BF16) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) x[2 * j] = __uint_as_float(raw[j] << 16), x[2 * j + 1] = __uint_as_float(raw[j] & 0xffff0000u);
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            x[j] = 0.f;
-            if (at + j < count)
-                x[j] = type == STAG_F32 ? ((const float *)p)[at + j] : type == STAG_BF16 ? (float)((const bf16 *)p)[at + j]
-                                                                                         : (float)((const f16 *)p)[at + j];
-        }
+        for (int j = 0; j < 2; ++j) x[2 * j] = (float)__builtin_bit_cast(f16, (uint16_t)raw[j]), x[2 * j + 1] = (float)__builtin_bit_cast(f16, (uint16_t)(raw[j] >> 16));
     }
-    return make_float4(x[0], x[1], x[2], x[3]);
 }
 
 __device__ __forceinline__ void store4(void *p, int type, int64_t at, int64_t count, bool whole, const float *x) {
+    if (type == STAG_F32) {
+        if (whole) {
+            __builtin_nontemporal_store((f32x4){x[0], x[1], x[2], x[3]}, (f32x4 *)((float *)p + at));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (at + j < count) ((float *)p)[at + j] = x[j];
+        }
+        return;
+    }
     uint16_t h[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) h[j] = type == STAG_BF16 ? __builtin_bit_cast(uint16_t, (bf16)x[j]) : __builtin_bit_cast(uint16_t, (f16)x[j]);
     if (whole) {
-        if (type == STAG_F32)
-            *(float4 *)((float *)p + at) = make_float4(x[0], x[1], x[2], x[3]);
-        else
-            *(uint2 *)((uint16_t *)p + at) = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+        __builtin_nontemporal_store((u32x2){h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16}, (u32x2 *)((uint16_t *)p + at));
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (at + j < count) {
-                if (type == STAG_F32)
-                    ((float *)p)[at + j] = x[j];
-                else
-                    ((uint16_t *)p)[at + j] = h[j];
-            }
+            if (at + j < count) ((uint16_t *)p)[at + j] = h[j];
     }
+}
+
+// the largest of the wave's values (not negative), the same for every lane
+__device__ __forceinline__ int wave_max(int x) {
+#define STAG_MAX_DPP(CONTROL) x = max(x, __builtin_amdgcn_update_dpp(x, x, CONTROL, 0xf, 0xf, false));
+    STAG_MAX_DPP(0x111)      // row_shr 1, 2, 4, 8: the last lane of each 16 has their maximum
+    STAG_MAX_DPP(0x112)
+    STAG_MAX_DPP(0x114)
+    STAG_MAX_DPP(0x118)
+    STAG_MAX_DPP(0x142)      // row_bcast 15, 31: the last lane has all
+    STAG_MAX_DPP(0x143)
+#undef STAG_MAX_DPP
+    return __builtin_amdgcn_readlane(x, 63);
 }
 
 // The exponent (biased) of the smallest power of two s with max|x| <= 448 s over the wave's 256 values; 448 = 1.75 * 2^8 is
@@ -743,24 +810,32 @@ __device__ __forceinline__ void store4(void *p, int type, int64_t at, int64_t co
 __device__ __forceinline__ int scale_exponent(const float *x) {
     int top = 10 << 23;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int a = __float_as_int(x[j]) & 0x7fffffff;
-        if (a < 0x7f800000) top = max(top, a);
-    }
+    for (int j = 0; j < 4; ++j) top = max(top, __float_as_int(x[j]) & 0x7fffffff);
+    top = wave_max(top);
+    if (top >= 0x7f800000) {
+        top = 10 << 23;
 #pragma unroll
-    for (int o = 32; o; o >>= 1) top = max(top, __shfl_xor(top, o));
+        for (int j = 0; j < 4; ++j) {
+            const int a = __float_as_int(x[j]) & 0x7fffffff;
+            top = max(top, a < 0x7f800000 ? a : 0);
+        }
+        top = wave_max(top);
+    }
     return (top >> 23) - 8 + ((top & 0x7fffff) > 0x600000);
 }
 
-// x / s as the value of an e4m3 code, up or down by `chance` (16 bits).  From 2^-6 on a code has 3 bits behind the leading
-// one: adding 20 random bits below them and cutting them off goes up with the probability of what is cut; below, codes
-// are 2^-9 apart.
-__device__ __forceinline__ float rounded(float x, float inv, uint32_t chance) {
-#pragma clang fp contract(off)
-    const float y = x * inv, a = fabsf(y);
-    const float normal = __uint_as_float((__float_as_uint(a) + (chance << 4 | 8u)) & 0xfff00000u);
-    const float small = floorf(a * 512.f + ((float)chance + 0.5f) * 0x1p-16f) * 0x1p-9f;
-    return copysignf(a < 0x1p-6f ? small : normal, y);
+// a = |x| / s as the value of an e4m3 code, up or down by `chance` (16 bits).  From 2^-6 on a code has 3 bits behind the
+// leading one: adding 20 random bits below them and cutting them off goes up with the probability of what is cut.  Below
+// 2^-6 codes are 2^-9 apart, as they are from 2^-6 to 2^-5: such a value is moved there, rounded and moved back.
+__device__ __forceinline__ float rounded(float a, uint32_t chance) {
+    const float up = a < 0x1p-6f ? 0x1p-6f : 0.f;
+    return __uint_as_float((__float_as_uint(a + up) + (chance << 4 | 8u)) & 0xfff00000u) - up;
+}
+
+// sqrt(x), x >= 0, from x / sqrt(x) and one step of Newton's method, which puts the rounding right
+__device__ __forceinline__ float root_of(float x) {
+    const float s = __builtin_amdgcn_rsqf(x), y = x * s;
+    return x == 0.f || x == INFINITY ? x : fmaf(fmaf(-y, y, x), 0.5f * s, y);
 }
 
 __device__ __forceinline__ uint32_t pack_e4m3(const float *x) {
@@ -775,12 +850,14 @@ __device__ __forceinline__ void unpack_e4m3(uint32_t q, float *x) {
     x[3] = __builtin_amdgcn_cvt_f32_fp8((int)q, 3);
 }
 
-// A wave takes a tile of four blocks of 256 values, four neighbouring values a lane.  Everything is read once and written
-// once; what bounds it is HBM.  m, v and the root are rounded after every operation (no fused multiply-add), so that the 8-bit codes are a
-// function of the inputs that any other 32-bit implementation can restate.
+// A wave takes a tile of four blocks of 256 values, four neighbouring values a lane, and has the loads of GROUP blocks in
+// flight before it computes.  Everything is read once and written once; what bounds it is HBM.  m, v and the root are rounded after
+// every operation (no fused multiply-add), so that the 8-bit codes are a function of the inputs that any other 32-bit
+// implementation can restate.
 template <int BITS>
 __global__ __launch_bounds__(256) void k_adamw(AdamwArgs a) {
 #pragma clang fp contract(off)
+    constexpr int GROUP = BITS == 32 ? 4 : 2;
     const int lane = threadIdx.x & 63;
     const int t = __hip_atomic_load(a.step, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
     // 1 - beta^t = -expm1(t log beta)
@@ -790,77 +867,114 @@ __global__ __launch_bounds__(256) void k_adamw(AdamwArgs a) {
     for (int64_t w = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); w < a.n_tiles; w += (int64_t)gridDim.x * 4) {
         const stag_adamw_tile_t tile = a.tiles[w];
         const stag_adamw_tensor_t d = a.tensors[tile.tensor];
-        const int64_t at0 = (int64_t)tile.tile * STAG_ADAMW_TILE + lane * 4;
-        const int vec_p = ((uintptr_t)d.param & (d.param_type == STAG_F32 ? 15 : 7)) == 0;
-        const int vec_g = ((uintptr_t)d.grad & (d.grad_type == STAG_F32 ? 15 : 7)) == 0;
+        const int64_t at0 = (int64_t)tile.tile * STAG_ADAMW_TILE, s0 = d.state_at + at0;
+        const bool vec_p = ((uintptr_t)d.param & (d.param_type == STAG_F32 ? 15 : 7)) == 0;
+        const bool vec_g = ((uintptr_t)d.grad & (d.grad_type == STAG_F32 ? 15 : 7)) == 0;
         const float keep = 1.f - a.lr * d.weight_decay, shrink = a.lr * d.l1;
+        const int blocks = (int)min((int64_t)STAG_ADAMW_TILE / STAG_ADAMW_BLOCK, (d.count - at0 + STAG_ADAMW_BLOCK - 1) / STAG_ADAMW_BLOCK);
+        const bool inside = at0 + STAG_ADAMW_TILE <= d.count;
+#pragma unroll 1
+        for (int b0 = 0; b0 < blocks; b0 += GROUP) {
+            u32x4 raw_p[GROUP], raw_g[GROUP], raw_m[GROUP], raw_v[GROUP];
+            float ms[GROUP], vs[GROUP];
 #pragma unroll
-        for (int b = 0; b < STAG_ADAMW_TILE / 256; ++b) {
-            const int64_t at = at0 + b * 256, s = d.state_at + at;
-            if (at - lane * 4 >= d.count) break;
-            const bool full = at + 4 <= d.count;
-            const float4 p4 = load4(d.param, d.param_type, at, d.count, full && vec_p);
-            const float4 g4 = load4(d.grad, d.grad_type, at, d.count, full && vec_g);
-            float p[4] = {p4.x, p4.y, p4.z, p4.w}, g[4] = {g4.x, g4.y, g4.z, g4.w}, m[4], v[4], root[4];
-            if constexpr (BITS == 32) {
-                const float4 m4 = *(const float4 *)((const float *)a.m + s), v4 = *(const float4 *)((const float *)a.v + s);
-                m[0] = m4.x, m[1] = m4.y, m[2] = m4.z, m[3] = m4.w;
-                v[0] = v4.x, v[1] = v4.y, v[2] = v4.z, v[3] = v4.w;
-            } else {
-                unpack_e4m3(*(const uint32_t *)((const uint8_t *)a.m + s), m);
-                unpack_e4m3(*(const uint32_t *)((const uint8_t *)a.v + s), v);
-                const float ms = a.m_scale[s >> 8], vs = a.v_scale[s >> 8];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    m[j] = m[j] * ms;
-                    v[j] = v[j] * vs;
-                    v[j] = v[j] * v[j];
+            for (int b = 0; b < GROUP; ++b) {
+                if (b0 + b >= blocks) continue;
+                const int64_t at = at0 + (b0 + b) * STAG_ADAMW_BLOCK + lane * 4, s = s0 + (b0 + b) * STAG_ADAMW_BLOCK + lane * 4;
+                const bool full = inside || at + 4 <= d.count;
+                raw_p[b] = load4(d.param, d.param_type, at, d.count, full && vec_p);
+                raw_g[b] = load4(d.grad, d.grad_type, at, d.count, full && vec_g);
+                if constexpr (BITS == 32) {
+                    raw_m[b] = load4(a.m, STAG_F32, s, 0, true);
+                    raw_v[b] = load4(a.v, STAG_F32, s, 0, true);
+                } else {
+                    raw_m[b][0] = __builtin_nontemporal_load((const uint32_t *)((const uint8_t *)a.m + s));
+                    raw_v[b][0] = __builtin_nontemporal_load((const uint32_t *)((const uint8_t *)a.v + s));
+                    ms[b] = a.m_scale[s0 / STAG_ADAMW_BLOCK + b0 + b];
+                    vs[b] = a.v_scale[s0 / STAG_ADAMW_BLOCK + b0 + b];
                 }
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (at + j >= d.count) m[j] = v[j] = 0.f;      // places between tensors hold nothing
-                m[j] = m[j] * a.beta1 + g[j] * a.one_minus_beta1;
-                v[j] = v[j] * a.beta2 + (g[j] * g[j]) * a.one_minus_beta2;
-                root[j] = sqrtf(v[j]);
-                const float r = __builtin_amdgcn_rcpf(root[j] * c2 + a.eps);
-                p[j] = p[j] * keep - c1 * m[j] * r;
-                const float left = fabsf(p[j]) - shrink * r;
-                if (shrink > 0.f) p[j] = copysignf(left < 0.f ? 0.f : left, p[j]);
-            }
-            store4(d.param, d.param_type, at, d.count, full && vec_p, p);
-            if constexpr (BITS == 32) {
-                *(float4 *)((float *)a.m + s) = make_float4(m[0], m[1], m[2], m[3]);
-                *(float4 *)((float *)a.v + s) = make_float4(v[0], v[1], v[2], v[3]);
-            } else {
-                const int me = scale_exponent(m), ve = scale_exponent(root);
-                const float mi = __int_as_float((254 - me) << 23), vi = __int_as_float((254 - ve) << 23);
+            for (int b = 0; b < GROUP; ++b) {
+                if (b0 + b >= blocks) continue;
+                const int64_t at = at0 + (b0 + b) * STAG_ADAMW_BLOCK + lane * 4, s = s0 + (b0 + b) * STAG_ADAMW_BLOCK + lane * 4;
+                const bool full = inside || at + 4 <= d.count;
+                float p[4], g[4], m[4], v[4], root[4];
+                values4(raw_p[b], d.param_type, p);
+                values4(raw_g[b], d.grad_type, g);
+                if constexpr (BITS == 32) {
+                    values4(raw_m[b], STAG_F32, m);
+                    values4(raw_v[b], STAG_F32, v);
+                } else {
+                    unpack_e4m3(raw_m[b][0], m);
+                    unpack_e4m3(raw_v[b][0], v);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        m[j] = m[j] * ms[b];
+                        v[j] = v[j] * vs[b];
+                        v[j] = v[j] * v[j];
+                    }
+                }
+                if (!inside) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (at + j >= d.count) m[j] = v[j] = 0.f;      // places between tensors hold nothing
+                }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    uint32_t x = (uint32_t)(s + j) ^ salt;
-                    x = (x ^ x >> 16) * 0x7FEB352Du;
-                    x = (x ^ x >> 15) * 0x846CA68Bu;
-                    x ^= x >> 16;
-                    m[j] = rounded(m[j], mi, x >> 16);
-                    const float q = rounded(root[j], vi, x & 0xffffu);
-                    v[j] = root[j] > 0.f && q == 0.f ? 0x1p-9f : q;      // a root of zero would divide by eps alone: what is not zero stays so
+                    m[j] = m[j] * a.beta1 + g[j] * a.one_minus_beta1;
+                    v[j] = v[j] * a.beta2 + (g[j] * g[j]) * a.one_minus_beta2;
+                    root[j] = BITS == 32 ? __builtin_amdgcn_sqrtf(v[j]) : root_of(v[j]);
                 }
-                *(uint32_t *)((uint8_t *)a.m + s) = pack_e4m3(m);
-                *(uint32_t *)((uint8_t *)a.v + s) = pack_e4m3(v);
-                if (lane == 0) {
-                    a.m_scale[s >> 8] = __int_as_float(me << 23);
-                    a.v_scale[s >> 8] = __int_as_float(ve << 23);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float r = __builtin_amdgcn_rcpf(fmaf(root[j], c2, a.eps));
+                    p[j] = fmaf(-c1 * m[j], r, p[j] * keep);
+                    if (shrink > 0.f) {
+                        const float left = fmaf(-shrink, r, fabsf(p[j]));
+                        p[j] = copysignf(left < 0.f ? 0.f : left, p[j]);
+                    }
+                }
+                store4(d.param, d.param_type, at, d.count, full && vec_p, p);
+                if constexpr (BITS == 32) {
+                    store4(a.m, STAG_F32, s, 0, true, m);
+                    store4(a.v, STAG_F32, s, 0, true, v);
+                } else {
+                    const int me = scale_exponent(m), ve = scale_exponent(root);
+                    const float mi = __int_as_float((254 - me) << 23), vi = __int_as_float((254 - ve) << 23);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t x = (uint32_t)(s + j) ^ salt;
+                        x = (x ^ x >> 16) * 0x7FEB352Du;
+                        x = (x ^ x >> 15) * 0x846CA68Bu;
+                        x ^= x >> 16;
+                        const float y = m[j] * mi, q = rounded(root[j] * vi, x & 0xffffu);
+                        m[j] = copysignf(rounded(fabsf(y), x >> 16), y);
+                        v[j] = root[j] > 0.f && q == 0.f ? 0x1p-9f : q;      // a root of zero would divide by eps alone: what is not zero stays so
+                    }
+                    __builtin_nontemporal_store(pack_e4m3(m), (uint32_t *)((uint8_t *)a.m + s));
+                    __builtin_nontemporal_store(pack_e4m3(v), (uint32_t *)((uint8_t *)a.v + s));
+                    if (lane == 0) {
+                        a.m_scale[s >> 8] = __int_as_float(me << 23);
+                        a.v_scale[s >> 8] = __int_as_float(ve << 23);
+                    }
                 }
             }
         }
     }
-    // the last workgroup to come here, when all have read t, counts the step
+    // The last workgroup to come here, when all have read t, counts the step.  2,048 atomics on one address took 120 us, so
+    // the workgroups come in by 32 counters in lines of their own, and the last of each goes on to the one of all.  Nothing
+    // else is ordered by this, so it is relaxed: a release would write back the L2 for every workgroup.
     __syncthreads();
     if (threadIdx.x == 0) {
-        const int before = __hip_atomic_fetch_add(a.step + 1, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-        if (before == (int)gridDim.x - 1) {
-            __hip_atomic_store(a.step + 1, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(a.step, t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int groups = min((int)gridDim.x, STEP_COUNTERS), g = blockIdx.x % STEP_COUNTERS;
+        int32_t *mine = a.step + STEP_LINE * (1 + g), *all = a.step + STEP_LINE * (1 + STEP_COUNTERS);
+        if (__hip_atomic_fetch_add(mine, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == ((int)gridDim.x - 1 - g) / STEP_COUNTERS) {
+            __hip_atomic_store(mine, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (__hip_atomic_fetch_add(all, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == groups - 1) {
+                __hip_atomic_store(all, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(a.step, t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
         }
     }
 }
@@ -996,13 +1110,13 @@ struct LossPlan {
     unsigned gx, gy;
 };
 
-LossPlan loss_plan(int64_t m, int32_t k, bool vectors) {
+LossPlan loss_plan(int64_t m, int32_t k, int v) {
     LossPlan p;
-    p.v = vectors ? 4 : 1;
+    p.v = v;
     const int64_t cols = ceil_div(k, p.v);
     p.ct = (int)(cols < 256 ? cols : 256);
     p.gy = (unsigned)ceil_div(cols, p.ct);
-    const int64_t passes = ceil_div(m, 256 / p.ct), wanted = 1024 / p.gy > 0 ? 1024 / p.gy : 1;
+    const int64_t passes = ceil_div(m, 256 / p.ct), wanted = 2048 / p.gy > 0 ? 2048 / p.gy : 1;
     // few values: one workgroup a column tile, whose sums are the result without a second launch
     p.gx = (unsigned)(m * (int64_t)k <= 16384 ? 1 : passes < wanted ? passes : wanted);
     return p;
@@ -1013,7 +1127,10 @@ int loss_typed(const LossPlan &p, const float *d_scores, int64_t score_stride, i
                const float *d_weight, float scale, float *d_loss, void *d_grad, int64_t grad_stride, float *parts, hipStream_t st) {
     float *to = d_loss && p.gx > 1 ? parts : d_loss;
     const dim3 grid(p.gx, p.gy);
-    if (p.v == 4)
+    if (p.v == 8) {
+        if constexpr (sizeof(T) == 2)
+            k_loss<T, 8><<<grid, 256, 0, st>>>(d_scores, score_stride, m, k, d_label, d_siblings, d_weight, scale, to, (T *)d_grad, grad_stride, p.ct);
+    } else if (p.v == 4)
         k_loss<T, 4><<<grid, 256, 0, st>>>(d_scores, score_stride, m, k, d_label, d_siblings, d_weight, scale, to, (T *)d_grad, grad_stride, p.ct);
     else
         k_loss<T, 1><<<grid, 256, 0, st>>>(d_scores, score_stride, m, k, d_label, d_siblings, d_weight, scale, to, (T *)d_grad, grad_stride, p.ct);
@@ -1094,7 +1211,11 @@ int stag_row_scores_grad_dev(const uint32_t *d_bits, int64_t n, int64_t row_stri
 int64_t stag_sibling_loss_workspace(int64_t m, int32_t k) {
     REQUIRE(m >= 0 && m < MAX_M, "m = %lld is not in 0..2^31-1", (long long)m);
     REQUIRE(k >= 1 && k <= MAX_K, "k = %d is not in 1..%d", k, MAX_K);
-    const unsigned a = loss_plan(m, k, true).gx, b = loss_plan(m, k, false).gx, most = a > b ? a : b;
+    unsigned most = 1;
+    for (int v : {1, 4, 8}) {
+        const unsigned gx = loss_plan(m, k, v).gx;
+        if (gx > most) most = gx;
+    }
     return most > 1 ? (int64_t)most * k * 4 : 0;
 }
 
@@ -1112,8 +1233,11 @@ int stag_sibling_loss_dev(const float *d_scores, int64_t score_stride, int64_t m
     }
     if (!d_loss && (!d_grad || m == 0)) return STAG_OK;
     REQUIRE(!d_loss || (work_bytes >= need && (need == 0 || (d_work && aligned(d_work, 256)))), "d_work: %lld bytes, 256-byte aligned, are wanted", (long long)need);
-    const bool vectors = k % 4 == 0 && score_stride % 4 == 0 && aligned(d_scores, 16) && (!d_grad || (grad_stride % 4 == 0 && aligned(d_grad, 4 * type_bytes(type))));
-    const LossPlan p = loss_plan(m, k, vectors);
+    // 16 bytes of gradient at once, if all rows of both matrices allow it
+    auto fits = [&](int v) {
+        return k % v == 0 && score_stride % v == 0 && aligned(d_scores, 16) && (!d_grad || (grad_stride % v == 0 && aligned(d_grad, v * type_bytes(type))));
+    };
+    const LossPlan p = loss_plan(m, k, type != STAG_F32 && fits(8) ? 8 : fits(4) ? 4 : 1);
     hipStream_t st = (hipStream_t)stream;
     float *parts = (float *)d_work;
     switch (type) {
@@ -1154,7 +1278,7 @@ int stag_adamw_dev(const stag_adamw_tensor_t *d_tensors, const stag_adamw_tile_t
     a.log_beta1 = (float)std::log(beta1);
     a.log_beta2 = (float)std::log(beta2);
     a.eps = (float)eps;
-    const unsigned grid = (unsigned)(n_tiles < 4 * 2048 ? ceil_div(n_tiles, 4) : 2048);
+    const unsigned grid = (unsigned)(n_tiles < 4 * 4096 ? ceil_div(n_tiles, 4) : 4096);
     if (state_bits == 32)
         k_adamw<32><<<grid, 256, 0, (hipStream_t)stream>>>(a);
     else

@@ -25,7 +25,7 @@ import torch
 
 from . import _lib
 
-BLOCK, TILE = 256, 1024            # STAG_ADAMW_BLOCK, STAG_ADAMW_TILE
+BLOCK, TILE, STEP_WORDS = 256, 1024, 1088            # STAG_ADAMW_BLOCK, STAG_ADAMW_TILE, STAG_ADAMW_STEP_WORDS
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _TENSOR = np.dtype([("param", "<u8"), ("grad", "<u8"), ("count", "<i8"), ("state_at", "<i8"), ("weight_decay", "<f4"), ("l1", "<f4"),
                     ("param_type", "<i4"), ("grad_type", "<i4")])      # stag_adamw_tensor_t
@@ -283,7 +283,7 @@ class AdamW:
         self._n_tiles = len(tiles)
         self._tensors = torch.from_numpy(table.view(np.uint8)).to(device)
         self._tiles = torch.from_numpy(tiles).to(device)
-        self._step = torch.zeros(2, dtype=torch.int32, device=device)
+        self._step = torch.zeros(STEP_WORDS, dtype=torch.int32, device=device)
         size = max(self.state_values, BLOCK)
         kind = torch.float32 if state_bits == 32 else torch.float8_e4m3fn
         self.m = torch.zeros(size, dtype=torch.float32, device=device).to(kind)
@@ -326,7 +326,7 @@ class AdamW:
         for name, t in given.items():
             if t is not None:
                 getattr(self, name).copy_(t)
-        self._step.copy_(torch.tensor([int(steps), 0], dtype=torch.int32))
+        self._step[0] = int(steps)
 
 
 def fit_siblings(bits, label, k, n_features, *, steps=200, batch=None, lr=0.05, l1=0.0, weight_decay=0.0, weight=None, table_dtype=torch.float32,

@@ -330,9 +330,9 @@ def test_adamw_32(which, t):
 def restated_rounding(x, scale, chance):
     y = (x / scale).astype(np.float32)
     a = np.abs(y)
-    normal = ((a.view(np.uint32) + (chance << 4 | 8).astype(np.uint32)) & np.uint32(0xfff00000)).view(np.float32)
-    small = (np.floor(a * np.float32(512) + (chance.astype(np.float32) + np.float32(0.5)) * np.float32(2.0 ** -16)) * np.float32(2.0 ** -9)).astype(np.float32)
-    return np.copysign(np.where(a < 2.0 ** -6, small, normal), y)
+    up = np.where(a < 2.0 ** -6, np.float32(2.0 ** -6), np.float32(0))       # below 2^-6 codes are as far apart as above it
+    bits = ((a + up).view(np.uint32) + (chance << 4 | 8).astype(np.uint32)) & np.uint32(0xfff00000)
+    return np.copysign(bits.view(np.float32) - up, y)
 
 
 def restated_scale(x):
