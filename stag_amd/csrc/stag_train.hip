@@ -628,14 +628,14 @@ __device__ __forceinline__ float log_one_plus(float e) {
 // flight together; loss sums stay in its registers until the workgroup adds them up in a fixed order and stores one
 // partial row of K sums.  Scores are read only where the row trains (a place of the tree has a handful of siblings among
 // the thousands of a level); the rest of the gradient is zeros, so what bounds a level's loss is writing the gradient.
-template <typename T, int V>
-__global__ __launch_bounds__(256) void k_loss(const float *scores, int64_t score_stride, int64_t m, int k, const int32_t *label,
+template <typename T, int V, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_loss(const float *scores, int64_t score_stride, int64_t m, int k, const int32_t *label,
                                               const int32_t *siblings, const float *weight, float scale, float *loss, T *grad,
                                               int64_t grad_stride, int ct) {
     constexpr int ROWS_AT_ONCE = 4;
     typedef __attribute__((ext_vector_type(V))) T out_t;
-    __shared__ float part[256 * V];
-    const int cv = threadIdx.x % ct, r = threadIdx.x / ct, rp = 256 / ct;
+    __shared__ float part[THREADS * V];
+    const int cv = threadIdx.x % ct, r = threadIdx.x / ct, rp = THREADS / ct;
     const int c0 = (blockIdx.y * ct + cv) * V;
     float sum[V] = {};
     if (r < rp && c0 < k) {
@@ -702,19 +702,19 @@ __global__ __launch_bounds__(256) void k_loss(const float *scores, int64_t score
     }
 }
 
-// adds up the partial rows: 32 columns a workgroup, every eighth row to a thread, then the eight sums in order
-__global__ __launch_bounds__(256) void k_loss_join(const float *part, int n_parts, int k, float *loss) {
-    __shared__ double sums[8][32];
+// adds up the partial rows: 32 columns a workgroup, every 32nd row to a thread, then the 32 sums in order
+__global__ __launch_bounds__(1024) void k_loss_join(const float *part, int n_parts, int k, float *loss) {
+    __shared__ double sums[32][33];
     const int col = threadIdx.x & 31, g = threadIdx.x >> 5, c = blockIdx.x * 32 + col;
     double s = 0.0;
     if (c < k) {
 #pragma unroll 8
-        for (int p = g; p < n_parts; p += 8) s += part[(int64_t)p * k + c];
+        for (int p = g; p < n_parts; p += 32) s += part[(int64_t)p * k + c];
     }
     sums[g][col] = s;
     __syncthreads();
     if (g == 0 && c < k) {
-        for (int q = 1; q < 8; ++q) s += sums[q][col];
+        for (int q = 1; q < 32; ++q) s += sums[q][col];
         loss[c] = (float)s;
     }
 }
@@ -729,6 +729,7 @@ struct AdamwArgs {
     const stag_adamw_tensor_t *tensors;
     const stag_adamw_tile_t *tiles;
     int64_t n_tiles;
+    int split;                  // waves to a tile: 1, or 4 (a block each) when there are few
     void *m, *v;
     float *m_scale, *v_scale;
     int32_t *step;
@@ -864,17 +865,18 @@ __global__ __launch_bounds__(256) void k_adamw(AdamwArgs a) {
     const float c1 = a.lr / -expm1f((float)t * a.log_beta1);
     const float c2 = 1.f / sqrtf(-expm1f((float)t * a.log_beta2));
     const uint32_t salt = (uint32_t)t * 0x9E3779B9u;
-    for (int64_t w = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); w < a.n_tiles; w += (int64_t)gridDim.x * 4) {
-        const stag_adamw_tile_t tile = a.tiles[w];
+    for (int64_t w = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); w < a.n_tiles * a.split; w += (int64_t)gridDim.x * 4) {
+        const stag_adamw_tile_t tile = a.tiles[a.split == 1 ? w : w / 4];
         const stag_adamw_tensor_t d = a.tensors[tile.tensor];
         const int64_t at0 = (int64_t)tile.tile * STAG_ADAMW_TILE, s0 = d.state_at + at0;
         const bool vec_p = ((uintptr_t)d.param & (d.param_type == STAG_F32 ? 15 : 7)) == 0;
         const bool vec_g = ((uintptr_t)d.grad & (d.grad_type == STAG_F32 ? 15 : 7)) == 0;
         const float keep = 1.f - a.lr * d.weight_decay, shrink = a.lr * d.l1;
-        const int blocks = (int)min((int64_t)STAG_ADAMW_TILE / STAG_ADAMW_BLOCK, (d.count - at0 + STAG_ADAMW_BLOCK - 1) / STAG_ADAMW_BLOCK);
+        const int from = a.split == 1 ? 0 : (int)(w & 3);
+        const int blocks = (int)min((int64_t)(a.split == 1 ? STAG_ADAMW_TILE / STAG_ADAMW_BLOCK : from + 1), (d.count - at0 + STAG_ADAMW_BLOCK - 1) / STAG_ADAMW_BLOCK);
         const bool inside = at0 + STAG_ADAMW_TILE <= d.count;
 #pragma unroll 1
-        for (int b0 = 0; b0 < blocks; b0 += GROUP) {
+        for (int b0 = from; b0 < blocks; b0 += GROUP) {
             u32x4 raw_p[GROUP], raw_g[GROUP], raw_m[GROUP], raw_v[GROUP];
             float ms[GROUP], vs[GROUP];
 #pragma unroll
@@ -1106,19 +1108,22 @@ int lookup(const ProductArgs &a, hipStream_t st) {
 
 // how k_loss is laid over [m][k]
 struct LossPlan {
-    int v, ct;
+    int v, ct, threads;
     unsigned gx, gy;
 };
 
 LossPlan loss_plan(int64_t m, int32_t k, int v) {
     LossPlan p;
-    p.v = v;
+    // few values: one workgroup a column tile, whose sums are the result without a second launch; the more threads, the
+    // fewer values one after the other (300 x 8: 9.3 us with 256 threads of four columns, 4.7 with 1,024 of one)
+    const bool few = m * (int64_t)k <= 16384;
+    p.threads = few ? 1024 : 256;
+    p.v = few ? 1 : v;
     const int64_t cols = ceil_div(k, p.v);
-    p.ct = (int)(cols < 256 ? cols : 256);
+    p.ct = (int)(cols < p.threads ? cols : p.threads);
     p.gy = (unsigned)ceil_div(cols, p.ct);
-    const int64_t passes = ceil_div(m, 256 / p.ct), wanted = 2048 / p.gy > 0 ? 2048 / p.gy : 1;
-    // few values: one workgroup a column tile, whose sums are the result without a second launch
-    p.gx = (unsigned)(m * (int64_t)k <= 16384 ? 1 : passes < wanted ? passes : wanted);
+    const int64_t passes = ceil_div(m, p.threads / p.ct), wanted = 1024 / p.gy > 0 ? 1024 / p.gy : 1;
+    p.gx = (unsigned)(few ? 1 : passes < wanted ? passes : wanted);
     return p;
 }
 
@@ -1127,16 +1132,18 @@ int loss_typed(const LossPlan &p, const float *d_scores, int64_t score_stride, i
                const float *d_weight, float scale, float *d_loss, void *d_grad, int64_t grad_stride, float *parts, hipStream_t st) {
     float *to = d_loss && p.gx > 1 ? parts : d_loss;
     const dim3 grid(p.gx, p.gy);
-    if (p.v == 8) {
-        if constexpr (sizeof(T) == 2)
-            k_loss<T, 8><<<grid, 256, 0, st>>>(d_scores, score_stride, m, k, d_label, d_siblings, d_weight, scale, to, (T *)d_grad, grad_stride, p.ct);
-    } else if (p.v == 4)
-        k_loss<T, 4><<<grid, 256, 0, st>>>(d_scores, score_stride, m, k, d_label, d_siblings, d_weight, scale, to, (T *)d_grad, grad_stride, p.ct);
+    auto launch = [&](auto kernel) { kernel<<<grid, p.threads, 0, st>>>(d_scores, score_stride, m, k, d_label, d_siblings, d_weight, scale, to, (T *)d_grad, grad_stride, p.ct); };
+    if (p.threads == 1024)
+        launch(k_loss<T, 1, 1024>);
+    else if (p.v == 1)
+        launch(k_loss<T, 1, 256>);
+    else if (p.v == 4 || sizeof(T) == 4)
+        launch(k_loss<T, 4, 256>);
     else
-        k_loss<T, 1><<<grid, 256, 0, st>>>(d_scores, score_stride, m, k, d_label, d_siblings, d_weight, scale, to, (T *)d_grad, grad_stride, p.ct);
+        launch(k_loss<T, sizeof(T) == 4 ? 4 : 8, 256>);
     HIP_TRY(hipGetLastError());
     if (d_loss && p.gx > 1) {
-        k_loss_join<<<(unsigned)ceil_div(k, 32), 256, 0, st>>>(parts, (int)p.gx, k, d_loss);
+        k_loss_join<<<(unsigned)ceil_div(k, 32), 1024, 0, st>>>(parts, (int)p.gx, k, d_loss);
         HIP_TRY(hipGetLastError());
     }
     return STAG_OK;
@@ -1278,7 +1285,9 @@ int stag_adamw_dev(const stag_adamw_tensor_t *d_tensors, const stag_adamw_tile_t
     a.log_beta1 = (float)std::log(beta1);
     a.log_beta2 = (float)std::log(beta2);
     a.eps = (float)eps;
-    const unsigned grid = (unsigned)(n_tiles < 4 * 4096 ? ceil_div(n_tiles, 4) : 4096);
+    a.split = n_tiles <= 2048 ? 4 : 1;
+    const int64_t waves = n_tiles * a.split;
+    const unsigned grid = (unsigned)(waves < 4 * 4096 ? ceil_div(waves, 4) : 4096);
     if (state_bits == 32)
         k_adamw<32><<<grid, 256, 0, (hipStream_t)stream>>>(a);
     else

@@ -17,7 +17,7 @@ All functions take torch tensors on one GPU, enqueue their work on that GPU's cu
 they take no part in autograd.  With their outputs given (``out=``) or allocated under capture they can be recorded into a
 HIP graph.  Inputs whose rows are not contiguous are copied first; outputs have to be as documented.
 """
-import ctypes
+import functools
 import math
 
 import numpy as np
@@ -31,18 +31,29 @@ _TENSOR = np.dtype([("param", "<u8"), ("grad", "<u8"), ("count", "<i8"), ("state
                     ("param_type", "<i4"), ("grad_type", "<i4")])      # stag_adamw_tensor_t
 
 
+_Tensor = torch.Tensor
+_BITS = (torch.int32, torch.uint32)
+_raw_stream = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream(i).cuda_stream without the objects
+_current = torch._C._cuda_getDevice
+
+
 def _need(cond, msg, *args):
     if not cond:
         raise ValueError(msg % args)
 
 
 def _is(name, t, dtypes, dim):
-    if not isinstance(t, torch.Tensor):
+    if not isinstance(t, _Tensor):
         raise TypeError("%s must be a torch tensor" % name)
     dtypes = dtypes if isinstance(dtypes, tuple) else (dtypes,)
     if t.dtype not in dtypes:
         raise TypeError("%s is %s: %s is wanted" % (name, t.dtype, " or ".join(str(d) for d in dtypes)))
     _need(t.dim() == dim, "%s has %d dimensions: %d are wanted", name, t.dim(), dim)
+
+
+def _plain(t, dtype, shape, gpu):
+    """Whether t is a contiguous tensor of this type and shape on this GPU: nothing to check or copy."""
+    return type(t) is _Tensor and t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == gpu
 
 
 def _one_gpu(**tensors):
@@ -89,36 +100,16 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _work(nbytes, device):
+@functools.lru_cache(maxsize=65536)
+def _workspace(name, *sizes):
+    nbytes = getattr(_lib.train_lib(), name)(*sizes)
     if nbytes < 0:
         _lib.check_train(int(nbytes))
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    return nbytes
 
 
-class _on:
-    """The tensors' GPU as the current one, and its current stream."""
-
-    def __init__(self, device):
-        self.guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
-        self.stream = torch.cuda.current_stream(device).cuda_stream
-
-    def __enter__(self):
-        if self.guard:
-            self.guard.__enter__()
-        return self.stream
-
-    def __exit__(self, *a):
-        if self.guard:
-            self.guard.__exit__(*a)
-
-
-def row_scores(bits, table, bias=None, *, scale=1.0, rows=None, out=None):
-    """scores[i, c] = scale * (sum of table[f, c] over the features f of row rows[i] of bits) + bias[c], float32 [m, k]
-    (the sum of run_logistic_prediction, stag/classify.py:22-27; an embedding lookup summed over a row's tokens).
-
-    bits: int32 / uint32 [n, words]; table: float32, bfloat16 or float16 [n_features, k]; bias: float32 [k]; rows: int32 [m], any
-    order, repeats allowed, an index outside 0..n-1 is padding and scores 0 (default: all rows of bits)."""
-    _is("bits", bits, (torch.int32, torch.uint32), 2)
+def _check_scores(bits, table, bias, rows, out):
+    _is("bits", bits, _BITS, 2)
     _is("table", table, tuple(_TYPES), 2)
     n_features, k = table.shape
     _need(n_features >= 1 and k >= 1, "table is empty: %s", tuple(table.shape))
@@ -131,18 +122,61 @@ def row_scores(bits, table, bias=None, *, scale=1.0, rows=None, out=None):
         rows = rows.contiguous()
     m = bits.shape[0] if rows is None else rows.shape[0]
     score_stride = k if out is None else _out_rows("out", out, (m, k), torch.float32)
-    device = _one_gpu(bits=bits, table=table, bias=bias, rows=rows, out=out)
+    _one_gpu(bits=bits, table=table, bias=bias, rows=rows, out=out)
     bits, row_stride = _packed(bits, n_features)
     table, table_stride = _rows(table)
-    lib = _lib.train_lib()
-    with _on(device) as stream:
-        if out is None:
-            out = torch.empty((m, k), dtype=torch.float32, device=device)
-        need = lib.stag_row_scores_workspace(m, n_features, k, _TYPES[table.dtype])
-        work = _work(need, device)
-        _lib.check_train(lib.stag_row_scores_dev(_ptr(bits), bits.shape[0], row_stride, n_features, _ptr(rows), m, _ptr(table), _TYPES[table.dtype],
-                                                 table_stride, _ptr(bias), k, float(scale), _ptr(out), score_stride, _ptr(work), need, stream))
+    return bits, table, bias, rows, row_stride, table_stride, score_stride
+
+
+def row_scores(bits, table, bias=None, *, scale=1.0, rows=None, out=None):
+    """scores[i, c] = scale * (sum of table[f, c] over the features f of row rows[i] of bits) + bias[c], float32 [m, k]
+    (the sum of run_logistic_prediction, stag/classify.py:22-27; an embedding lookup summed over a row's tokens).
+
+    bits: int32 / uint32 [n, words]; table: float32, bfloat16 or float16 [n_features, k]; bias: float32 [k]; rows: int32 [m], any
+    order, repeats allowed, an index outside 0..n-1 is padding and scores 0 (default: all rows of bits)."""
+    gpu = bits.get_device() if type(bits) is _Tensor else -1
+    if (gpu >= 0 and type(table) is _Tensor and bits.dim() == table.dim() == 2 and bits.dtype in _BITS and table.dtype in _TYPES and table.numel() and out is None
+            and bits.is_contiguous() and table.is_contiguous() and table.get_device() == gpu and not bits.shape[1] % 4 and bits.shape[1] * 32 >= table.shape[0]
+            and (bias is None or _plain(bias, torch.float32, table.shape[1:], gpu))
+            and (rows is None or (rows.dim() == 1 and _plain(rows, torch.int32, rows.shape, gpu)))):
+        row_stride, table_stride, score_stride = bits.shape[1], table.shape[1], table.shape[1]
+    else:
+        bits, table, bias, rows, row_stride, table_stride, score_stride = _check_scores(bits, table, bias, rows, out)
+        gpu = bits.get_device()
+    if gpu != _current():
+        with torch.cuda.device(gpu):
+            return row_scores(bits, table, bias, scale=scale, rows=rows, out=out)
+    n_features, k = table.shape
+    m = bits.shape[0] if rows is None else rows.shape[0]
+    kind = _TYPES[table.dtype]
+    if out is None:
+        out = torch.empty((m, k), dtype=torch.float32, device=bits.device)
+    need = _workspace("stag_row_scores_workspace", m, n_features, k, kind)
+    work = torch.empty(need, dtype=torch.uint8, device=bits.device) if need else None
+    _lib.check_train(_lib.train_lib().stag_row_scores_dev(bits.data_ptr(), bits.shape[0], row_stride, n_features, _ptr(rows), m, table.data_ptr(), kind, table_stride,
+                                                          _ptr(bias), k, float(scale), out.data_ptr(), score_stride, _ptr(work), need, _raw_stream(gpu)))
     return out
+
+
+def _check_grad(bits, grad, n_features, rows, out):
+    _is("bits", bits, _BITS, 2)
+    _is("grad", grad, tuple(_TYPES), 2)
+    m, k = grad.shape
+    _need(n_features >= 1 and k >= 1, "no features (%d) or no classifiers (%d)", n_features, k)
+    if rows is not None:
+        _is("rows", rows, torch.int32, 1)
+        rows = rows.contiguous()
+    batch = bits.shape[0] if rows is None else rows.shape[0]
+    _need(m == batch, "grad has %d rows, the batch %d", m, batch)
+    table_grad, bias_grad = out if out is not None else (None, None)
+    stride = k
+    if out is not None:
+        stride = _out_rows("out[0]", table_grad, (n_features, k), torch.float32)
+        _out_rows("out[1]", bias_grad, (k,), torch.float32)
+    _one_gpu(bits=bits, grad=grad, rows=rows, table_grad=table_grad, bias_grad=bias_grad)
+    bits, row_stride = _packed(bits, n_features)
+    grad, grad_stride = _rows(grad)
+    return bits, grad, rows, row_stride, grad_stride, stride
 
 
 def row_scores_grad(bits, grad, n_features, *, scale=1.0, rows=None, out=None):
@@ -151,43 +185,31 @@ def row_scores_grad(bits, grad, n_features, *, scale=1.0, rows=None, out=None):
 
     grad: float32, bfloat16 or float16 [m, k].  Padding rows (see row_scores) take part in neither, whatever grad holds for
     them.  out: a pair of tensors to overwrite."""
-    _is("bits", bits, (torch.int32, torch.uint32), 2)
-    _is("grad", grad, tuple(_TYPES), 2)
     n_features = int(n_features)
+    gpu = bits.get_device() if type(bits) is _Tensor else -1
+    if (gpu >= 0 and type(grad) is _Tensor and bits.dim() == grad.dim() == 2 and bits.dtype in _BITS and grad.dtype in _TYPES and grad.numel() and n_features >= 1
+            and bits.is_contiguous() and grad.is_contiguous() and grad.get_device() == gpu and not bits.shape[1] % 4 and bits.shape[1] * 32 >= n_features
+            and (bits.shape[:1] == grad.shape[:1] if rows is None else _plain(rows, torch.int32, grad.shape[:1], gpu))
+            and (out is None or (_plain(out[0], torch.float32, (n_features, grad.shape[1]), gpu) and _plain(out[1], torch.float32, grad.shape[1:], gpu)))):
+        row_stride, grad_stride, stride = bits.shape[1], grad.shape[1], grad.shape[1]
+    else:
+        bits, grad, rows, row_stride, grad_stride, stride = _check_grad(bits, grad, n_features, rows, out)
+        gpu = bits.get_device()
+    if gpu != _current():
+        with torch.cuda.device(gpu):
+            return row_scores_grad(bits, grad, n_features, scale=scale, rows=rows, out=out)
     m, k = grad.shape
-    _need(n_features >= 1 and k >= 1, "no features (%d) or no classifiers (%d)", n_features, k)
-    if rows is not None:
-        _is("rows", rows, torch.int32, 1)
-        rows = rows.contiguous()
-    _need(m == (bits.shape[0] if rows is None else rows.shape[0]), "grad has %d rows, the batch %d", m, bits.shape[0] if rows is None else rows.shape[0])
-    table_grad, bias_grad = out if out is not None else (None, None)
-    stride = k
-    if out is not None:
-        stride = _out_rows("out[0]", table_grad, (n_features, k), torch.float32)
-        _out_rows("out[1]", bias_grad, (k,), torch.float32)
-    device = _one_gpu(bits=bits, grad=grad, rows=rows, table_grad=table_grad, bias_grad=bias_grad)
-    bits, row_stride = _packed(bits, n_features)
-    grad, grad_stride = _rows(grad)
-    lib = _lib.train_lib()
-    with _on(device) as stream:
-        if out is None:
-            table_grad = torch.empty((n_features, k), dtype=torch.float32, device=device)
-            bias_grad = torch.empty((k,), dtype=torch.float32, device=device)
-        need = lib.stag_row_scores_grad_workspace(m, n_features, k, _TYPES[grad.dtype])
-        work = _work(need, device)
-        _lib.check_train(lib.stag_row_scores_grad_dev(_ptr(bits), bits.shape[0], row_stride, n_features, _ptr(rows), m, _ptr(grad), _TYPES[grad.dtype],
-                                                      grad_stride, k, float(scale), _ptr(table_grad), stride, _ptr(bias_grad), _ptr(work), need, stream))
-    return table_grad, bias_grad
+    kind = _TYPES[grad.dtype]
+    if out is None:
+        out = torch.empty((n_features, k), dtype=torch.float32, device=bits.device), torch.empty(k, dtype=torch.float32, device=bits.device)
+    need = _workspace("stag_row_scores_grad_workspace", m, n_features, k, kind)
+    work = torch.empty(need, dtype=torch.uint8, device=bits.device) if need else None
+    _lib.check_train(_lib.train_lib().stag_row_scores_grad_dev(bits.data_ptr(), bits.shape[0], row_stride, n_features, _ptr(rows), m, grad.data_ptr(), kind, grad_stride, k,
+                                                               float(scale), out[0].data_ptr(), stride, out[1].data_ptr(), _ptr(work), need, _raw_stream(gpu)))
+    return out[0], out[1]
 
 
-def sibling_loss(scores, label, *, siblings=None, weight=None, scale=1.0, grad_dtype=None, out=None):
-    """Logistic loss of "this sibling or one of the others" and its gradient: (loss float32 [k], grad [m, k]).
-
-    Row i trains the columns siblings[i, 0] <= c < siblings[i, 1] (int32 [m, 2]; children of a node are neighbours in
-    breadth-first numbering; default: all k) with target 1 for c == label[i] (int32 [m]) and 0 for the others; a label
-    outside them makes the row a negative example for all.  loss[c] = scale * sum of weight[i] * softplus(+-score);
-    grad is d(sum of loss)/d(scores) of type grad_dtype (default float32), 0 where a row does not train, and scores are not
-    read there.  weight: float32 [m].  out: a pair of tensors to overwrite."""
+def _check_loss(scores, label, siblings, weight, dtype, out):
     _is("scores", scores, torch.float32, 2)
     _is("label", label, torch.int32, 1)
     m, k = scores.shape
@@ -202,26 +224,46 @@ def sibling_loss(scores, label, *, siblings=None, weight=None, scale=1.0, grad_d
         _is("weight", weight, torch.float32, 1)
         _need(weight.shape[0] == m, "weight has %d values, scores %d rows", weight.shape[0], m)
         weight = weight.contiguous()
-    loss, grad = out if out is not None else (None, None)
-    dtype = grad_dtype or (grad.dtype if grad is not None else torch.float32)
     if dtype not in _TYPES:
         raise TypeError("grad_dtype is %s: %s is wanted" % (dtype, " or ".join(str(d) for d in _TYPES)))
+    loss, grad = out if out is not None else (None, None)
     grad_stride = k
     if out is not None:
         _out_rows("out[0]", loss, (k,), torch.float32)
         grad_stride = _out_rows("out[1]", grad, (m, k), dtype)
-    device = _one_gpu(scores=scores, label=label, siblings=siblings, weight=weight, loss=loss, grad=grad)
+    _one_gpu(scores=scores, label=label, siblings=siblings, weight=weight, loss=loss, grad=grad)
     scores, score_stride = _rows(scores)
-    lib = _lib.train_lib()
-    with _on(device) as stream:
-        if out is None:
-            loss = torch.empty((k,), dtype=torch.float32, device=device)
-            grad = torch.empty((m, k), dtype=dtype, device=device)
-        need = lib.stag_sibling_loss_workspace(m, k)
-        work = _work(need, device)
-        _lib.check_train(lib.stag_sibling_loss_dev(_ptr(scores), score_stride, m, k, _ptr(label), _ptr(siblings), _ptr(weight), float(scale),
-                                                   _ptr(loss), _ptr(grad), _TYPES[dtype], grad_stride, _ptr(work), need, stream))
-    return loss, grad
+    return scores, label, siblings, weight, score_stride, grad_stride
+
+
+def sibling_loss(scores, label, *, siblings=None, weight=None, scale=1.0, grad_dtype=None, out=None):
+    """Logistic loss of "this sibling or one of the others" and its gradient: (loss float32 [k], grad [m, k]).
+
+    Row i trains the columns siblings[i, 0] <= c < siblings[i, 1] (int32 [m, 2]; children of a node are neighbours in
+    breadth-first numbering; default: all k) with target 1 for c == label[i] (int32 [m]) and 0 for the others; a label
+    outside them makes the row a negative example for all.  loss[c] = scale * sum of weight[i] * softplus(+-score);
+    grad is d(sum of loss)/d(scores) of type grad_dtype (default float32), 0 where a row does not train, and scores are not
+    read there.  weight: float32 [m].  out: a pair of tensors to overwrite."""
+    dtype = grad_dtype or (out[1].dtype if out is not None else torch.float32)
+    gpu = scores.get_device() if type(scores) is _Tensor else -1
+    if (gpu >= 0 and scores.dtype is torch.float32 and scores.dim() == 2 and scores.numel() and scores.is_contiguous() and dtype in _TYPES and out is None
+            and _plain(label, torch.int32, scores.shape[:1], gpu) and (siblings is None or _plain(siblings, torch.int32, (scores.shape[0], 2), gpu))
+            and (weight is None or _plain(weight, torch.float32, scores.shape[:1], gpu))):
+        score_stride = grad_stride = scores.shape[1]
+    else:
+        scores, label, siblings, weight, score_stride, grad_stride = _check_loss(scores, label, siblings, weight, dtype, out)
+        gpu = scores.get_device()
+    if gpu != _current():
+        with torch.cuda.device(gpu):
+            return sibling_loss(scores, label, siblings=siblings, weight=weight, scale=scale, grad_dtype=dtype, out=out)
+    m, k = scores.shape
+    if out is None:
+        out = torch.empty(k, dtype=torch.float32, device=scores.device), torch.empty((m, k), dtype=dtype, device=scores.device)
+    need = _workspace("stag_sibling_loss_workspace", m, k)
+    work = torch.empty(need, dtype=torch.uint8, device=scores.device) if need else None
+    _lib.check_train(_lib.train_lib().stag_sibling_loss_dev(scores.data_ptr(), score_stride, m, k, label.data_ptr(), _ptr(siblings), _ptr(weight), float(scale), out[0].data_ptr(),
+                                                            out[1].data_ptr(), _TYPES[dtype], grad_stride, _ptr(work), need, _raw_stream(gpu)))
+    return out[0], out[1]
 
 
 class AdamW:
@@ -246,7 +288,10 @@ class AdamW:
         for x in decay + l1:
             _need(math.isfinite(x) and x >= 0, "weight_decay and l1 are not negative: got %r", x)
         self.lr, self.betas, self.eps, self.state_bits = lr, tuple(betas), eps, state_bits
-        self._check()
+        b1, b2 = self.betas
+        _need(math.isfinite(lr) and lr >= 0, "lr = %r", lr)
+        _need(0 < b1 < 1 and 0 < b2 < 1, "betas = %r: not inside (0, 1)", betas)
+        _need(math.isfinite(eps) and eps >= 0, "eps = %r", eps)
         spans = []
         for j, (p, g) in enumerate(zip(params, grads)):
             for name, t in (("params[%d]" % j, p), ("grads[%d]" % j, g)):
@@ -286,27 +331,24 @@ class AdamW:
         self._step = torch.zeros(STEP_WORDS, dtype=torch.int32, device=device)
         size = max(self.state_values, BLOCK)
         kind = torch.float32 if state_bits == 32 else torch.float8_e4m3fn
-        self.m = torch.zeros(size, dtype=torch.float32, device=device).to(kind)
-        self.v = torch.zeros(size, dtype=torch.float32, device=device).to(kind)
-        self.m_scale = self.v_scale = None
+        self._m = torch.zeros(size, dtype=torch.float32, device=device).to(kind)
+        self._v = torch.zeros(size, dtype=torch.float32, device=device).to(kind)
+        self._m_scale = self._v_scale = None
         if state_bits == 8:
-            self.m_scale = torch.ones(size // BLOCK, dtype=torch.float32, device=device)
-            self.v_scale = torch.ones(size // BLOCK, dtype=torch.float32, device=device)
+            self._m_scale = torch.ones(size // BLOCK, dtype=torch.float32, device=device)
+            self._v_scale = torch.ones(size // BLOCK, dtype=torch.float32, device=device)
+        self._where = (self._tensors.data_ptr(), self._tiles.data_ptr(), self._n_tiles, state_bits, self._m.data_ptr(), self._v.data_ptr(), _ptr(self._m_scale),
+                       _ptr(self._v_scale), self._step.data_ptr())
 
-    def _check(self):
-        b1, b2 = self.betas
-        _need(math.isfinite(self.lr) and self.lr >= 0, "lr = %r", self.lr)
-        _need(0 < b1 < 1 and 0 < b2 < 1, "betas = %r: not inside (0, 1)", self.betas)
-        _need(math.isfinite(self.eps) and self.eps >= 0, "eps = %r", self.eps)
+    m, v, m_scale, v_scale = (property(lambda self, name=name: getattr(self, name)) for name in ("_m", "_v", "_m_scale", "_v_scale"))
 
     def step(self):
         """One step with the gradients as they stand."""
-        self._check()
-        lib = _lib.train_lib()
-        with _on(self.device) as stream:
-            _lib.check_train(lib.stag_adamw_dev(_ptr(self._tensors), _ptr(self._tiles), self._n_tiles, self.state_bits, _ptr(self.m), _ptr(self.v),
-                                                _ptr(self.m_scale), _ptr(self.v_scale), _ptr(self._step), float(self.lr), float(self.betas[0]),
-                                                float(self.betas[1]), float(self.eps), stream))
+        gpu = self.device.index
+        if gpu != _current():
+            with torch.cuda.device(gpu):
+                return self.step()
+        _lib.check_train(_lib.train_lib().stag_adamw_dev(*self._where, self.lr, *self.betas, self.eps, _raw_stream(gpu)))
 
     @property
     def steps(self):
