@@ -7,9 +7,6 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
-#ifdef STAG_TUNE
-#include <cstdlib>
-#endif
 
 namespace {
 
@@ -145,23 +142,28 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x, int lane) {
 // turns out of their packed rows as it goes; TURNED: a feature, from bits that k_turn has laid out by feature before.
 enum Source { ROWS, TURN, TURNED };
 
-// A workgroup of four waves makes 4 MT x 32 rows of the result by NT x 32 columns; a wave its own MT row tiles.  A K-step
+constexpr int W = 8;      // waves of a workgroup
+
+// A workgroup of W waves makes W MT x 32 rows of the result by NT x 32 columns; a wave its own MT row tiles.  A K-step
 // is 64 terms of the sum: two words of bits, one for each half of the wave (the matrix instruction takes 8 terms from
 // each half), in four instructions of 16 terms.  The workgroup loads the coefficients of U K-steps, 64 U x 32 NT, cuts them into pieces
 // and stores them to LDS in operand order; the next ones are in flight while the matrix cores work on these.
-template <int TYPE, Source SRC, int MT, int NT, int U>
-__global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
+template <int TYPE, Source SRC, int MT, int NT>
+__global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
     typedef typename Raw<TYPE>::type raw_t;
     constexpr bool GRAD = SRC != ROWS;
-    constexpr int P = TYPE == STAG_F32 ? 3 : 1, COLS = 32 * NT, GROUPS = 256 / COLS, BUFFERS = U == 1 ? 2 : 1;
+    constexpr int P = TYPE == STAG_F32 ? 3 : 1, COLS = 32 * NT, U = SRC == TURN ? 2 : 4;
+    // a thread's share of the 8 x COLS groups of 8 terms of U K-steps; PASSES of them are of one K-step
+    constexpr int ITEMS = U * 8 * COLS / (64 * W), PASSES = 8 * COLS > 64 * W ? 8 * COLS / (64 * W) : 1;
+    static_assert(ITEMS >= 1, "a group for every thread");
     typedef __attribute__((ext_vector_type(MT))) uint32_t words_t;          // TURN: a lane loads the words of its wave's row tiles at once
-    __shared__ u32x4 lds[BUFFERS][U][P][8][COLS];
-    __shared__ float sums[GRAD ? 256 : 1];
+    __shared__ u32x4 lds[U][P][8][COLS];
+    __shared__ float sums[GRAD ? 64 * W : 1];
     __shared__ int found;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int64_t tile0 = ((int64_t)blockIdx.x * 4 + wave) * MT;           // this wave's first row tile
+    const int64_t tile0 = ((int64_t)blockIdx.x * W + wave) * MT;           // this wave's first row tile
     const int64_t out_rows = GRAD ? a.n_features : a.m;
-    const int col = threadIdx.x % COLS, group = threadIdx.x / COLS, c0 = blockIdx.y * COLS, c = c0 + col;
+    const int col = threadIdx.x % COLS, c0 = blockIdx.y * COLS, c = c0 + col;
     const bool c_ok = c < a.k;
     const int64_t limit = GRAD ? a.m : a.n_features;                       // terms of the sum
     constexpr int UNIT = SRC == TURN ? 1 : 4;                              // K-steps of a step of the plan
@@ -184,30 +186,34 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
     float column_sum = 0.f;
 
     // Buffer loads: one 32-bit offset a lane, and what lies behind the last term or column reads as zero.
-    raw_t b[U][NT][8];
-    uint32_t at_b[NT];
+    raw_t b[ITEMS][8];
+    auto step_of = [&](int i) { return (i * 64 * W + wave * 64) / (8 * COLS); };                       // the same for a whole wave
+    auto group_of = [&](int i) -> int { return (i * 64 * W + threadIdx.x) % (8 * COLS) / COLS; };
+    uint32_t at_b[PASSES];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        const int g = group + i * GROUPS, r0 = 4 * (g >> 1) + (g & 1) * (GRAD ? 32 : 128);
+    for (int i = 0; i < PASSES; ++i) {
+        const int g = group_of(i), r0 = 4 * (g >> 1) + (g & 1) * (GRAD ? 32 : 128);
         at_b[i] = c_ok ? (uint32_t)((r0 * (int)a.mat_stride + c) * (int)sizeof(raw_t)) : NOWHERE;
     }
     const uint32_t row_b = (uint32_t)a.mat_stride * sizeof(raw_t);
-    auto load_b = [&](int u, int ks) {
-        const int64_t t0 = term(ks, 0);
-        const auto from = buffer((const raw_t *)a.mat + t0 * a.mat_stride, (limit - t0) * row_b);
+    auto load_b = [&](int ks) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
+        for (int i = 0; i < ITEMS; ++i) {
+            const int64_t t0 = term(ks + step_of(i), 0);
+            const auto from = buffer((const raw_t *)a.mat + t0 * a.mat_stride, (limit - t0) * row_b);
 #pragma unroll
-            for (int q = 0; q < 8; ++q) b[u][i][q] = load_raw<raw_t>(from, at_b[i] + ((q >> 1) + 16 * (q & 1)) * row_b);
+            for (int q = 0; q < 8; ++q) b[i][q] = load_raw<raw_t>(from, at_b[i % PASSES] + ((q >> 1) + 16 * (q & 1)) * row_b);
+        }
     };
-    // `real`: which of the K-step's rows are no padding (GRAD); the others are zeros, whatever the memory holds
-    auto store_b = [&](int buf, int u, uint64_t real) {
+    // `real_at`: which of a K-step's rows are no padding (GRAD); the others are zeros, whatever the memory holds
+    auto store_b = [&](auto real_at) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const int g = group + i * GROUPS;
-            raw_t(&v)[8] = b[u][i];
+        for (int i = 0; i < ITEMS; ++i) {
+            const int u = step_of(i), g = group_of(i);
+            raw_t(&v)[8] = b[i];
             if constexpr (GRAD) {
-                if (a.rows && real != ~0ull) {
+                const uint64_t real = SRC == TURN || a.rows ? real_at(u) : ~0ull;      // TURN: a part may end inside the U K-steps
+                if (real != ~0ull) {
                     const uint32_t there = (uint32_t)(real >> (32 * (g & 1) + 4 * (g >> 1)));
 #pragma unroll
                     for (int q = 0; q < 8; ++q)
@@ -252,9 +258,9 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
                     p1[j] = high_halves(y[2 * j], y[2 * j + 1]);
                     p2[j] = high_halves(z[2 * j], z[2 * j + 1]);
                 }
-                lds[buf][u][0][g][col] = p0;
-                lds[buf][u][P > 1 ? 1 : 0][g][col] = p1;
-                lds[buf][u][P > 2 ? 2 : 0][g][col] = p2;
+                lds[u][0][g][col] = p0;
+                lds[u][P > 1 ? 1 : 0][g][col] = p1;
+                lds[u][P > 2 ? 2 : 0][g][col] = p2;
             } else {
                 constexpr uint32_t EXPONENT = TYPE == STAG_BF16 ? 0x7f807f80u : 0x7c007c00u, ONE = TYPE == STAG_BF16 ? 0x00800080u : 0x04000400u;
                 u32x4 p0;
@@ -272,11 +278,11 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
                         if (not_finite<TYPE>(p0[j] >> 16)) p0[j] &= 0x0000ffffu;
                     }
                 }
-                lds[buf][u][0][g][col] = p0;
+                lds[u][0][g][col] = p0;
             }
         }
     };
-    auto multiply = [&](int buf, int u, const uint32_t *x) {
+    auto multiply = [&](int u, const uint32_t *x) {
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             u32x4 w[MT];
@@ -286,7 +292,7 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
             for (int p = P - 1; p >= 0; --p)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const u32x4 v = lds[buf][u][p][2 * s + half][32 * n + (lane & 31)];
+                    const u32x4 v = lds[u][p][2 * s + half][32 * n + (lane & 31)];
 #pragma unroll
                     for (int t = 0; t < MT; ++t) {
                         if constexpr (TYPE == STAG_F16)
@@ -325,37 +331,27 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
             return ~0ull;
         };
         u32x4 x[MT], next[MT];
+        load_b(first);
         load_x(first >> 2, x);
-#pragma unroll
-        for (int u = 0; u < U; ++u) load_b(u, first + u);
-        if constexpr (U == 1) store_b(0, 0, real_of(first));
 #pragma unroll 1
         for (int ks = first; ks < last; ks += U) {
-            const bool more = ks + U < last, turn = ((ks + U) & 3) == 0;
-            if constexpr (U > 1) {
-#pragma unroll
-                for (int u = 0; u < U; ++u) store_b(0, u, real_of(ks + u));
-            }
+            const bool more = ks + U < last;
+            store_b([&](int u) { return real_of(ks + u); });
             __syncthreads();
-            if ((U == 4 || (ks & 3) == 0) && ks + 4 < last) load_x((ks >> 2) + 1, next);
             if (more) {
-#pragma unroll
-                for (int u = 0; u < U; ++u) load_b(u, ks + U + u);
+                load_x((ks + U) >> 2, next);
+                load_b(ks + U);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 uint32_t w[MT];
 #pragma unroll
                 for (int t = 0; t < MT; ++t) w[t] = x[t][u];
-                multiply(U == 1 ? ks & 1 : 0, u, w);
+                multiply(u, w);
             }
+            __syncthreads();
 #pragma unroll
-            for (int t = 0; t < MT; ++t) x[t] = U == 4 || turn ? next[t] : U == 2 ? __builtin_shufflevector(x[t], x[t], 2, 3, 0, 1) : __builtin_shufflevector(x[t], x[t], 1, 2, 3, 0);
-            if constexpr (U == 1) {
-                if (more) store_b((ks & 1) ^ 1, 0, real_of(ks + 1));
-            } else {
-                __syncthreads();
-            }
+            for (int t = 0; t < MT; ++t) x[t] = next[t];
         }
     } else {
         const int64_t w0 = tile0 < a.words ? tile0 : a.words - MT;
@@ -370,31 +366,31 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
             real[u] = __ballot(row[u] != nullptr);
             x[u] = row[u] ? *(const words_t *)(row[u] + w0) : (words_t)(0u);
         };
+        auto real_at = [&](int u) {
+            uint64_t r = real[0];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            load_row(u, first + u);
-            load_b(u, first + u);
-        }
+            for (int i = 1; i < U; ++i) r = u == i ? real[i] : r;
+            return r;
+        };
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_row(u, first + u);
+        load_b(first);
 #pragma unroll
         for (int u = 0; u < U; ++u) load_x(u);
 #pragma unroll
         for (int u = 0; u < U; ++u) load_row(u, first + U + u);
-        if constexpr (U == 1) store_b(0, 0, real[0]);
 #pragma unroll 1
         for (int ks = first; ks < last; ks += U) {
             const bool more = ks + U < last;
-            if constexpr (U > 1) {
-#pragma unroll
-                for (int u = 0; u < U; ++u) store_b(0, u, real[u]);
-            }
+            store_b(real_at);
             __syncthreads();
             words_t now[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) now[u] = x[u];
             if (more) {
+                load_b(ks + U);
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    load_b(u, ks + U + u);
                     load_x(u);
                     load_row(u, ks + 2 * U + u);
                 }
@@ -404,16 +400,11 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
                 uint32_t w[MT];
 #pragma unroll
                 for (int t = 0; t < MT; ++t) w[t] = transposed(now[u][t], lane);
-                multiply(U == 1 ? (ks - first) & 1 : 0, u, w);
+                multiply(u, w);
             }
-            if constexpr (U == 1) {
-                if (more) store_b(((ks - first) & 1) ^ 1, 0, real[0]);
-            } else {
-                __syncthreads();
-            }
+            __syncthreads();
         }
     }
-    __syncthreads();
 
     const bool whole = gridDim.z == 1;
     float *to = whole ? a.out : a.part + (int64_t)blockIdx.z * out_rows * a.k;
@@ -447,10 +438,10 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
         if (blockIdx.x == 0) {
             sums[threadIdx.x] = column_sum;
             __syncthreads();
-            if (group == 0 && c_ok) {
+            if (threadIdx.x < COLS && c_ok) {
                 float s = 0.f;
 #pragma unroll
-                for (int g = 0; g < GROUPS; ++g) s += sums[g * COLS + col];
+                for (int g = 0; g < 64 * W / COLS; ++g) s += sums[g * COLS + col];
                 if (!whole)
                     a.part[(int64_t)gridDim.z * out_rows * a.k + (int64_t)blockIdx.z * a.k + c] = s;
                 else if (a.bias_out)
@@ -460,8 +451,8 @@ __global__ __launch_bounds__(256, 2) void k_product(ProductArgs a) {
     }
     if (found && to) {       // the terms left out above, to the results whose rows have the bit
         __syncthreads();
-        for (int e = threadIdx.x; e < 128 * MT * COLS; e += 256) {
-            const int64_t r = (int64_t)blockIdx.x * 128 * MT + e / COLS;
+        for (int e = threadIdx.x; e < 32 * W * MT * COLS; e += 64 * W) {
+            const int64_t r = (int64_t)blockIdx.x * 32 * W * MT + e / COLS;
             const int cc = c0 + e % COLS;
             if (r >= out_rows || cc >= a.k) continue;
             const int64_t end = min(limit, term(last, 0));
@@ -515,15 +506,13 @@ __global__ __launch_bounds__(256) void k_join(ProductArgs a, int parts, int64_t 
     const float *part = bias ? a.part + parts * all + (at - all) : a.part + at;
     const int64_t step = bias ? a.k : all;
     float s = 0.f;
-    int p = 0;
-    for (; p + 8 <= parts; p += 8) {
+    for (int p = 0; p < parts; p += 8) {
         float v[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) v[u] = part[(p + u) * step];
+        for (int u = 0; u < 8; ++u) v[u] = p + u < parts ? part[(p + u) * step] : 0.f;
 #pragma unroll
         for (int u = 0; u < 8; ++u) s += v[u];
     }
-    for (; p < parts; ++p) s += part[p * step];
     if (bias) {
         if (a.bias_out) a.bias_out[at - all] = s;
         return;
@@ -1024,31 +1013,61 @@ struct Plan {
     int64_t row_blocks, col_blocks, out_rows, turned_words, turned_bytes, work_bytes;
 };
 
-Plan product_plan(bool grad, int64_t m, int32_t n_features, int32_t k) {
+// In how many parts the sum is cut, so that few result tiles still fill the card: the one whose time is the least by what was measured
+// on the card, in ns -- `step` for each step of a workgroup that has its CU to itself, half as much again where two share
+// one (`shared`: they fit), and for more than one part 3,000 and the parts' sums once out and once in at 4 TB/s.
+int best_parts(int64_t blocks, int steps, int step, bool shared, int64_t values) {
+    int best = 1;
+    double least = 0;
+    for (int parts = 1; parts <= steps && parts <= 256; ++parts) {
+        const int64_t per = ceil_div(steps, parts), all = blocks * ceil_div(steps, per);
+        const double load = !shared ? (double)ceil_div(all, 256) : all <= 256 ? 1.0 : 1.5 * ceil_div(all, 512);
+        const double time = per * step * load + (parts > 1 ? 3000.0 + 8.0 * parts * values / 4000.0 : 0.0);
+        if (parts == 1 || time < least) {
+            least = time;
+            best = parts;
+        }
+    }
+    return best;
+}
+
+Plan product_plan(bool grad, int64_t m, int32_t n_features, int32_t k, int type) {
     Plan p = {};
     p.out_rows = grad ? n_features : m;
     if (m == 0) return p;
-    p.lookup = !grad && m <= 64;
+    // Few lookups are done one by one: 4.3 us for a row of 7,500 features and 8 columns, where the product and its join take 8;
+    // 512 rows 7.5 against 8.9, 32 columns 10.0 against 9.4; 16 rows of 1,000 columns 16 against 19, 32 rows 23 against 19.
+    // A row is one workgroup's: 100,000 features keep it 25 us, the product 16.
+    p.lookup = !grad && m * ceil_div(k, 64) <= 512 && n_features <= 32768 && m * k * n_features <= 120000000;
     if (p.lookup) return p;
     p.nt = k <= 32 ? 1 : 2;
     p.col_blocks = ceil_div(k, 32 * p.nt);
-    p.src = !grad ? ROWS : p.col_blocks > 2 && m > 256 ? TURNED : TURN;
+    // Turning the bits beforehand pays when many column blocks would each turn them (7,500 features; 4,096 rows: 200 columns 53
+    // against 56 us, 1,000 columns 146 against 172, in bf16 73 against 102; 1,024 rows, 1,000 columns 47 against 49, 400 columns
+    // 38 against 36; 500 features, 4,096 rows, 1,000 columns 31 against 27)
+    p.src = !grad ? ROWS : k > 128 && n_features >= 2048 && m * k >= 800000 ? TURNED : TURN;
     if (p.src == TURNED) {
         p.turned_words = 8 * ceil_div(m, 256);
         p.turned_bytes = ceil_div(((int64_t)n_features + 1) * p.turned_words * 4, 256) * 256;
     }
-    p.mt = grad || m > 1024 ? 4 : 1;
-    p.row_blocks = ceil_div(p.out_rows, 128 * p.mt);
+    p.mt = p.src == TURNED || (p.src == ROWS && p.nt == 2 && m > 512) ? 2 : 1;
+    p.row_blocks = ceil_div(p.out_rows, 32 * W * p.mt);
     p.steps = (int)(p.src == ROWS ? ceil_div(n_features, 256) : p.src == TURN ? ceil_div(m, 64) : ceil_div(m, 256));
-    const int64_t blocks = p.row_blocks * p.col_blocks, wanted = blocks < 512 ? 512 / blocks : 1, most = p.src == TURN ? ceil_div(p.steps, 2) : p.steps;
-    int64_t parts = wanted < most ? wanted : most;
-#ifdef STAG_TUNE
-    if (const char *e = getenv("STAG_TUNE")) { int mt, pp; sscanf(e, "%d,%d", &mt, &pp); if (p.src != TURNED) { p.mt = mt; p.row_blocks = ceil_div(p.out_rows, 128 * p.mt);} parts = pp < p.steps ? pp : p.steps; }
-#endif
+    const int step = type == STAG_F32 ? (p.src == TURN ? (p.nt == 2 ? 1100 : 800) : p.nt == 1 ? 2200 : p.mt == 1 ? 4500 : 8500)
+                                      : (p.src == TURN ? (p.nt == 2 ? 700 : 500) : p.nt == 1 ? 1300 : p.mt == 1 ? 2200 : 3800);
+    const int64_t parts = best_parts(p.row_blocks * p.col_blocks, p.steps, step, p.src == TURN || p.nt == 1, p.out_rows * k);
     p.per_part = (int)ceil_div(p.steps, parts);
     p.parts = (int)ceil_div(p.steps, p.per_part);
     p.work_bytes = p.turned_bytes + (p.parts > 1 ? ((int64_t)p.parts * (p.out_rows + (grad ? 1 : 0)) * k) * 4 : 0);
     return p;
+}
+
+// launches k_product<TYPE, SRC, MT, NT> if that is what the plan says
+template <int TYPE, Source SRC, int MT, int NT>
+bool launched(const Plan &p, const ProductArgs &a, hipStream_t st) {
+    if (p.src != SRC || p.mt != MT || p.nt != NT) return false;
+    k_product<TYPE, SRC, MT, NT><<<dim3((unsigned)p.row_blocks, (unsigned)p.col_blocks, (unsigned)p.parts), 64 * W, 0, st>>>(a);
+    return true;
 }
 
 template <int TYPE, bool GRAD>
@@ -1060,33 +1079,19 @@ int product(const Plan &p, ProductArgs a, void *work, hipStream_t st) {
     REQUIRE(p.row_blocks < (int64_t)1 << 31 && ceil_div((p.out_rows + 1) * a.k, 256) < (int64_t)1 << 31, "%lld rows of %d columns are too many",
             (long long)p.out_rows, a.k);
     if (p.parts) {
-        const dim3 grid((unsigned)p.row_blocks, (unsigned)p.col_blocks, (unsigned)p.parts);
+        bool done;
         if constexpr (GRAD) {
             if (p.src == TURNED) {
                 const int row_words = a.words;
                 a.turned = (const uint32_t *)work;
                 a.words = (int32_t)p.turned_words;
                 k_turn<<<dim3((unsigned)ceil_div(a.m, 256), (unsigned)ceil_div(row_words, 16)), 256, 0, st>>>(a, (uint32_t *)work, row_words);
-                k_product<TYPE, TURNED, 4, 2, 1><<<grid, 256, 0, st>>>(a);
-            } else if (p.nt == 2 && p.mt == 4) {
-                k_product<TYPE, TURN, 4, 2, 1><<<grid, 256, 0, st>>>(a);
-            } else if (p.nt == 2) {
-                k_product<TYPE, TURN, 1, 2, 2><<<grid, 256, 0, st>>>(a);
-            } else if (p.mt == 4) {
-                k_product<TYPE, TURN, 4, 1, 2><<<grid, 256, 0, st>>>(a);
-            } else {
-                k_product<TYPE, TURN, 1, 1, 4><<<grid, 256, 0, st>>>(a);
             }
+            done = launched<TYPE, TURNED, 2, 2>(p, a, st) || launched<TYPE, TURN, 1, 2>(p, a, st) || launched<TYPE, TURN, 1, 1>(p, a, st);
         } else {
-            if (p.mt == 4 && p.nt == 2)
-                k_product<TYPE, ROWS, 4, 2, 1><<<grid, 256, 0, st>>>(a);
-            else if (p.mt == 4)
-                k_product<TYPE, ROWS, 4, 1, 2><<<grid, 256, 0, st>>>(a);
-            else if (p.nt == 2)
-                k_product<TYPE, ROWS, 1, 2, 2><<<grid, 256, 0, st>>>(a);
-            else
-                k_product<TYPE, ROWS, 1, 1, 4><<<grid, 256, 0, st>>>(a);
+            done = launched<TYPE, ROWS, 2, 2>(p, a, st) || launched<TYPE, ROWS, 1, 2>(p, a, st) || launched<TYPE, ROWS, 1, 1>(p, a, st);
         }
+        REQUIRE(done, "no kernel for %d x %d tiles", p.mt, p.nt);
         HIP_TRY(hipGetLastError());
     }
     if (p.parts != 1) {      // an empty sum has no parts
@@ -1157,12 +1162,12 @@ const char *stag_train_last_error(void) { return g_err; }
 
 int64_t stag_row_scores_workspace(int64_t m, int32_t n_features, int32_t k, int32_t type) {
     TRY(check_rows(nullptr, 0, (((int64_t)n_features + 127) / 128) * 4, n_features, (const int32_t *)16, m, k, type));
-    return product_plan(false, m, n_features, k).work_bytes;
+    return product_plan(false, m, n_features, k, type).work_bytes;
 }
 
 int64_t stag_row_scores_grad_workspace(int64_t m, int32_t n_features, int32_t k, int32_t type) {
     TRY(check_rows(nullptr, 0, (((int64_t)n_features + 127) / 128) * 4, n_features, (const int32_t *)16, m, k, type));
-    return product_plan(true, m, n_features, k).work_bytes;
+    return product_plan(true, m, n_features, k, type).work_bytes;
 }
 
 int stag_row_scores_dev(const uint32_t *d_bits, int64_t n, int64_t row_stride, int32_t n_features, const int32_t *d_rows, int64_t m, const void *d_table,
@@ -1173,7 +1178,7 @@ int stag_row_scores_dev(const uint32_t *d_bits, int64_t n, int64_t row_stride, i
     if (m == 0) return STAG_OK;
     TRY(check_matrix("d_scores", d_scores, STAG_F32, score_stride, k));
     REQUIRE(aligned(d_bias, 4), "d_bias is not aligned to its type");
-    const Plan p = product_plan(false, m, n_features, k);
+    const Plan p = product_plan(false, m, n_features, k, type);
     REQUIRE(work_bytes >= p.work_bytes && (p.work_bytes == 0 || (d_work && aligned(d_work, 256))), "d_work: %lld bytes, 256-byte aligned, are wanted",
             (long long)p.work_bytes);
     ProductArgs a = {};
@@ -1198,7 +1203,7 @@ int stag_row_scores_grad_dev(const uint32_t *d_bits, int64_t n, int64_t row_stri
     if (d_table_grad) TRY(check_matrix("d_table_grad", d_table_grad, STAG_F32, table_grad_stride, k));
     REQUIRE(aligned(d_bias_grad, 4), "d_bias_grad is not aligned to its type");
     if (!d_table_grad && !d_bias_grad) return STAG_OK;
-    const Plan p = product_plan(true, m, n_features, k);
+    const Plan p = product_plan(true, m, n_features, k, type);
     REQUIRE(work_bytes >= p.work_bytes && (p.work_bytes == 0 || (d_work && aligned(d_work, 256))), "d_work: %lld bytes, 256-byte aligned, are wanted",
             (long long)p.work_bytes);
     ProductArgs a = {};

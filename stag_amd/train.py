@@ -285,37 +285,48 @@ class AdamW:
         decay = [float(x) for x in (weight_decay if isinstance(weight_decay, (list, tuple)) else [weight_decay] * len(params))]
         l1 = [float(x) for x in (l1 if isinstance(l1, (list, tuple)) else [l1] * len(params))]
         _need(len(decay) == len(params) and len(l1) == len(params), "weight_decay and l1 are one number, or one for each of the %d tensors", len(params))
-        for x in decay + l1:
+        for x in set(decay + l1):
             _need(math.isfinite(x) and x >= 0, "weight_decay and l1 are not negative: got %r", x)
         self.lr, self.betas, self.eps, self.state_bits = lr, tuple(betas), eps, state_bits
         b1, b2 = self.betas
         _need(math.isfinite(lr) and lr >= 0, "lr = %r", lr)
         _need(0 < b1 < 1 and 0 < b2 < 1, "betas = %r: not inside (0, 1)", betas)
         _need(math.isfinite(eps) and eps >= 0, "eps = %r", eps)
-        spans = []
-        for j, (p, g) in enumerate(zip(params, grads)):
-            for name, t in (("params[%d]" % j, p), ("grads[%d]" % j, g)):
-                if not isinstance(t, torch.Tensor) or t.dtype not in _TYPES:
-                    raise TypeError("%s must be a float32, bfloat16 or float16 tensor" % name)
-                _need(t.is_contiguous(), "%s is not contiguous", name)
-            _need(p.shape == g.shape, "params[%d] has shape %s, its gradient %s", j, tuple(p.shape), tuple(g.shape))
-        device = _one_gpu(**{"params[%d]" % j: p for j, p in enumerate(params)}, **{"grads[%d]" % j: g for j, g in enumerate(grads)})
-        for written, kind, tensors in ((True, "params", params), (False, "grads", grads)):
-            spans += [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), written, "%s[%d]" % (kind, j)) for j, t in enumerate(tensors) if t.numel()]
-        last, last_written = (0, 0, False, ""), (0, 0, True, "")
-        for span in sorted(spans):         # gradients may share memory with each other, what is written with nothing
-            before = last if span[2] else last_written
-            _need(before[1] <= span[0], "%s and %s share memory", before[3], span[3])
-            last = max(last, span, key=lambda x: x[1])
-            last_written = max(last_written, span, key=lambda x: x[1]) if span[2] else last_written
+        both = params + grads
+        n = len(params)
+        name = lambda j: "params[%d]" % j if j < n else "grads[%d]" % (j - n)      # noqa: E731
+        if not all(isinstance(x, _Tensor) for x in both) or not {x.dtype for x in both} <= set(_TYPES):
+            j = next(j for j, x in enumerate(both) if not isinstance(x, _Tensor) or x.dtype not in _TYPES)
+            raise TypeError("%s must be a float32, bfloat16 or float16 tensor" % name(j))
+        for j, x in enumerate(both):
+            if not x.is_contiguous():
+                raise ValueError("%s is not contiguous" % name(j))
+        for j, (x, g) in enumerate(zip(params, grads)):
+            if x.shape != g.shape:
+                raise ValueError("params[%d] has shape %s, its gradient %s" % (j, tuple(x.shape), tuple(g.shape)))
+        gpus = [x.get_device() for x in both]
+        if len(set(gpus)) > 1 or gpus[0] < 0:
+            _one_gpu(**{name(j): x for j, x in enumerate(both)})
+        device = params[0].device
+        counts = np.array([x.numel() for x in params], dtype=np.int64)
+        at = np.array([x.data_ptr() for x in both], dtype=np.uint64)
+        end = at + np.array([x.nbytes for x in both], dtype=np.uint64)
+        order = np.flatnonzero(end > at)
+        order = order[np.lexsort((order, at[order]))]
+        # gradients may share memory with each other, what is written with nothing
+        for mine, others in ((order < n, np.ones(len(order), bool)), (order >= n, order < n)):
+            reach = np.maximum.accumulate(np.where(others, end[order], 0))[:-1]          # how far those before go
+            bad = np.flatnonzero(mine[1:] & (reach > at[order][1:]))
+            if len(bad):
+                k = int(bad[0]) + 1
+                before = max((int(end[q]), int(q)) for q, o in zip(order[:k], others[:k]) if o)[1]
+                raise ValueError("%s and %s share memory" % (name(before), name(int(order[k]))))
         self.device, self.params, self.grads = device, params, grads
-        table = np.zeros(len(params), dtype=_TENSOR)
-        counts = np.array([p.numel() for p in params], dtype=np.int64)
+        table = np.zeros(n, dtype=_TENSOR)
         padded = -(-counts // BLOCK) * BLOCK
-        self.state_at = [int(x) for x in np.concatenate([[0], np.cumsum(padded)[:-1]])]
+        self.state_at = np.concatenate([[0], np.cumsum(padded)[:-1]]).tolist()
         self.state_values = int(padded.sum())
-        table["param"] = [p.data_ptr() for p in params]
-        table["grad"] = [g.data_ptr() for g in grads]
+        table["param"], table["grad"] = at[:n], at[n:]
         table["count"], table["state_at"] = counts, self.state_at
         table["weight_decay"], table["l1"] = decay, l1
         table["param_type"] = [_TYPES[p.dtype] for p in params]
