@@ -613,10 +613,18 @@ __device__ __forceinline__ float log_one_plus(float e) {
     return e < 0x1p-26f ? e : 2.f * fmaf(p * q, z, z);
 }
 
+// one score's loss and slope, times w
+__device__ __forceinline__ void loss_of(float z, bool positive, float w, float &term, float &slope) {
+    const float s = positive ? -z : z;
+    const float e = exp_minus_abs(s), d = 1.f + e, r = __builtin_amdgcn_rcpf(d);
+    term = w * ((s < 0.f ? 0.f : s) + log_one_plus(e));                              // softplus(s); NaN stays NaN
+    const float p = (s >= 0.f ? 1.f : e) * fmaf(fmaf(-d, r, 1.f), r, r) * w;         // sigmoid(s)
+    slope = positive ? -p : p;
+}
+
 // A thread owns V neighbouring columns and goes down the rows of its workgroup, four at a time so that their loads are in
 // flight together; loss sums stay in its registers until the workgroup adds them up in a fixed order and stores one
-// partial row of K sums.  Scores are read only where the row trains (a place of the tree has a handful of siblings among
-// the thousands of a level); the rest of the gradient is zeros, so what bounds a level's loss is writing the gradient.
+// partial row of K sums.  Scores are read only where the row trains.
 template <typename T, int V, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_loss(const float *scores, int64_t score_stride, int64_t m, int k, const int32_t *label,
                                               const int32_t *siblings, const float *weight, float scale, float *loss, T *grad,
@@ -667,16 +675,94 @@ __global__ __launch_bounds__(THREADS) void k_loss(const float *scores, int64_t s
                     for (int j = 0; j < V; ++j) {
                         const int c = c0 + j;
                         if (c < lo[u] || c >= hi[u]) continue;
-                        const float s = c == lab[u] ? -z[u][j] : z[u][j];
-                        const float e = exp_minus_abs(s), d = 1.f + e, r = __builtin_amdgcn_rcpf(d);
-                        sum[j] += wu * ((s < 0.f ? 0.f : s) + log_one_plus(e));        // softplus(s); NaN stays NaN
-                        const float p = (s >= 0.f ? 1.f : e) * fmaf(fmaf(-d, r, 1.f), r, r) * wu;   // sigmoid(s)
-                        g[j] = (T)(c == lab[u] ? -p : p);
+                        float term, slope;
+                        loss_of(z[u][j], c == lab[u], wu, term, slope);
+                        sum[j] += term;
+                        g[j] = (T)slope;
                     }
                 }
-                if (grad) *(out_t *)(grad + i * grad_stride + c0) = g;
+                if (grad) __builtin_nontemporal_store(g, (out_t *)(grad + i * grad_stride + c0));
             }
         }
+    }
+    if (!loss) return;
+#pragma unroll
+    for (int j = 0; j < V; ++j) part[threadIdx.x * V + j] = sum[j];
+    __syncthreads();
+    if (r == 0 && c0 < k) {
+        for (int j = 0; j < V; ++j) {
+            float s = 0.f;
+            for (int q = 0; q < rp; ++q) s += part[(q * ct + cv) * V + j];
+            loss[(int64_t)blockIdx.x * k + c0 + j] = s;
+        }
+    }
+}
+
+// The same where rows train ranges of columns: a place of the tree has a handful of siblings among the thousands of a level,
+// so a row's gradient is zeros but for them, and what bounds the loss is writing those.  A workgroup takes ROWS rows at once: 256 / ROWS
+// threads to a row compute its siblings (if they are no more) into LDS, then the owners of columns put them into the vectors
+// of zeros that they store and into their sums.  Wider ranges are computed by the owners.  65,536 x 1,000 in bf16: 39 us a
+// pass with 8 rows, 45 with 16, 49 with 32; each owner computing its own, one lane in 64 busy: 65.  Narrow tables, where an
+// owner's next row is many rows on, take 32.
+template <typename T, int V, int ROWS>
+__global__ __launch_bounds__(256) void k_loss_siblings(const float *scores, int64_t score_stride, int64_t m, int k, const int32_t *label,
+                                                       const int32_t *siblings, const float *weight, float scale, float *loss, T *grad,
+                                                       int64_t grad_stride, int ct) {
+    constexpr int NARROW = 256 / ROWS;
+    typedef __attribute__((ext_vector_type(V))) T out_t;
+    __shared__ int s_lo[ROWS], s_hi[ROWS], s_label[ROWS];
+    __shared__ float s_weight[ROWS], s_term[ROWS][NARROW], s_slope[ROWS][NARROW];
+    __shared__ float part[256 * V];
+    const int cv = threadIdx.x % ct, r = threadIdx.x / ct, rp = 256 / ct;
+    const int c0 = (blockIdx.y * ct + cv) * V;
+    float sum[V] = {};
+    for (int64_t i0 = (int64_t)blockIdx.x * ROWS; i0 < m; i0 += (int64_t)gridDim.x * ROWS) {
+        {
+            const int q = threadIdx.x / NARROW, j = threadIdx.x % NARROW;
+            const int64_t i = i0 + q;
+            int lo = 0, hi = 0, lab = -1;
+            float w = 0.f;
+            if (i < m) {
+                lo = max(siblings[2 * i], 0);
+                hi = max(min(siblings[2 * i + 1], k), 0);
+                lab = label[i];
+                w = scale * (weight ? weight[i] : 1.f);
+            }
+            if (hi - lo <= NARROW && j < hi - lo) loss_of(scores[i * score_stride + lo + j], lo + j == lab, w, s_term[q][j], s_slope[q][j]);
+            if (j == 0) {
+                s_lo[q] = lo;
+                s_hi[q] = hi;
+                s_label[q] = lab;
+                s_weight[q] = w;
+            }
+        }
+        __syncthreads();
+        if (r < rp && c0 < k) {
+            for (int q = r; q < ROWS; q += rp) {
+                const int64_t i = i0 + q;
+                if (i >= m) break;
+                const int lo = s_lo[q], hi = s_hi[q];
+                out_t g = (out_t)(T)0.f;
+                if (c0 + V > lo && c0 < hi) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        const int c = c0 + j;
+                        if (c < lo || c >= hi) continue;
+                        float term, slope;
+                        if (hi - lo <= NARROW) {
+                            term = s_term[q][c - lo];
+                            slope = s_slope[q][c - lo];
+                        } else {
+                            loss_of(scores[i * score_stride + c], c == s_label[q], s_weight[q], term, slope);
+                        }
+                        sum[j] += term;
+                        g[j] = (T)slope;
+                    }
+                }
+                if (grad) __builtin_nontemporal_store(g, (out_t *)(grad + i * grad_stride + c0));
+            }
+        }
+        __syncthreads();
     }
     if (!loss) return;
 #pragma unroll
@@ -1138,14 +1224,19 @@ int loss_typed(const LossPlan &p, const float *d_scores, int64_t score_stride, i
     float *to = d_loss && p.gx > 1 ? parts : d_loss;
     const dim3 grid(p.gx, p.gy);
     auto launch = [&](auto kernel) { kernel<<<grid, p.threads, 0, st>>>(d_scores, score_stride, m, k, d_label, d_siblings, d_weight, scale, to, (T *)d_grad, grad_stride, p.ct); };
+    constexpr int MOST = sizeof(T) == 4 ? 4 : 8;
     if (p.threads == 1024)
         launch(k_loss<T, 1, 1024>);
+    else if (d_siblings && p.ct >= 64)
+        p.v == 1 ? launch(k_loss_siblings<T, 1, 8>) : p.v == 4 ? launch(k_loss_siblings<T, 4, 8>) : launch(k_loss_siblings<T, MOST, 8>);
+    else if (d_siblings)
+        p.v == 1 ? launch(k_loss_siblings<T, 1, 32>) : p.v == 4 ? launch(k_loss_siblings<T, 4, 32>) : launch(k_loss_siblings<T, MOST, 32>);
     else if (p.v == 1)
         launch(k_loss<T, 1, 256>);
-    else if (p.v == 4 || sizeof(T) == 4)
+    else if (p.v == 4)
         launch(k_loss<T, 4, 256>);
     else
-        launch(k_loss<T, sizeof(T) == 4 ? 4 : 8, 256>);
+        launch(k_loss<T, MOST, 256>);
     HIP_TRY(hipGetLastError());
     if (d_loss && p.gx > 1) {
         k_loss_join<<<(unsigned)ceil_div(k, 32), 1024, 0, st>>>(parts, (int)p.gx, k, d_loss);
