@@ -527,18 +527,16 @@ __global__ __launch_bounds__(256) void k_join(ProductArgs a, int parts, int64_t 
 // lists the row's tokens in LDS, 256 words at a time, and its 1024 / cw column groups take the tokens in turn.
 constexpr int LOOKUP_WORDS = 256;
 template <typename T>
-__global__ __launch_bounds__(1024) void k_lookup(const uint32_t *bits, int64_t n, int64_t row_stride, int n_features, const int32_t *rows, const T *table,
-                                                 int64_t table_stride, const float *bias, int k, float scale, float *scores, int64_t score_stride,
-                                                 int cw_log) {
+__global__ __launch_bounds__(1024) void k_lookup(ProductArgs a, int cw_log) {
     __shared__ uint16_t token[LOOKUP_WORDS * 32];
     __shared__ int before[5];
     __shared__ float part[1024];
     const int64_t i = blockIdx.x;
     const int cw = 1 << cw_log, c = blockIdx.y * cw + (threadIdx.x & (cw - 1)), slot = threadIdx.x >> cw_log, slots = 1024 >> cw_log;
-    const uint32_t *row = row_of(bits, n, row_stride, rows, i);
+    const uint32_t *row = row_of(a.bits, a.n, a.row_stride, a.rows, i);
     float s = 0.f;
     if (row) {
-        const int words = (n_features + 31) / 32;
+        const int words = (a.n_features + 31) / 32;
         for (int w0 = 0; w0 < words; w0 += LOOKUP_WORDS) {
             __syncthreads();
             uint32_t x = 0;
@@ -546,7 +544,7 @@ __global__ __launch_bounds__(1024) void k_lookup(const uint32_t *bits, int64_t n
             if (threadIdx.x < LOOKUP_WORDS) {
                 const int w = w0 + threadIdx.x;
                 if (w < words) x = row[w];
-                if (32 * (w + 1) > n_features) x &= w < words ? 0xffffffffu >> (32 * words - n_features) : 0u;
+                if (32 * (w + 1) > a.n_features) x &= w < words ? 0xffffffffu >> (32 * words - a.n_features) : 0u;
                 count = __builtin_popcount(x);
                 inside = count;
 #pragma unroll
@@ -564,16 +562,16 @@ __global__ __launch_bounds__(1024) void k_lookup(const uint32_t *bits, int64_t n
                 for (; x; x &= x - 1) token[at++] = (uint16_t)(threadIdx.x * 32 + __builtin_ctz(x));
             }
             __syncthreads();
-            if (c < k) {
-                const T *from = table + (int64_t)w0 * 32 * table_stride + c;
+            if (c < a.k) {
+                const T *from = (const T *)a.mat + (int64_t)w0 * 32 * a.mat_stride + c;
                 int t = slot;
                 for (; t + 3 * slots < total; t += 4 * slots) {
                     float v[4];
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) v[u] = (float)from[(int64_t)token[t + u * slots] * table_stride];
+                    for (int u = 0; u < 4; ++u) v[u] = (float)from[(int64_t)token[t + u * slots] * a.mat_stride];
                     s += (v[0] + v[1]) + (v[2] + v[3]);
                 }
-                for (; t < total; t += slots) s += (float)from[(int64_t)token[t] * table_stride];
+                for (; t < total; t += slots) s += (float)from[(int64_t)token[t] * a.mat_stride];
             }
         }
     }
@@ -582,7 +580,7 @@ __global__ __launch_bounds__(1024) void k_lookup(const uint32_t *bits, int64_t n
         __syncthreads();
         if (slot < half) part[threadIdx.x] += part[threadIdx.x + (half << cw_log)];
     }
-    if (slot == 0 && c < k) scores[i * score_stride + c] = row ? part[threadIdx.x] * scale + (bias ? bias[c] : 0.f) : 0.f;
+    if (slot == 0 && c < a.k) a.out[i * a.out_stride + c] = row ? part[threadIdx.x] * a.scale + (a.bias ? a.bias[c] : 0.f) : 0.f;
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -613,6 +611,16 @@ __device__ __forceinline__ float log_one_plus(float e) {
     return e < 0x1p-26f ? e : 2.f * fmaf(p * q, z, z);
 }
 
+struct LossArgs {
+    const float *scores, *weight;
+    const int32_t *label, *siblings;
+    float *loss;                // one partial row of sums a workgroup row
+    void *grad;
+    int64_t score_stride, grad_stride, m;
+    int32_t k, ct;              // ct: column vectors of a workgroup
+    float scale;
+};
+
 // one score's loss and slope, times w
 __device__ __forceinline__ void loss_of(float z, bool positive, float w, float &term, float &slope) {
     const float s = positive ? -z : z;
@@ -626,9 +634,14 @@ __device__ __forceinline__ void loss_of(float z, bool positive, float w, float &
 // flight together; loss sums stay in its registers until the workgroup adds them up in a fixed order and stores one
 // partial row of K sums.  Scores are read only where the row trains.
 template <typename T, int V, int THREADS>
-__global__ __launch_bounds__(THREADS) void k_loss(const float *scores, int64_t score_stride, int64_t m, int k, const int32_t *label,
-                                              const int32_t *siblings, const float *weight, float scale, float *loss, T *grad,
-                                              int64_t grad_stride, int ct) {
+__global__ __launch_bounds__(THREADS) void k_loss(LossArgs a) {
+    const float *const scores = a.scores, *const weight = a.weight;
+    const int32_t *const label = a.label, *const siblings = a.siblings;
+    float *const loss = a.loss;
+    T *const grad = (T *)a.grad;
+    const int64_t score_stride = a.score_stride, grad_stride = a.grad_stride, m = a.m;
+    const int k = a.k, ct = a.ct;
+    const float scale = a.scale;
     constexpr int ROWS_AT_ONCE = 4;
     typedef __attribute__((ext_vector_type(V))) T out_t;
     __shared__ float part[THREADS * V];
@@ -705,9 +718,14 @@ __global__ __launch_bounds__(THREADS) void k_loss(const float *scores, int64_t s
 // pass with 8 rows, 45 with 16, 49 with 32; each owner computing its own, one lane in 64 busy: 65.  Narrow tables, where an
 // owner's next row is many rows on, take 32.
 template <typename T, int V, int ROWS>
-__global__ __launch_bounds__(256) void k_loss_siblings(const float *scores, int64_t score_stride, int64_t m, int k, const int32_t *label,
-                                                       const int32_t *siblings, const float *weight, float scale, float *loss, T *grad,
-                                                       int64_t grad_stride, int ct) {
+__global__ __launch_bounds__(256) void k_loss_siblings(LossArgs a) {
+    const float *const scores = a.scores, *const weight = a.weight;
+    const int32_t *const label = a.label, *const siblings = a.siblings;
+    float *const loss = a.loss;
+    T *const grad = (T *)a.grad;
+    const int64_t score_stride = a.score_stride, grad_stride = a.grad_stride, m = a.m;
+    const int k = a.k, ct = a.ct;
+    const float scale = a.scale;
     constexpr int NARROW = 256 / ROWS;
     typedef __attribute__((ext_vector_type(V))) T out_t;
     __shared__ int s_lo[ROWS], s_hi[ROWS], s_label[ROWS];
@@ -1191,8 +1209,7 @@ template <typename T>
 int lookup(const ProductArgs &a, hipStream_t st) {
     int cw_log = 0;
     while (cw_log < 6 && (1 << cw_log) < a.k) ++cw_log;
-    k_lookup<T><<<dim3((unsigned)a.m, (unsigned)ceil_div(a.k, 1 << cw_log)), 1024, 0, st>>>(a.bits, a.n, a.row_stride, a.n_features, a.rows, (const T *)a.mat,
-                                                                                          a.mat_stride, a.bias, a.k, a.scale, a.out, a.out_stride, cw_log);
+    k_lookup<T><<<dim3((unsigned)a.m, (unsigned)ceil_div(a.k, 1 << cw_log)), 1024, 0, st>>>(a, cw_log);
     HIP_TRY(hipGetLastError());
     return STAG_OK;
 }
@@ -1219,11 +1236,12 @@ LossPlan loss_plan(int64_t m, int32_t k, int v) {
 }
 
 template <typename T>
-int loss_typed(const LossPlan &p, const float *d_scores, int64_t score_stride, int64_t m, int32_t k, const int32_t *d_label, const int32_t *d_siblings,
-               const float *d_weight, float scale, float *d_loss, void *d_grad, int64_t grad_stride, float *parts, hipStream_t st) {
-    float *to = d_loss && p.gx > 1 ? parts : d_loss;
-    const dim3 grid(p.gx, p.gy);
-    auto launch = [&](auto kernel) { kernel<<<grid, p.threads, 0, st>>>(d_scores, score_stride, m, k, d_label, d_siblings, d_weight, scale, to, (T *)d_grad, grad_stride, p.ct); };
+int loss_typed(const LossPlan &p, LossArgs a, float *parts, hipStream_t st) {
+    float *const d_loss = a.loss;
+    const bool d_siblings = a.siblings != nullptr, join = d_loss && p.gx > 1;
+    if (join) a.loss = parts;
+    a.ct = p.ct;
+    auto launch = [&](auto kernel) { kernel<<<dim3(p.gx, p.gy), p.threads, 0, st>>>(a); };
     constexpr int MOST = sizeof(T) == 4 ? 4 : 8;
     if (p.threads == 1024)
         launch(k_loss<T, 1, 1024>);
@@ -1238,8 +1256,8 @@ int loss_typed(const LossPlan &p, const float *d_scores, int64_t score_stride, i
     else
         launch(k_loss<T, MOST, 256>);
     HIP_TRY(hipGetLastError());
-    if (d_loss && p.gx > 1) {
-        k_loss_join<<<(unsigned)ceil_div(k, 32), 1024, 0, st>>>(parts, (int)p.gx, k, d_loss);
+    if (join) {
+        k_loss_join<<<(unsigned)ceil_div(a.k, 32), 1024, 0, st>>>(parts, (int)p.gx, a.k, d_loss);
         HIP_TRY(hipGetLastError());
     }
     return STAG_OK;
@@ -1341,15 +1359,17 @@ int stag_sibling_loss_dev(const float *d_scores, int64_t score_stride, int64_t m
         return k % v == 0 && score_stride % v == 0 && aligned(d_scores, 16) && (!d_grad || (grad_stride % v == 0 && aligned(d_grad, v * type_bytes(type))));
     };
     const LossPlan p = loss_plan(m, k, type != STAG_F32 && fits(8) ? 8 : fits(4) ? 4 : 1);
+    LossArgs a = {};
+    a.scores = d_scores, a.weight = d_weight, a.label = d_label, a.siblings = d_siblings, a.loss = d_loss, a.grad = d_grad;
+    a.score_stride = score_stride, a.grad_stride = grad_stride, a.m = m, a.k = k, a.scale = scale;
     hipStream_t st = (hipStream_t)stream;
-    float *parts = (float *)d_work;
     switch (type) {
     case STAG_F32:
-        return loss_typed<float>(p, d_scores, score_stride, m, k, d_label, d_siblings, d_weight, scale, d_loss, d_grad, grad_stride, parts, st);
+        return loss_typed<float>(p, a, (float *)d_work, st);
     case STAG_BF16:
-        return loss_typed<bf16>(p, d_scores, score_stride, m, k, d_label, d_siblings, d_weight, scale, d_loss, d_grad, grad_stride, parts, st);
+        return loss_typed<bf16>(p, a, (float *)d_work, st);
     default:
-        return loss_typed<f16>(p, d_scores, score_stride, m, k, d_label, d_siblings, d_weight, scale, d_loss, d_grad, grad_stride, parts, st);
+        return loss_typed<f16>(p, a, (float *)d_work, st);
     }
 }
 

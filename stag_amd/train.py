@@ -32,7 +32,10 @@ _TENSOR = np.dtype([("param", "<u8"), ("grad", "<u8"), ("count", "<i8"), ("state
 
 
 _Tensor = torch.Tensor
+_F32, _I32 = torch.float32, torch.int32
 _BITS = (torch.int32, torch.uint32)
+_PAIRS = {(b, x): kind for b in _BITS for x, kind in _TYPES.items()}
+_empty = torch.empty_strided
 _raw_stream = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream(i).cuda_stream without the objects
 _current = torch._C._cuda_getDevice
 
@@ -53,7 +56,7 @@ def _is(name, t, dtypes, dim):
 
 def _plain(t, dtype, shape, gpu):
     """Whether t is a contiguous tensor of this type and shape on this GPU: nothing to check or copy."""
-    return type(t) is _Tensor and t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == gpu
+    return type(t) is _Tensor and t.dtype is dtype and t.get_device() == gpu and t.is_contiguous() and t.shape == shape
 
 
 def _one_gpu(**tensors):
@@ -134,27 +137,32 @@ def row_scores(bits, table, bias=None, *, scale=1.0, rows=None, out=None):
 
     bits: int32 / uint32 [n, words]; table: float32, bfloat16 or float16 [n_features, k]; bias: float32 [k]; rows: int32 [m], any
     order, repeats allowed, an index outside 0..n-1 is padding and scores 0 (default: all rows of bits)."""
-    gpu = bits.get_device() if type(bits) is _Tensor else -1
-    if (gpu >= 0 and type(table) is _Tensor and bits.dim() == table.dim() == 2 and bits.dtype in _BITS and table.dtype in _TYPES and table.numel() and out is None
-            and bits.is_contiguous() and table.is_contiguous() and table.get_device() == gpu and not bits.shape[1] % 4 and bits.shape[1] * 32 >= table.shape[0]
-            and (bias is None or _plain(bias, torch.float32, table.shape[1:], gpu))
-            and (rows is None or (rows.dim() == 1 and _plain(rows, torch.int32, rows.shape, gpu)))):
-        row_stride, table_stride, score_stride = bits.shape[1], table.shape[1], table.shape[1]
-    else:
+    kind = -1
+    if type(bits) is _Tensor and type(table) is _Tensor and out is None and bits.is_contiguous() and table.is_contiguous():
+        (*n, row_stride), (*n_features, k), gpu = bits.shape, table.shape, bits.get_device()
+        if (len(n) == len(n_features) == 1 and gpu >= 0 and table.get_device() == gpu and row_stride & 3 == 0 and k
+                and 0 < n_features[0] <= row_stride * 32 and (bias is None or _plain(bias, _F32, (k,), gpu))
+                and (rows is None or (type(rows) is _Tensor and rows.dim() == 1 and _plain(rows, _I32, rows.shape, gpu)))):
+            kind = _PAIRS.get((bits.dtype, table.dtype), -1)
+            table_stride = score_stride = k
+    if kind < 0:
         bits, table, bias, rows, row_stride, table_stride, score_stride = _check_scores(bits, table, bias, rows, out)
-        gpu = bits.get_device()
+        gpu, kind = bits.get_device(), _TYPES[table.dtype]
     if gpu != _current():
         with torch.cuda.device(gpu):
             return row_scores(bits, table, bias, scale=scale, rows=rows, out=out)
+    n = bits.shape[0]
     n_features, k = table.shape
-    m = bits.shape[0] if rows is None else rows.shape[0]
-    kind = _TYPES[table.dtype]
+    m = n if rows is None else rows.shape[0]
     if out is None:
-        out = torch.empty((m, k), dtype=torch.float32, device=bits.device)
+        out = _empty((m, k), (k, 1), dtype=_F32, device=bits.device)
     need = _workspace("stag_row_scores_workspace", m, n_features, k, kind)
-    work = torch.empty(need, dtype=torch.uint8, device=bits.device) if need else None
-    _lib.check_train(_lib.train_lib().stag_row_scores_dev(bits.data_ptr(), bits.shape[0], row_stride, n_features, _ptr(rows), m, table.data_ptr(), kind, table_stride,
-                                                          _ptr(bias), k, float(scale), out.data_ptr(), score_stride, _ptr(work), need, _raw_stream(gpu)))
+    work = _empty((need,), (1,), dtype=torch.uint8, device=bits.device) if need else None
+    rc = _lib.train_lib().stag_row_scores_dev(bits.data_ptr(), n, row_stride, n_features, None if rows is None else rows.data_ptr(), m, table.data_ptr(), kind,
+                                              table_stride, None if bias is None else bias.data_ptr(), k, float(scale), out.data_ptr(), score_stride,
+                                              work.data_ptr() if need else None, need, _raw_stream(gpu))
+    if rc:
+        _lib.check_train(rc)
     return out
 
 
@@ -185,28 +193,34 @@ def row_scores_grad(bits, grad, n_features, *, scale=1.0, rows=None, out=None):
 
     grad: float32, bfloat16 or float16 [m, k].  Padding rows (see row_scores) take part in neither, whatever grad holds for
     them.  out: a pair of tensors to overwrite."""
-    n_features = int(n_features)
-    gpu = bits.get_device() if type(bits) is _Tensor else -1
-    if (gpu >= 0 and type(grad) is _Tensor and bits.dim() == grad.dim() == 2 and bits.dtype in _BITS and grad.dtype in _TYPES and grad.numel() and n_features >= 1
-            and bits.is_contiguous() and grad.is_contiguous() and grad.get_device() == gpu and not bits.shape[1] % 4 and bits.shape[1] * 32 >= n_features
-            and (bits.shape[:1] == grad.shape[:1] if rows is None else _plain(rows, torch.int32, grad.shape[:1], gpu))
-            and (out is None or (_plain(out[0], torch.float32, (n_features, grad.shape[1]), gpu) and _plain(out[1], torch.float32, grad.shape[1:], gpu)))):
-        row_stride, grad_stride, stride = bits.shape[1], grad.shape[1], grad.shape[1]
-    else:
+    n_features, kind = int(n_features), -1
+    if type(bits) is _Tensor and type(grad) is _Tensor and bits.is_contiguous() and grad.is_contiguous():
+        (*n, row_stride), (*m, k), gpu = bits.shape, grad.shape, bits.get_device()
+        if (len(n) == len(m) == 1 and gpu >= 0 and grad.get_device() == gpu and row_stride & 3 == 0 and k and m[0] and 0 < n_features <= row_stride * 32
+                and (n == m if rows is None else _plain(rows, _I32, (m[0],), gpu))
+                and (out is None or (_plain(out[0], _F32, (n_features, k), gpu) and _plain(out[1], _F32, (k,), gpu)))):
+            kind = _PAIRS.get((bits.dtype, grad.dtype), -1)
+            grad_stride = stride = k
+    if kind < 0:
         bits, grad, rows, row_stride, grad_stride, stride = _check_grad(bits, grad, n_features, rows, out)
-        gpu = bits.get_device()
+        gpu, kind = bits.get_device(), _TYPES[grad.dtype]
     if gpu != _current():
         with torch.cuda.device(gpu):
             return row_scores_grad(bits, grad, n_features, scale=scale, rows=rows, out=out)
     m, k = grad.shape
-    kind = _TYPES[grad.dtype]
     if out is None:
-        out = torch.empty((n_features, k), dtype=torch.float32, device=bits.device), torch.empty(k, dtype=torch.float32, device=bits.device)
+        table_grad = _empty((n_features, k), (k, 1), dtype=_F32, device=bits.device)
+        bias_grad = _empty((k,), (1,), dtype=_F32, device=bits.device)
+    else:
+        table_grad, bias_grad = out
     need = _workspace("stag_row_scores_grad_workspace", m, n_features, k, kind)
-    work = torch.empty(need, dtype=torch.uint8, device=bits.device) if need else None
-    _lib.check_train(_lib.train_lib().stag_row_scores_grad_dev(bits.data_ptr(), bits.shape[0], row_stride, n_features, _ptr(rows), m, grad.data_ptr(), kind, grad_stride, k,
-                                                               float(scale), out[0].data_ptr(), stride, out[1].data_ptr(), _ptr(work), need, _raw_stream(gpu)))
-    return out[0], out[1]
+    work = _empty((need,), (1,), dtype=torch.uint8, device=bits.device) if need else None
+    rc = _lib.train_lib().stag_row_scores_grad_dev(bits.data_ptr(), bits.shape[0], row_stride, n_features, None if rows is None else rows.data_ptr(), m, grad.data_ptr(),
+                                                   kind, grad_stride, k, float(scale), table_grad.data_ptr(), stride, bias_grad.data_ptr(),
+                                                   work.data_ptr() if need else None, need, _raw_stream(gpu))
+    if rc:
+        _lib.check_train(rc)
+    return table_grad, bias_grad
 
 
 def _check_loss(scores, label, siblings, weight, dtype, out):
@@ -245,12 +259,14 @@ def sibling_loss(scores, label, *, siblings=None, weight=None, scale=1.0, grad_d
     grad is d(sum of loss)/d(scores) of type grad_dtype (default float32), 0 where a row does not train, and scores are not
     read there.  weight: float32 [m].  out: a pair of tensors to overwrite."""
     dtype = grad_dtype or (out[1].dtype if out is not None else torch.float32)
-    gpu = scores.get_device() if type(scores) is _Tensor else -1
-    if (gpu >= 0 and scores.dtype is torch.float32 and scores.dim() == 2 and scores.numel() and scores.is_contiguous() and dtype in _TYPES and out is None
-            and _plain(label, torch.int32, scores.shape[:1], gpu) and (siblings is None or _plain(siblings, torch.int32, (scores.shape[0], 2), gpu))
-            and (weight is None or _plain(weight, torch.float32, scores.shape[:1], gpu))):
-        score_stride = grad_stride = scores.shape[1]
-    else:
+    plain = False
+    if type(scores) is _Tensor and out is None and scores.dtype is _F32 and scores.is_contiguous() and dtype in _TYPES:
+        (*m, k), gpu = scores.shape, scores.get_device()
+        if (len(m) == 1 and m[0] and k and gpu >= 0 and _plain(label, _I32, (m[0],), gpu) and (siblings is None or _plain(siblings, _I32, (m[0], 2), gpu))
+                and (weight is None or _plain(weight, _F32, (m[0],), gpu))):
+            plain = True
+            score_stride = grad_stride = k
+    if not plain:
         scores, label, siblings, weight, score_stride, grad_stride = _check_loss(scores, label, siblings, weight, dtype, out)
         gpu = scores.get_device()
     if gpu != _current():
@@ -258,12 +274,18 @@ def sibling_loss(scores, label, *, siblings=None, weight=None, scale=1.0, grad_d
             return sibling_loss(scores, label, siblings=siblings, weight=weight, scale=scale, grad_dtype=dtype, out=out)
     m, k = scores.shape
     if out is None:
-        out = torch.empty(k, dtype=torch.float32, device=scores.device), torch.empty((m, k), dtype=dtype, device=scores.device)
+        loss = _empty((k,), (1,), dtype=_F32, device=scores.device)
+        grad = _empty((m, k), (k, 1), dtype=dtype, device=scores.device)
+    else:
+        loss, grad = out
     need = _workspace("stag_sibling_loss_workspace", m, k)
-    work = torch.empty(need, dtype=torch.uint8, device=scores.device) if need else None
-    _lib.check_train(_lib.train_lib().stag_sibling_loss_dev(scores.data_ptr(), score_stride, m, k, label.data_ptr(), _ptr(siblings), _ptr(weight), float(scale), out[0].data_ptr(),
-                                                            out[1].data_ptr(), _TYPES[dtype], grad_stride, _ptr(work), need, _raw_stream(gpu)))
-    return out[0], out[1]
+    work = _empty((need,), (1,), dtype=torch.uint8, device=scores.device) if need else None
+    rc = _lib.train_lib().stag_sibling_loss_dev(scores.data_ptr(), score_stride, m, k, label.data_ptr(), None if siblings is None else siblings.data_ptr(),
+                                                None if weight is None else weight.data_ptr(), float(scale), loss.data_ptr(), grad.data_ptr(), _TYPES[dtype], grad_stride,
+                                                work.data_ptr() if need else None, need, _raw_stream(gpu))
+    if rc:
+        _lib.check_train(rc)
+    return loss, grad
 
 
 class AdamW:
@@ -359,7 +381,9 @@ class AdamW:
         if gpu != _current():
             with torch.cuda.device(gpu):
                 return self.step()
-        _lib.check_train(_lib.train_lib().stag_adamw_dev(*self._where, self.lr, *self.betas, self.eps, _raw_stream(gpu)))
+        rc = _lib.train_lib().stag_adamw_dev(*self._where, self.lr, *self.betas, self.eps, _raw_stream(gpu))
+        if rc:
+            _lib.check_train(rc)
 
     @property
     def steps(self):
