@@ -34,11 +34,6 @@ int fail(int code, const char *fmt, ...) {
 typedef _Float16 f16;
 typedef __bf16 bf16;
 
-template <int TYPE> struct Of;
-template <> struct Of<STAG_F32> { typedef float type; };
-template <> struct Of<STAG_BF16> { typedef bf16 type; };
-template <> struct Of<STAG_F16> { typedef f16 type; };
-
 int type_bytes(int type) { return type == STAG_F32 ? 4 : 2; }
 bool type_known(int type) { return type == STAG_F32 || type == STAG_BF16 || type == STAG_F16; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -472,10 +467,10 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
 // The batch's bits by feature: turned[f][w], w < words = 8 * ceil(m / 256), with the words in the order in which k_product
 // takes them: word 8 s + 4 h + q holds batch rows 64 (4 s + q) + 32 h + (0..31).  Row n_features says which batch rows are no padding.
 // A wave turns 256 rows by 4 words of features; a lane loads 16 bytes of four rows and stores 16 bytes of four features.
-__global__ __launch_bounds__(256) void k_turn(ProductArgs a, uint32_t *turned, int row_words) {
+__global__ __launch_bounds__(256) void k_turn(ProductArgs a, uint32_t *turned, int row_words, int word_blocks) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    const int64_t s = blockIdx.x;
-    const int w0 = (blockIdx.y * 4 + wave) * 4;
+    const int64_t s = blockIdx.x / word_blocks;
+    const int w0 = (blockIdx.x % word_blocks * 4 + wave) * 4;
     if (w0 >= row_words) return;
     u32x4 x[4], real;
 #pragma unroll
@@ -1117,21 +1112,30 @@ struct Plan {
     int64_t row_blocks, col_blocks, out_rows, turned_words, turned_bytes, work_bytes;
 };
 
-// In how many parts the sum is cut, so that few result tiles still fill the card: the one whose time is the least by what was measured
-// on the card, in ns -- `step` for each step of a workgroup that has its CU to itself, half as much again where two share
-// one (`shared`: they fit), and for more than one part 3,000 and the parts' sums once out and once in at 4 TB/s.
+// In how many parts the sum is cut, so that few result tiles still fill the card: of 1, 2, 3, 4, 6, 8, 12 .. 256 and those that fill it once,
+// the one whose time is the least by what was measured on the card, in ns -- `step` for each step of a workgroup that has its CU to
+// itself, half as much again where two share one (`shared`: they fit), and for more than one part 3,000 and the parts'
+// sums once out and once in at 4 TB/s.
 int best_parts(int64_t blocks, int steps, int step, bool shared, int64_t values) {
     int best = 1;
     double least = 0;
-    for (int parts = 1; parts <= steps && parts <= 256; ++parts) {
-        const int64_t per = ceil_div(steps, parts), all = blocks * ceil_div(steps, per);
-        const double load = !shared ? (double)ceil_div(all, 256) : all <= 256 ? 1.0 : 1.5 * ceil_div(all, 512);
-        const double time = per * step * load + (parts > 1 ? 3000.0 + 8.0 * parts * values / 4000.0 : 0.0);
+    auto look = [&](int parts) {
+        if (parts < 1 || parts > steps || parts > 256) return;
+        const int per = (steps + parts - 1) / parts;
+        const double all = (double)blocks * ((steps + per - 1) / per);
+        const double load = !shared ? std::ceil(all / 256) : all <= 256 ? 1.0 : 1.5 * std::ceil(all / 512);
+        const double time = per * (double)step * load + (parts > 1 ? 3000.0 + 8.0 * parts * (double)values / 4000.0 : 0.0);
         if (parts == 1 || time < least) {
             least = time;
             best = parts;
         }
+    };
+    for (int parts = 1; parts <= 256; parts *= 2) {
+        look(parts);
+        look(parts + parts / 2);
     }
+    look((int)(256 / blocks));
+    look((int)(512 / blocks));
     return best;
 }
 
@@ -1189,7 +1193,9 @@ int product(const Plan &p, ProductArgs a, void *work, hipStream_t st) {
                 const int row_words = a.words;
                 a.turned = (const uint32_t *)work;
                 a.words = (int32_t)p.turned_words;
-                k_turn<<<dim3((unsigned)ceil_div(a.m, 256), (unsigned)ceil_div(row_words, 16)), 256, 0, st>>>(a, (uint32_t *)work, row_words);
+                const int64_t word_blocks = ceil_div(row_words, 16), turns = ceil_div(a.m, 256) * word_blocks;
+                REQUIRE(turns < (int64_t)1 << 31, "%lld rows of %d features are too many", (long long)a.m, a.n_features);
+                k_turn<<<(unsigned)turns, 256, 0, st>>>(a, (uint32_t *)work, row_words, (int)word_blocks);
             }
             done = launched<TYPE, TURNED, 2, 2>(p, a, st) || launched<TYPE, TURN, 1, 2>(p, a, st) || launched<TYPE, TURN, 1, 1>(p, a, st);
         } else {

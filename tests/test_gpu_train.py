@@ -55,7 +55,7 @@ SHAPES = [
     (1, None, 1, 1), (1, None, 145, 2), (2, None, 31, 3), (3, None, 32, 8), (5, 7, 33, 1), (16, None, 127, 31), (17, 1, 128, 32), (20, 40, 129, 33),
     (31, None, 145, 7), (32, None, 640, 64), (33, 65, 643, 65), (64, None, 750, 13), (65, 63, 750, 100), (100, 129, 1000, 257), (300, None, 2100, 5),
     (200, 300, 5250, 4), (1, None, 7500, 8), (4, 4, 7500, 1000), (1000, 1025, 300, 40), (700, 513, 1500, 96), (2000, 3001, 145, 10), (40, None, 20000, 12),
-    (600, 1100, 700, 300),
+    (600, 1100, 700, 300), (2100, 2100, 2600, 400), (5, None, 40000, 9), (400, 513, 33000, 33),
 ]
 
 
@@ -109,11 +109,10 @@ def test_grad(n, m, n_features, k, dtype):
     assert torch.equal(table_grad, again[0]) and torch.equal(bias_grad, again[1])
 
 
-@pytest.mark.parametrize("n, k", [(4, 3), (80, 8), (700, 24), (2500, 200)])
-def test_32_bit_values_keep_their_24_bits(n, k):
+@pytest.mark.parametrize("n, k, n_features", [(4, 3, 900), (80, 8, 900), (700, 24, 900), (2500, 200, 900), (2100, 400, 2500)])
+def test_32_bit_values_keep_their_24_bits(n, k, n_features):
     """One token a row, so that nothing hides the rounding of a value: what comes back is the value."""
     rng = np.random.default_rng(n)
-    n_features = 900
     words = -(-n_features // 128) * 4
     f = rng.permutation(np.arange(n) % n_features)
     bits = np.zeros((n, words), np.uint32)
@@ -131,11 +130,10 @@ def test_32_bit_values_keep_their_24_bits(n, k):
     near(table_grad, want, (2 + n // n_features + 1) * U * size)
 
 
-@pytest.mark.parametrize("n, k", [(1, 4), (40, 5), (600, 70), (1500, 200)])
+@pytest.mark.parametrize("n, k, n_features", [(1, 4, 333), (40, 5, 333), (600, 70, 333), (1500, 200, 333), (2100, 400, 2500), (700, 20, 333)])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
-def test_infinities_reach_only_the_rows_that_have_the_token(n, k, dtype):
+def test_infinities_reach_only_the_rows_that_have_the_token(n, k, n_features, dtype):
     rng = np.random.default_rng(9)
-    n_features = 333
     bits, x = packed(rng, n, n_features)
     table = torch.from_numpy(rng.normal(size=(n_features, k)).astype(np.float32)).to(DEV).to(dtype)
     table[17, 0], table[200, k - 1], table[201, k // 2] = math.inf, math.nan, -math.inf
@@ -145,7 +143,7 @@ def test_infinities_reach_only_the_rows_that_have_the_token(n, k, dtype):
         want = np.stack([t[r > 0].sum(0) for r in x])
     fine = np.isfinite(want)
     assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)])
-    near(got[fine], want[fine], 400 * U * np.abs(t[np.isfinite(t)]).max() * 400)
+    near(got[fine], want[fine], n_features * U * np.abs(t[np.isfinite(t)]).max() * n_features)
     grad = torch.from_numpy(rng.normal(size=(n, k)).astype(np.float32)).to(DEV).to(dtype)
     grad[n // 2, 0], grad[n - 1, k - 1] = math.inf, math.nan
     got = train.row_scores_grad(bits, grad, n_features)
@@ -155,6 +153,73 @@ def test_infinities_reach_only_the_rows_that_have_the_token(n, k, dtype):
         near_bias = g.sum(0)
     assert np.array_equal(np.isnan(got[0].cpu().numpy()), np.isnan(want)) and np.array_equal(np.isinf(got[0].cpu().numpy()), np.isinf(want))
     assert np.array_equal(np.isnan(got[1].cpu().numpy()), np.isnan(near_bias)) and np.array_equal(np.isinf(got[1].cpu().numpy()), np.isinf(near_bias))
+
+
+@pytest.mark.parametrize("dtype, smallest", [(F16, 2.0 ** -24), (BF16, 2.0 ** -133), (F32, 2.0 ** -149)])
+@pytest.mark.parametrize("n, k", [(6, 8), (700, 24)])
+def test_values_below_the_normal_ones(n, k, dtype, smallest):
+    """Subnormal coefficients and gradients count.  16-bit ones exactly; the pieces of a 32-bit one are at least 2^-133 apart."""
+    rng = np.random.default_rng(n)
+    n_features = 300
+    words = -(-n_features // 128) * 4
+    f = np.arange(n) % n_features
+    bits = np.zeros((n, words), np.uint32)
+    bits[np.arange(n), f >> 5] = np.uint32(1) << (f & 31).astype(np.uint32)
+    bits = torch.from_numpy(bits.view(np.int32)).to(DEV)
+    table = torch.from_numpy(rng.integers(-60, 60, (n_features, k)) * smallest).to(dtype).to(DEV)
+    slack = 2.0 ** -133 if dtype == F32 else 0.0
+    near(train.row_scores(bits, table).double().cpu(), table.double().cpu().numpy()[f], slack)
+    grad = torch.from_numpy(rng.integers(-60, 60, (n, k)) * smallest).to(dtype).to(DEV)
+    want = np.zeros((n_features, k))
+    np.add.at(want, f, grad.double().cpu().numpy())
+    near(train.row_scores_grad(bits, grad, n_features)[0].double().cpu(), want, 3 * slack)
+
+
+def test_offsets_beyond_32_bits():
+    """Scores, a table, its gradient and packed rows of more than 2^32 bytes each, looked at where an offset of 32 bits would go astray."""
+    rng = np.random.default_rng(0)
+    n_features, k, m = 100, 1000, 2_200_000                      # 2.2e9 scores
+    base, x = packed(rng, 64, n_features)
+    rows = torch.arange(m, device=DEV, dtype=torch.int32) % 64
+    rows[-1] = -1
+    table = torch.from_numpy(rng.normal(size=(n_features, k)).astype(np.float32)).to(DEV)
+    scores = train.row_scores(base, table, rows=rows)
+    want = x @ table.double().cpu().numpy()
+    for i in (0, 1, 1_073_741, 1_073_742, 2_147_483, 2_147_484, m - 2):
+        near(scores[i].cpu(), want[i % 64], (n_features + 4) * U * (x @ np.abs(table.double().cpu().numpy()))[i % 64])
+    assert (scores[-1] == 0).all()
+    label = (rows % k).to(torch.int32)
+    loss, grad = train.sibling_loss(scores, label, scale=1.0, grad_dtype=F16)
+    z = scores[m - 2].double().cpu().numpy()
+    g = 1 / (1 + np.exp(-z)) - (np.arange(k) == int(label[m - 2]))
+    near(grad[m - 2].double().cpu(), g, 8 * U * np.abs(g) + half_step(g, F16) * (1 + 8 * U))
+    counts = np.bincount(rows[:-1].cpu().numpy(), minlength=64)
+    del scores
+    table_grad, bias_grad = train.row_scores_grad(base, grad, n_features, rows=rows)
+    per = grad[:64].double().cpu().numpy()                       # rows repeat with a period of 64, and so do their labels
+    near(table_grad.double().cpu(), x.T @ (per * counts[:, None]), (m + 4) * U * (x.T @ np.abs(per * counts[:, None])))
+    del grad, table_grad
+    f, k = 70_000, 32_768                                        # 2.3e9 coefficients in 16 bits, gradients in 32
+    bits, x = packed(rng, 3, f)
+    table = torch.randn((f, k), device=DEV, dtype=BF16)
+    near(train.row_scores(bits, table)[:, -40:].cpu(), x @ table[:, -40:].double().cpu().numpy(), (x.sum(1)[:, None] + 4) * U * (x @ np.abs(table[:, -40:].double().cpu().numpy())))
+    grad = torch.from_numpy(rng.normal(size=(3, k)).astype(np.float32)).to(DEV)
+    got = train.row_scores_grad(bits, grad, f)[0]
+    near(got[-50:].cpu(), x.T[-50:] @ grad.double().cpu().numpy(), 7 * U * (x.T[-50:] @ np.abs(grad.double().cpu().numpy())))
+    del table, got
+    n, f = 2_400_000, 16_000                                     # 4.8 GB of packed rows
+    rows = torch.tensor([0, 1_073_741, 2_147_483, 2_147_484, n - 1, n], dtype=torch.int32, device=DEV)
+    bits = torch.zeros((n, 500), dtype=torch.int32, device=DEV)
+    small, x = packed(rng, 5, f, garbage=False)
+    bits[rows[:5].long()] = small
+    table = torch.from_numpy(rng.normal(size=(f, 3)).astype(np.float32)).to(DEV)
+    got = train.row_scores(bits, table, rows=rows)
+    t = table.double().cpu().numpy()
+    near(got[:5].cpu(), x @ t, (x.sum(1)[:, None] + 4) * U * (x @ np.abs(t)))
+    assert (got[5] == 0).all()
+    grad = torch.from_numpy(rng.normal(size=(6, 3)).astype(np.float32)).to(DEV)
+    g = grad[:5].double().cpu().numpy()
+    near(train.row_scores_grad(bits, grad, f, rows=rows)[0].cpu(), x.T @ g, 9 * U * (x.T @ np.abs(g)))
 
 
 @pytest.mark.parametrize("n, k", [(3, 5), (50, 40), (700, 130)])
@@ -246,6 +311,29 @@ def test_loss(m, k, siblings, dtype):
     again = train.sibling_loss(torch.from_numpy(z).to(DEV), torch.from_numpy(label.astype(np.int32)).to(DEV), siblings=sib,
                                weight=torch.from_numpy(w).to(DEV), scale=scale, grad_dtype=dtype)
     assert torch.equal(loss, again[0]) and torch.equal(grad, again[1])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m, k, widest", [(700, 300, 300), (700, 301, 40), (1200, 40, 40), (1200, 41, 9), (5, 9000, 9000), (3000, 2048, 33)])
+def test_loss_of_wide_ranges(m, k, widest, dtype):
+    rng = np.random.default_rng(m + k)
+    z = (rng.normal(size=(m, k)) * 5).astype(np.float32)
+    lo = rng.integers(-3, k, m)
+    hi = lo + rng.integers(0, widest + 1, m)
+    inside = (np.arange(k) >= lo[:, None]) & (np.arange(k) < hi[:, None])
+    z[~inside] = np.nan
+    label = np.clip(lo + rng.integers(-1, widest + 1, m), -2**31, 2**31 - 1)
+    sib = torch.from_numpy(np.stack([lo, hi], 1).astype(np.int32)).to(DEV)
+    loss, grad = train.sibling_loss(torch.from_numpy(z).to(DEV), torch.from_numpy(label.astype(np.int32)).to(DEV), siblings=sib, grad_dtype=dtype)
+    want_loss, want_grad, size = plain_loss(z.astype(np.float64), label, lo, hi, np.ones(m), 1.0)
+    near(loss.cpu(), want_loss, (m + 8) * U * size, "loss")
+    near(grad.float().cpu(), want_grad, 8 * U * np.abs(want_grad) + half_step(want_grad, dtype) * (1 + 8 * U), "grad")
+    extreme = torch.tensor([[-2**31, 2**31 - 1], [2**31 - 1, -2**31], [2**31 - 1, 2**31 - 1], [-2**31, -2**31], [k, k + 5]], dtype=torch.int32, device=DEV)
+    z = torch.from_numpy(rng.normal(size=(2000, k)).astype(np.float32)).to(DEV)
+    whole = train.sibling_loss(z, torch.zeros(2000, dtype=torch.int32, device=DEV))
+    sib = extreme[torch.arange(2000, device=DEV) % 5]
+    part = train.sibling_loss(z, torch.zeros(2000, dtype=torch.int32, device=DEV), siblings=sib)
+    assert torch.equal(part[1][::5], whole[1][::5]) and (part[1].view(400, 5, k)[:, 1:] == 0).all()
 
 
 def test_loss_at_the_ends():
