@@ -34,7 +34,6 @@ _TENSOR = np.dtype([("param", "<u8"), ("grad", "<u8"), ("count", "<i8"), ("state
 _Tensor = torch.Tensor
 _F32, _I32 = torch.float32, torch.int32
 _BITS = (torch.int32, torch.uint32)
-_PAIRS = {(b, x): kind for b in _BITS for x, kind in _TYPES.items()}
 _empty = torch.empty_strided
 _raw_stream = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream(i).cuda_stream without the objects
 _current = torch._C._cuda_getDevice
@@ -139,12 +138,13 @@ def row_scores(bits, table, bias=None, *, scale=1.0, rows=None, out=None):
     order, repeats allowed, an index outside 0..n-1 is padding and scores 0 (default: all rows of bits)."""
     kind = -1
     if type(bits) is _Tensor and type(table) is _Tensor and out is None and bits.is_contiguous() and table.is_contiguous():
-        (*n, row_stride), (*n_features, k), gpu = bits.shape, table.shape, bits.get_device()
-        if (len(n) == len(n_features) == 1 and gpu >= 0 and table.get_device() == gpu and row_stride & 3 == 0 and k
-                and 0 < n_features[0] <= row_stride * 32 and (bias is None or _plain(bias, _F32, (k,), gpu))
-                and (rows is None or (type(rows) is _Tensor and rows.dim() == 1 and _plain(rows, _I32, rows.shape, gpu)))):
-            kind = _PAIRS.get((bits.dtype, table.dtype), -1)
-            table_stride = score_stride = k
+        gpu = bits.get_device()
+        if gpu >= 0 and table.get_device() == gpu and bits.dim() == 2 and table.dim() == 2 and bits.dtype in _BITS:
+            row_stride, (n_features, k) = bits.shape[1], table.shape
+            if (row_stride & 3 == 0 and k and 0 < n_features <= row_stride * 32 and (bias is None or _plain(bias, _F32, (k,), gpu))
+                    and (rows is None or (type(rows) is _Tensor and rows.dim() == 1 and _plain(rows, _I32, rows.shape, gpu)))):
+                kind = 0 if table.dtype is _F32 else _TYPES.get(table.dtype, -1)
+                table_stride = score_stride = k
     if kind < 0:
         bits, table, bias, rows, row_stride, table_stride, score_stride = _check_scores(bits, table, bias, rows, out)
         gpu, kind = bits.get_device(), _TYPES[table.dtype]
@@ -195,12 +195,13 @@ def row_scores_grad(bits, grad, n_features, *, scale=1.0, rows=None, out=None):
     them.  out: a pair of tensors to overwrite."""
     n_features, kind = int(n_features), -1
     if type(bits) is _Tensor and type(grad) is _Tensor and bits.is_contiguous() and grad.is_contiguous():
-        (*n, row_stride), (*m, k), gpu = bits.shape, grad.shape, bits.get_device()
-        if (len(n) == len(m) == 1 and gpu >= 0 and grad.get_device() == gpu and row_stride & 3 == 0 and k and m[0] and 0 < n_features <= row_stride * 32
-                and (n == m if rows is None else _plain(rows, _I32, (m[0],), gpu))
-                and (out is None or (_plain(out[0], _F32, (n_features, k), gpu) and _plain(out[1], _F32, (k,), gpu)))):
-            kind = _PAIRS.get((bits.dtype, grad.dtype), -1)
-            grad_stride = stride = k
+        gpu = bits.get_device()
+        if gpu >= 0 and grad.get_device() == gpu and bits.dim() == 2 and grad.dim() == 2 and bits.dtype in _BITS:
+            (n, row_stride), (m, k) = bits.shape, grad.shape
+            if (row_stride & 3 == 0 and k and m and 0 < n_features <= row_stride * 32 and (n == m if rows is None else _plain(rows, _I32, (m,), gpu))
+                    and (out is None or (_plain(out[0], _F32, (n_features, k), gpu) and _plain(out[1], _F32, (k,), gpu)))):
+                kind = 0 if grad.dtype is _F32 else _TYPES.get(grad.dtype, -1)
+                grad_stride = stride = k
     if kind < 0:
         bits, grad, rows, row_stride, grad_stride, stride = _check_grad(bits, grad, n_features, rows, out)
         gpu, kind = bits.get_device(), _TYPES[grad.dtype]
@@ -261,10 +262,11 @@ def sibling_loss(scores, label, *, siblings=None, weight=None, scale=1.0, grad_d
     dtype = grad_dtype or (out[1].dtype if out is not None else torch.float32)
     plain = False
     if type(scores) is _Tensor and out is None and scores.dtype is _F32 and scores.is_contiguous() and dtype in _TYPES:
-        (*m, k), gpu = scores.shape, scores.get_device()
-        if (len(m) == 1 and m[0] and k and gpu >= 0 and _plain(label, _I32, (m[0],), gpu) and (siblings is None or _plain(siblings, _I32, (m[0], 2), gpu))
-                and (weight is None or _plain(weight, _F32, (m[0],), gpu))):
-            plain = True
+        gpu = scores.get_device()
+        if gpu >= 0 and scores.dim() == 2:
+            m, k = scores.shape
+            plain = (m and k and _plain(label, _I32, (m,), gpu) and (siblings is None or _plain(siblings, _I32, (m, 2), gpu))
+                     and (weight is None or _plain(weight, _F32, (m,), gpu)))
             score_stride = grad_stride = k
     if not plain:
         scores, label, siblings, weight, score_stride, grad_stride = _check_loss(scores, label, siblings, weight, dtype, out)
