@@ -57,8 +57,8 @@ __device__ __forceinline__ const uint32_t *row_of(const uint32_t *bits, int64_t 
 // in 16 bits; a 32-bit coefficient is cut into three bf16 pieces of 8 bits each, which together are the coefficient,
 // and multiplied piece by piece into the same 32-bit sums.  16-bit coefficients go in as they are.
 //
-// An infinity or NaN must not meet a zero bit in a product: such values go in as 0 and, where there were any, are added
-// afterwards to the results whose rows have the bit (slow, and only then).
+// An infinity or NaN that meets a zero bit makes NaN of a sum that it has no part in: sums that come out not finite are added up
+// again, term by term (slow, and only then).
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
@@ -86,9 +86,6 @@ struct ProductArgs {
 template <int TYPE> struct Raw { typedef uint16_t type; };
 template <> struct Raw<STAG_F32> { typedef uint32_t type; };
 
-template <int TYPE> __device__ __forceinline__ bool not_finite(uint32_t raw) {
-    return TYPE == STAG_F32 ? (raw & 0x7f800000u) == 0x7f800000u : TYPE == STAG_BF16 ? (raw & 0x7f80u) == 0x7f80u : (raw & 0x7c00u) == 0x7c00u;
-}
 template <int TYPE> __device__ __forceinline__ float value_of(uint32_t raw) {
     return TYPE == STAG_F32 ? __uint_as_float(raw) : TYPE == STAG_BF16 ? __uint_as_float(raw << 16) : (float)__builtin_bit_cast(f16, (uint16_t)raw);
 }
@@ -98,7 +95,7 @@ constexpr uint32_t NOWHERE = 0x80000000u;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void *p, int64_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, (int)(bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : bytes), 0x00020000);
 }
-template <typename raw_t> __device__ __forceinline__ raw_t load_raw(__amdgpu_buffer_rsrc_t from, uint32_t at) {
+template <typename raw_t> __device__ __forceinline__ uint32_t load_raw(__amdgpu_buffer_rsrc_t from, uint32_t at) {
     if constexpr (sizeof(raw_t) == 4)
         return __builtin_amdgcn_raw_buffer_load_b32(from, at, 0, 0);
     else
@@ -154,7 +151,6 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
     typedef __attribute__((ext_vector_type(MT))) uint32_t words_t;          // TURN: a lane loads the words of its wave's row tiles at once
     __shared__ u32x4 lds[U][P][8][COLS];
     __shared__ float sums[GRAD ? 64 * W : 1];
-    __shared__ int found;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int64_t tile0 = ((int64_t)blockIdx.x * W + wave) * MT;           // this wave's first row tile
     const int64_t out_rows = GRAD ? a.n_features : a.m;
@@ -164,8 +160,6 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
     constexpr int UNIT = SRC == TURN ? 1 : 4;                              // K-steps of a step of the plan
     const int first = blockIdx.z * a.steps_per_part * UNIT, last = min((int)(blockIdx.z + 1) * a.steps_per_part, a.steps) * UNIT;
     uint32_t padding[MT] = {}, any_padding = 0;                             // ROWS: which rows of a tile are padding
-    if (threadIdx.x == 0) found = 0;
-    __syncthreads();
 
     // the term that stands at place r (0..63) of K-step ks
     auto term = [&](int ks, int r) -> int64_t {
@@ -181,8 +175,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
     float column_sum = 0.f;
 
     // Buffer loads: one 32-bit offset a lane, and what lies behind the last term or column reads as zero.
-    raw_t b[ITEMS][8];
-    auto step_of = [&](int i) { return (i * 64 * W + wave * 64) / (8 * COLS); };                       // the same for a whole wave
+    uint32_t b[ITEMS][8];
+    auto step_of = [&](int i) { return PASSES * 64 * W == 8 * COLS ? i / PASSES : (i * 64 * W + wave * 64) / (8 * COLS); };      // the same for a whole wave
     auto group_of = [&](int i) -> int { return (i * 64 * W + threadIdx.x) % (8 * COLS) / COLS; };
     uint32_t at_b[PASSES];
 #pragma unroll
@@ -205,7 +199,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             const int u = step_of(i), g = group_of(i);
-            raw_t(&v)[8] = b[i];
+            uint32_t(&v)[8] = b[i];
             if constexpr (GRAD) {
                 const uint64_t real = SRC == TURN || a.rows ? real_at(u) : ~0ull;      // TURN: a part may end inside the U K-steps
                 if (real != ~0ull) {
@@ -224,27 +218,12 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
                 }
             }
             if constexpr (TYPE == STAG_F32) {
-                // an infinity or NaN makes NaN of the remainder, whatever the others are
-                auto cut = [&](uint32_t *y, uint32_t *z) -> float {
-                    float sum = 0.f;
-#pragma unroll
-                    for (int q = 0; q < 8; ++q) {
-                        const float left = __uint_as_float(v[q]) - __uint_as_float(v[q] & 0xffff0000u);        // exact: the low 16 bits
-                        const float rest = left - __uint_as_float(__float_as_uint(left) & 0xffff0000u);        // exact: the low 8 bits
-                        y[q] = __float_as_uint(left);
-                        z[q] = __float_as_uint(rest);
-                        sum += rest;
-                    }
-                    return sum;
-                };
                 uint32_t y[8], z[8];
-                const float sum = cut(y, z);
-                if (!(sum == sum)) {
-                    found = 1;
 #pragma unroll
-                    for (int q = 0; q < 8; ++q)
-                        if (not_finite<TYPE>(v[q])) v[q] = 0;
-                    cut(y, z);
+                for (int q = 0; q < 8; ++q) {
+                    const float left = __uint_as_float(v[q]) - __uint_as_float(v[q] & 0xffff0000u);        // exact: the low 16 bits
+                    y[q] = __float_as_uint(left);
+                    z[q] = __float_as_uint(left - __uint_as_float(y[q] & 0xffff0000u));                    // exact: the low 8 bits
                 }
                 u32x4 p0, p1, p2;
 #pragma unroll
@@ -257,21 +236,13 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
                 lds[u][P > 1 ? 1 : 0][g][col] = p1;
                 lds[u][P > 2 ? 2 : 0][g][col] = p2;
             } else {
-                constexpr uint32_t EXPONENT = TYPE == STAG_BF16 ? 0x7f807f80u : 0x7c007c00u, ONE = TYPE == STAG_BF16 ? 0x00800080u : 0x04000400u;
                 u32x4 p0;
-                uint32_t over = 0;       // bit 15 and bit 31: an exponent of ones came by
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    p0[j] = (uint32_t)v[2 * j] | (uint32_t)v[2 * j + 1] << 16;
-                    over |= (p0[j] & EXPONENT) + ONE;
-                }
-                if (over & 0x80008000u) {
-                    found = 1;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (not_finite<TYPE>(p0[j] & 0xffffu)) p0[j] &= 0xffff0000u;
-                        if (not_finite<TYPE>(p0[j] >> 16)) p0[j] &= 0x0000ffffu;
-                    }
+                    // Kept in registers of their own up to here: a load into the upper half of one that another load is to fill waits
+                    // for that load, and 32 loads one after the other took 236 us where these take 130.
+                    asm("" : "+v"(v[2 * j]), "+v"(v[2 * j + 1]));
+                    p0[j] = v[2 * j] | v[2 * j + 1] << 16;
                 }
                 lds[u][0][g][col] = p0;
             }
@@ -321,21 +292,33 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
                 if (row[t] && w < a.words) x[t] = *(const u32x4 *)(row[t] + w);
             }
         };
-        auto real_of = [&](int ks) -> uint64_t {
-            if constexpr (SRC == TURNED) return valid[(ks >> 2) * 8 + (ks & 3)] | (uint64_t)valid[(ks >> 2) * 8 + (ks & 3) + 4] << 32;
-            return ~0ull;
+        uint32_t real[8];                                                   // TURNED: which of the U K-steps' rows are no padding
+        auto load_real = [&](int sb) {
+            if constexpr (SRC == TURNED) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) real[q] = valid[sb * 8 + q];
+            }
+        };
+        auto real_at = [&](int u) -> uint64_t {
+            if constexpr (SRC != TURNED) return ~0ull;
+            uint32_t lo = real[0], hi = real[4];
+#pragma unroll
+            for (int i = 1; i < U; ++i) lo = u == i ? real[i] : lo, hi = u == i ? real[4 + i] : hi;
+            return (uint32_t)__builtin_amdgcn_readfirstlane(lo) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(hi) << 32;
         };
         u32x4 x[MT], next[MT];
         load_b(first);
         load_x(first >> 2, x);
+        load_real(first >> 2);
 #pragma unroll 1
         for (int ks = first; ks < last; ks += U) {
             const bool more = ks + U < last;
-            store_b([&](int u) { return real_of(ks + u); });
+            store_b(real_at);
             __syncthreads();
             if (more) {
                 load_x((ks + U) >> 2, next);
                 load_b(ks + U);
+                load_real((ks + U) >> 2);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -444,22 +427,37 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
             }
         }
     }
-    if (found && to) {       // the terms left out above, to the results whose rows have the bit
-        __syncthreads();
-        for (int e = threadIdx.x; e < 32 * W * MT * COLS; e += 64 * W) {
-            const int64_t r = (int64_t)blockIdx.x * 32 * W * MT + e / COLS;
-            const int cc = c0 + e % COLS;
-            if (r >= out_rows || cc >= a.k) continue;
-            const int64_t end = min(limit, term(last, 0));
+    // A sum that is not finite: an infinity or NaN may have met a zero bit.  Added up again, from the terms that the row has.
+    if (!to) return;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int cc = c0 + 32 * n + (lane & 31);
+        float probe = 0.f;
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) probe = fmaf(acc[t][n][i], 0.f, probe);
+        if (probe == 0.f || cc >= a.k) continue;
+        const int64_t end = min(limit, term(last, 0));
+        for (int e = 0; e < 16 * MT; ++e) {
+            const int64_t r = tile0 * 32 + 32 * (e >> 4) + 8 * (e >> 2 & 3) + 4 * half + (e & 3);
+            if (r >= out_rows) break;
             float s = 0.f;
-            for (int64_t at = term(first, 0); at < end; ++at) {
-                const raw_t v = ((const raw_t *)a.mat)[at * a.mat_stride + cc];
-                if (!not_finite<TYPE>(v)) continue;
-                const int64_t bit = GRAD ? r : at;
-                const uint32_t *words = row_of(a.bits, a.n, a.row_stride, a.rows, GRAD ? at : r);
-                if (words && (words[bit >> 5] >> (bit & 31) & 1u)) s += value_of<TYPE>(v);
+            if constexpr (GRAD) {
+                for (int64_t at = term(first, 0); at < end && s == s; ++at) {
+                    const uint32_t *words = row_of(a.bits, a.n, a.row_stride, a.rows, at);
+                    if (words && (words[r >> 5] >> (r & 31) & 1u)) s += value_of<TYPE>(((const raw_t *)a.mat)[at * a.mat_stride + cc]);
+                }
+            } else {
+                const uint32_t *words = row_of(a.bits, a.n, a.row_stride, a.rows, r);
+                if (!words) continue;
+                for (int64_t w = term(first, 0) >> 5; 32 * w < end && s == s; ++w)
+                    for (uint32_t bits = words[w]; bits; bits &= bits - 1) {
+                        const int64_t at = 32 * w + __builtin_ctz(bits);
+                        if (at < end) s += value_of<TYPE>(((const raw_t *)a.mat)[at * a.mat_stride + cc]);
+                    }
             }
-            if (!(s == 0.f)) to[r * stride + cc] += whole ? s * a.scale : s;
+            to[r * stride + cc] = whole ? s * a.scale + (!GRAD && a.bias ? a.bias[cc] : 0.f) : 2.f * s;
         }
     }
 }
