@@ -7,6 +7,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <type_traits>
 
 namespace {
 
@@ -57,8 +58,6 @@ __device__ __forceinline__ const uint32_t *row_of(const uint32_t *bits, int64_t 
 // in 16 bits; a 32-bit coefficient is cut into three bf16 pieces of 8 bits each, which together are the coefficient,
 // and multiplied piece by piece into the same 32-bit sums.  16-bit coefficients go in as they are.
 //
-// An infinity or NaN that meets a zero bit makes NaN of a sum that it has no part in: sums that come out not finite are added up
-// again, term by term (slow, and only then).
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
@@ -86,6 +85,10 @@ struct ProductArgs {
 template <int TYPE> struct Raw { typedef uint16_t type; };
 template <> struct Raw<STAG_F32> { typedef uint32_t type; };
 
+template <int TYPE> __device__ __forceinline__ bool not_finite(uint32_t raw) {
+    constexpr uint32_t ONES = TYPE == STAG_F32 ? 0x7f800000u : TYPE == STAG_BF16 ? 0x7f80u : 0x7c00u;
+    return (raw & ONES) == ONES;
+}
 template <int TYPE> __device__ __forceinline__ float value_of(uint32_t raw) {
     return TYPE == STAG_F32 ? __uint_as_float(raw) : TYPE == STAG_BF16 ? __uint_as_float(raw << 16) : (float)__builtin_bit_cast(f16, (uint16_t)raw);
 }
@@ -134,7 +137,10 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x, int lane) {
 // turns out of their packed rows as it goes; TURNED: a feature, from bits that k_turn has laid out by feature before.
 enum Source { ROWS, TURN, TURNED };
 
+typedef const uint32_t __attribute__((address_space(4))) *const_words;      // read through the scalar cache
+
 constexpr int W = 8;      // waves of a workgroup
+constexpr int NOTES = 1024;      // groups of U K-steps
 
 // A workgroup of W waves makes W MT x 32 rows of the result by NT x 32 columns; a wave its own MT row tiles.  A K-step
 // is 64 terms of the sum: two words of bits, one for each half of the wave (the matrix instruction takes 8 terms from
@@ -151,6 +157,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
     typedef __attribute__((ext_vector_type(MT))) uint32_t words_t;          // TURN: a lane loads the words of its wave's row tiles at once
     __shared__ u32x4 lds[U][P][8][COLS];
     __shared__ float sums[GRAD ? 64 * W : 1];
+    __shared__ int note[NOTES], noted, met, bad;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int64_t tile0 = ((int64_t)blockIdx.x * W + wave) * MT;           // this wave's first row tile
     const int64_t out_rows = GRAD ? a.n_features : a.m;
@@ -168,11 +175,11 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
     };
 
     f32x16 acc[MT][NT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[t][n] = (f32x16)(0.f);
-    float column_sum = 0.f;
+    float column_sum;
+    // An infinity or NaN that met a zero bit has made NaN of a sum that it has no part in.  If a sum is not finite after the first
+    // sweep, a second one takes such coefficients for zeros and notes the K-steps that have them; they are added afterwards to
+    // the sums whose rows have the bit.
+    if (threadIdx.x == 0) noted = met = bad = 0;
 
     // Buffer loads: one 32-bit offset a lane, and what lies behind the last term or column reads as zero.
     uint32_t b[ITEMS][8];
@@ -195,7 +202,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
         }
     };
     // `real_at`: which of a K-step's rows are no padding (GRAD); the others are zeros, whatever the memory holds
-    auto store_b = [&](auto real_at) {
+    auto store_b = [&](auto careful, auto real_at) {
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             const int u = step_of(i), g = group_of(i);
@@ -216,6 +223,14 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
                     for (int q = 0; q < 8; ++q) s += value_of<TYPE>(v[q]);
                     column_sum += s;
                 }
+            }
+            if constexpr (careful.value) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (not_finite<TYPE>(v[q])) {
+                        met = 1;
+                        v[q] = 0;
+                    }
             }
             if constexpr (TYPE == STAG_F32) {
                 uint32_t y[8], z[8];
@@ -270,118 +285,172 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
         }
     };
 
-    if constexpr (SRC != TURN) {
-        const uint32_t *row[MT];
+    auto sweep = [&](auto careful) -> bool {
+        column_sum = 0.f;
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const int64_t i = (tile0 + t) * 32 + (lane & 31);
-            if constexpr (SRC == ROWS) {
-                row[t] = i < a.m ? row_of(a.bits, a.n, a.row_stride, a.rows, i) : nullptr;
-                padding[t] = (uint32_t)__ballot(row[t] == nullptr);
-                any_padding |= padding[t];
-            } else {
-                row[t] = i < out_rows ? a.turned + i * a.words : nullptr;
-            }
-        }
-        const uint32_t *valid = SRC == TURNED ? a.turned + out_rows * a.words : nullptr;
-        auto load_x = [&](int sb, u32x4 *x) {
-            const int w = sb * 8 + half * 4;
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[t][n] = (f32x16)(0.f);
+        if constexpr (SRC != TURN) {
+            const uint32_t *row[MT];
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                x[t] = (u32x4)(0u);
-                if (row[t] && w < a.words) x[t] = *(const u32x4 *)(row[t] + w);
-            }
-        };
-        uint32_t real[8];                                                   // TURNED: which of the U K-steps' rows are no padding
-        auto load_real = [&](int sb) {
-            if constexpr (SRC == TURNED) {
-#pragma unroll
-                for (int q = 0; q < 8; ++q) real[q] = valid[sb * 8 + q];
-            }
-        };
-        auto real_at = [&](int u) -> uint64_t {
-            if constexpr (SRC != TURNED) return ~0ull;
-            uint32_t lo = real[0], hi = real[4];
-#pragma unroll
-            for (int i = 1; i < U; ++i) lo = u == i ? real[i] : lo, hi = u == i ? real[4 + i] : hi;
-            return (uint32_t)__builtin_amdgcn_readfirstlane(lo) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(hi) << 32;
-        };
-        u32x4 x[MT], next[MT];
-        load_b(first);
-        load_x(first >> 2, x);
-        load_real(first >> 2);
-#pragma unroll 1
-        for (int ks = first; ks < last; ks += U) {
-            const bool more = ks + U < last;
-            store_b(real_at);
-            __syncthreads();
-            if (more) {
-                load_x((ks + U) >> 2, next);
-                load_b(ks + U);
-                load_real((ks + U) >> 2);
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                uint32_t w[MT];
-#pragma unroll
-                for (int t = 0; t < MT; ++t) w[t] = x[t][u];
-                multiply(u, w);
-            }
-            __syncthreads();
-#pragma unroll
-            for (int t = 0; t < MT; ++t) x[t] = next[t];
-        }
-    } else {
-        const int64_t w0 = tile0 < a.words ? tile0 : a.words - MT;
-        const uint32_t *row[U];
-        words_t x[U];
-        uint64_t real[U];
-        auto load_row = [&](int u, int ks) {
-            const int64_t i = (int64_t)ks * 64 + lane;
-            row[u] = ks < last && i < a.m ? row_of(a.bits, a.n, a.row_stride, a.rows, i) : nullptr;
-        };
-        auto load_x = [&](int u) {
-            real[u] = __ballot(row[u] != nullptr);
-            x[u] = row[u] ? *(const words_t *)(row[u] + w0) : (words_t)(0u);
-        };
-        auto real_at = [&](int u) {
-            uint64_t r = real[0];
-#pragma unroll
-            for (int i = 1; i < U; ++i) r = u == i ? real[i] : r;
-            return r;
-        };
-#pragma unroll
-        for (int u = 0; u < U; ++u) load_row(u, first + u);
-        load_b(first);
-#pragma unroll
-        for (int u = 0; u < U; ++u) load_x(u);
-#pragma unroll
-        for (int u = 0; u < U; ++u) load_row(u, first + U + u);
-#pragma unroll 1
-        for (int ks = first; ks < last; ks += U) {
-            const bool more = ks + U < last;
-            store_b(real_at);
-            __syncthreads();
-            words_t now[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) now[u] = x[u];
-            if (more) {
-                load_b(ks + U);
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    load_x(u);
-                    load_row(u, ks + 2 * U + u);
+                const int64_t i = (tile0 + t) * 32 + (lane & 31);
+                if constexpr (SRC == ROWS) {
+                    row[t] = i < a.m ? row_of(a.bits, a.n, a.row_stride, a.rows, i) : nullptr;
+                    padding[t] = (uint32_t)__ballot(row[t] == nullptr);
+                    any_padding |= padding[t];
+                } else {
+                    row[t] = i < out_rows ? a.turned + i * a.words : nullptr;
                 }
             }
+            const auto valid = (const_words)(uintptr_t)(SRC == TURNED ? a.turned + out_rows * a.words : nullptr);
+            auto load_x = [&](int sb, u32x4 *x) {
+                const int w = sb * 8 + half * 4;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                uint32_t w[MT];
+                for (int t = 0; t < MT; ++t) {
+                    x[t] = (u32x4)(0u);
+                    if (row[t] && w < a.words) x[t] = *(const u32x4 *)(row[t] + w);
+                }
+            };
+            uint32_t real[8];                                                   // TURNED: which of the U K-steps' rows are no padding
+            auto load_real = [&](int sb) {
+                if constexpr (SRC == TURNED) {
 #pragma unroll
-                for (int t = 0; t < MT; ++t) w[t] = transposed(now[u][t], lane);
-                multiply(u, w);
+                    for (int q = 0; q < 8; ++q) real[q] = valid[sb * 8 + q];
+                }
+            };
+            auto real_at = [&](int u) -> uint64_t {
+                if constexpr (SRC != TURNED) return ~0ull;
+                uint32_t lo = real[0], hi = real[4];
+#pragma unroll
+                for (int i = 1; i < U; ++i) lo = u == i ? real[i] : lo, hi = u == i ? real[4 + i] : hi;
+                return (uint32_t)__builtin_amdgcn_readfirstlane(lo) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(hi) << 32;
+            };
+            u32x4 x[MT], next[MT];
+            load_b(first);
+            load_x(first >> 2, x);
+            load_real(first >> 2);
+#pragma unroll 1
+            for (int ks = first; ks < last; ks += U) {
+                const bool more = ks + U < last;
+                store_b(careful, real_at);
+                __syncthreads();
+                if (careful.value && threadIdx.x == 0 && met) {
+                    if (noted < NOTES) note[noted] = ks;
+                    ++noted;
+                    met = 0;
+                }
+                if (more) {
+                    load_x((ks + U) >> 2, next);
+                    load_real((ks + U) >> 2);
+                    load_b(ks + U);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    uint32_t w[MT];
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) w[t] = x[t][u];
+                    multiply(u, w);
+                }
+                __syncthreads();
+#pragma unroll
+                for (int t = 0; t < MT; ++t) x[t] = next[t];
             }
-            __syncthreads();
+        } else {
+            const int64_t w0 = tile0 < a.words ? tile0 : a.words - MT;
+            const uint32_t *row[U];
+            words_t x[U];
+            uint64_t real[U];
+            auto load_row = [&](int u, int ks) {
+                const int64_t i = (int64_t)ks * 64 + lane;
+                row[u] = ks < last && i < a.m ? row_of(a.bits, a.n, a.row_stride, a.rows, i) : nullptr;
+            };
+            auto load_x = [&](int u) {
+                real[u] = __ballot(row[u] != nullptr);
+                x[u] = row[u] ? *(const words_t *)(row[u] + w0) : (words_t)(0u);
+            };
+            auto real_at = [&](int u) {
+                uint64_t r = real[0];
+#pragma unroll
+                for (int i = 1; i < U; ++i) r = u == i ? real[i] : r;
+                return r;
+            };
+#pragma unroll
+            for (int u = 0; u < U; ++u) load_row(u, first + u);
+            load_b(first);
+#pragma unroll
+            for (int u = 0; u < U; ++u) load_x(u);
+#pragma unroll
+            for (int u = 0; u < U; ++u) load_row(u, first + U + u);
+#pragma unroll 1
+            for (int ks = first; ks < last; ks += U) {
+                const bool more = ks + U < last;
+                store_b(careful, real_at);
+                __syncthreads();
+                if (careful.value && threadIdx.x == 0 && met) {
+                    if (noted < NOTES) note[noted] = ks;
+                    ++noted;
+                    met = 0;
+                }
+                words_t now[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) now[u] = x[u];
+                if (more) {
+                    load_b(ks + U);
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        load_x(u);
+                        load_row(u, ks + 2 * U + u);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    uint32_t w[MT];
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) w[t] = transposed(now[u][t], lane);
+                    multiply(u, w);
+                }
+                __syncthreads();
+            }
         }
+        float probe = 0.f;
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) probe = fmaf(acc[t][n][i], 0.f, probe);
+        return probe == 0.f;
+    };
+    if (!sweep(std::false_type())) bad = 1;
+    __syncthreads();
+    const bool careful = bad;
+    if (careful) {
+        sweep(std::true_type());
+        __syncthreads();
+        for (int e = 0; e < min(noted, NOTES); ++e)
+            for (int q = 0; q < 64 * U; ++q) {
+                const int64_t at = term(note[e] + q / 64, q % 64);
+                if (note[e] + q / 64 >= last || at >= limit) continue;
+                const uint32_t *words = GRAD ? row_of(a.bits, a.n, a.row_stride, a.rows, at) : nullptr;
+                if (GRAD && !words) continue;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const int cc = c0 + 32 * n + (lane & 31);
+                    const uint32_t v = cc < a.k ? ((const raw_t *)a.mat)[at * a.mat_stride + cc] : 0;
+                    if (!not_finite<TYPE>(v)) continue;
+#pragma unroll
+                    for (int t = 0; t < MT; ++t)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int64_t r = (tile0 + t) * 32 + 8 * (i >> 2) + 4 * half + (i & 3), bit = GRAD ? r : at;
+                            if (r >= out_rows) continue;
+                            const uint32_t *of = GRAD ? words : row_of(a.bits, a.n, a.row_stride, a.rows, r);
+                            if (of && (of[bit >> 5] >> (bit & 31) & 1u)) acc[t][n][i] += value_of<TYPE>(v);
+                        }
+                }
+            }
     }
 
     const bool whole = gridDim.z == 1;
@@ -427,8 +496,9 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
             }
         }
     }
-    // A sum that is not finite: an infinity or NaN may have met a zero bit.  Added up again, from the terms that the row has.
-    if (!to) return;
+    // Still not finite without having met an infinity or NaN (or with more K-steps of them than could be noted): twice the sum, which
+    // is what the matrix cores make, may be too large where the sum is not.  Added up term by term.
+    if (!careful || !to || (noted && noted <= NOTES)) return;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int cc = c0 + 32 * n + (lane & 31);
