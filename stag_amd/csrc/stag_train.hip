@@ -58,6 +58,10 @@ __device__ __forceinline__ const uint32_t *row_of(const uint32_t *bits, int64_t 
 // in 16 bits; a 32-bit coefficient is cut into three bf16 pieces of 8 bits each, which together are the coefficient,
 // and multiplied piece by piece into the same 32-bit sums.  16-bit coefficients go in as they are.
 //
+// What bounds them: the matrix cores for 32-bit coefficients (8,192 rows x 7,500 features x 1,000 columns: 237 us, 1.6 PFLOP/s of bf16
+// operations counted densely; a library's bf16 product of 8,192^3 reaches 1.19 on the same card), the making of operands
+// beside them for 16-bit ones (that size's gradient in bf16: 119 us, 1.06 PFLOP/s), latency for one node's batch (4,096 x
+// 7,500 x 13: 10 us and 3 for adding up its parts).
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
@@ -146,6 +150,11 @@ constexpr int NOTES = 1024;      // groups of U K-steps
 // is 64 terms of the sum: two words of bits, one for each half of the wave (the matrix instruction takes 8 terms from
 // each half), in four instructions of 16 terms.  The workgroup loads the coefficients of U K-steps, 64 U x 32 NT, cuts them into pieces
 // and stores them to LDS in operand order; the next ones are in flight while the matrix cores work on these.
+//
+// Why these tiles: 2 x 2 tiles a wave make 8 (or 24) matrix instructions of the 4 (or 6) operands loaded from LDS and two made
+// from bits, and 8 waves share what the workgroup cuts, at two waves a SIMD (150 to 190 registers).  Measured at the level's size, scores in
+// 32 bits and gradient in bf16, in us: 4 waves of 4 x 2 tiles with the sum in two parts 273 and 157; 8 of 2 x 2, one K-step a barrier 290
+// and 164, two 275 and 142, four 260 and 135; two buffers in LDS instead of one gained nothing.  One tile a wave where there are few.
 template <int TYPE, Source SRC, int MT, int NT>
 __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
     typedef typename Raw<TYPE>::type raw_t;
