@@ -20,8 +20,11 @@
  * DEVICE pointers on the current device; calls enqueue work on `stream` (a hipStream_t as void*; NULL = the null stream),
  * allocate nothing and do not synchronise, so they can be captured into a HIP graph.  d_work is scratch memory of at
  * least the bytes that the matching *_workspace function returns, 256-byte aligned; its contents are not kept between
- * calls, and two calls that may run at the same time need two of them.  Results do not depend on timing: equal
- * inputs give equal bits.
+ * calls, and two calls that may run at the same time need two of them.  Outputs and d_work share memory with nothing else
+ * that a call takes.  Results do not depend on timing: equal inputs give equal bits.
+ *
+ * Sizes: 0 <= m < 2^31 rows of a batch, 1 <= k <= 2^20 classifiers, 1 <= n_features <= 2^27; the strides of tables, scores and
+ * gradients are at least k and at most 2^21 values.  What is larger is refused.
  */
 #ifndef STAG_TRAIN_H
 #define STAG_TRAIN_H
@@ -99,11 +102,12 @@ int stag_sibling_loss_dev(const float *d_scores, int64_t score_stride, int64_t m
  * state_values values.  state_bits 32: d_m, d_v are floats.  state_bits 8: d_m holds e4m3 codes of m / s and d_v of
  * sqrt(v) / s, where s = d_m_scale[b], d_v_scale[b] is a power of two for each 256 values; a value between two codes goes
  * to either by a hash of its place and t, so that it is right on the mean: with beta2 = 0.999 a step moves sqrt(v) by
- * 1/2000 of itself, which rounding to nearest would lose every time.
+ * 1/2000 of itself, which rounding to nearest would lose every time.  A second moment that overflows is kept as an infinity
+ * (the value then stands still) with 32 bits and becomes NaN, as the value does one step later, with 8.
  *
  * d_tensors: n descriptors in device memory; d_tiles: for each STAG_ADAMW_TILE values of each tensor (the last tile
  * of a tensor may be shorter) its tensor and its number in the tensor.  d_step: STAG_ADAMW_STEP_WORDS words, t and then
- * zeros, which the call leaves zero.
+ * zeros, which the call leaves zero.  Two steps that share any of these buffers have to run one after the other.
  */
 #define STAG_ADAMW_BLOCK 256
 #define STAG_ADAMW_TILE 1024

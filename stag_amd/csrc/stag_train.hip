@@ -80,9 +80,9 @@ struct ProductArgs {
     float *out, *bias_out;      // bias_out: grad: column sums
     int64_t out_stride;
     const uint32_t *turned;     // TURNED: the bits by feature, see k_turn
-    float *part;                // more than one part: raw sums [parts][result rows][k], then column sums [parts][k]
+    float *part;                // more than one part: their sums [parts][result rows][k], then column sums [parts][k]
     int32_t n_features, words, k;       // words of a row of bits (TURNED: of a turned row)
-    int32_t steps, steps_per_part;      // in units of 4 K-steps (scores), 1 K-step (grad)
+    int32_t steps, steps_per_part;      // in units of 4 K-steps (TURN: of 1)
     float scale;
 };
 
@@ -435,8 +435,9 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
     if (!sweep(std::false_type())) bad = 1;
     __syncthreads();
     const bool careful = bad;
+    bool overflowed = false;
     if (careful) {
-        sweep(std::true_type());
+        overflowed = !sweep(std::true_type());
         __syncthreads();
         for (int e = 0; e < min(noted, NOTES); ++e)
             for (int q = 0; q < 64 * U; ++q) {
@@ -465,7 +466,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
     const bool whole = gridDim.z == 1;
     float *to = whole ? a.out : a.part + (int64_t)blockIdx.z * out_rows * a.k;
     const int64_t stride = whole ? a.out_stride : a.k;
-    const float scale = whole ? 0.5f * a.scale : 1.f;
+    const float scale = whole ? 0.5f * a.scale : 0.5f;
     const auto into = buffer(to + tile0 * 32 * stride, to ? (out_rows - tile0 * 32) * stride * 4 : 0);
     const uint32_t row_to = (uint32_t)stride * 4;
 #pragma unroll
@@ -505,9 +506,9 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
             }
         }
     }
-    // Still not finite without having met an infinity or NaN (or with more K-steps of them than could be noted): twice the sum, which
-    // is what the matrix cores make, may be too large where the sum is not.  Added up term by term.
-    if (!careful || !to || (noted && noted <= NOTES)) return;
+    // Not finite without the infinities and NaN (or with more K-steps of those than could be noted): twice the sum, which is what the
+    // matrix cores make, may be too large where the sum is not.  Added up term by term.
+    if (!to || (!overflowed && (!careful || noted <= NOTES))) return;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int cc = c0 + 32 * n + (lane & 31);
@@ -536,7 +537,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
                         if (at < end) s += value_of<TYPE>(((const raw_t *)a.mat)[at * a.mat_stride + cc]);
                     }
             }
-            to[r * stride + cc] = whole ? s * a.scale + (!GRAD && a.bias ? a.bias[cc] : 0.f) : 2.f * s;
+            to[r * stride + cc] = whole ? s * a.scale + (!GRAD && a.bias ? a.bias[cc] : 0.f) : s;
         }
     }
 }
@@ -592,7 +593,7 @@ __global__ __launch_bounds__(256) void k_join(ProductArgs a, int parts, int64_t 
     const int64_t r = at / a.k;
     const int c = (int)(at - r * a.k);
     const bool padding = !GRAD && a.rows && !row_of(a.bits, a.n, a.row_stride, a.rows, r);
-    if (a.out) a.out[r * a.out_stride + c] = padding ? 0.f : s * (0.5f * a.scale) + (!GRAD && a.bias ? a.bias[c] : 0.f);
+    if (a.out) a.out[r * a.out_stride + c] = padding ? 0.f : s * a.scale + (!GRAD && a.bias ? a.bias[c] : 0.f);
 }
 
 // Few rows: the lookups themselves.  A workgroup makes one row of scores, `cw` columns of it (a power of two up to 64): it

@@ -15,7 +15,8 @@ these steps for the children of one node and returns coefficients in the form ``
 
 All functions take torch tensors on one GPU, enqueue their work on that GPU's current stream and return without waiting;
 they take no part in autograd.  With their outputs given (``out=``) or allocated under capture they can be recorded into a
-HIP graph.  Inputs whose rows are not contiguous are copied first; outputs have to be as documented.
+HIP graph.  Inputs whose rows are not contiguous (or lie more than 2^21 values apart) are copied first; outputs have to be as
+documented and may share memory with nothing else that the call takes.
 """
 import functools
 import math
@@ -37,6 +38,7 @@ _BITS = (torch.int32, torch.uint32)
 _empty = torch.empty_strided
 _raw_stream = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream(i).cuda_stream without the objects
 _current = torch._C._cuda_getDevice
+_MAX_STRIDE = 1 << 21                                # values from one row of a matrix to the next
 
 
 def _need(cond, msg, *args):
@@ -72,7 +74,7 @@ def _one_gpu(**tensors):
 def _rows(t):
     """t with contiguous rows (copied if they are not), and its row stride."""
     n, k = t.shape
-    if (k > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < k):
+    if (k > 1 and t.stride(1) != 1) or (n > 1 and not k <= t.stride(0) <= _MAX_STRIDE):
         t = t.contiguous()
     return t, (t.stride(0) if n > 1 else k)
 
@@ -84,7 +86,37 @@ def _out_rows(name, t, shape, dtype):
         _need(shape[0] <= 1 or t.stride(0) == 1, "%s must be contiguous", name)
         return shape[0]
     _need((shape[1] <= 1 or t.stride(1) == 1) and (shape[0] <= 1 or t.stride(0) >= shape[1]), "%s must have contiguous rows that do not overlap", name)
+    _need(shape[0] <= 1 or t.stride(0) <= _MAX_STRIDE, "%s has rows more than %d values apart", name, _MAX_STRIDE)
     return t.stride(0) if shape[0] > 1 else shape[1]
+
+
+def _share(a, b):
+    """Whether two tensors of contiguous rows share memory."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    place = []
+    for t in (a, b):
+        size, rows = t.element_size(), t.shape[0] if t.dim() == 2 else 1
+        step = t.stride(0) * size if rows > 1 else 0
+        width = t.shape[-1] * size
+        place.append((t.data_ptr(), step, width, (rows - 1) * step + width))
+    (at, step_a, width_a, all_a), (bt, step_b, width_b, all_b) = place
+    if at + all_a <= bt or bt + all_b <= at:
+        return False
+    step = step_a or step_b
+    if not step or (step_a and step_b and step_a != step_b):
+        return True
+    apart = (at - bt) % step                           # columns of one buffer
+    return apart < width_b or apart + width_a > step
+
+
+def _apart(outputs, inputs):
+    """Refuses outputs that share memory with one another or an input."""
+    named = list(outputs.items())
+    for j, (name, t) in enumerate(named):
+        for other, u in named[j + 1:] + list(inputs.items()):
+            if u is not None and t is not None and _share(t, u):
+                raise ValueError("%s and %s share memory" % (name, other))
 
 
 def _packed(bits, n_features):
@@ -127,6 +159,7 @@ def _check_scores(bits, table, bias, rows, out):
     _one_gpu(bits=bits, table=table, bias=bias, rows=rows, out=out)
     bits, row_stride = _packed(bits, n_features)
     table, table_stride = _rows(table)
+    _apart({"out": out}, {"bits": bits, "table": table, "bias": bias, "rows": rows})
     return bits, table, bias, rows, row_stride, table_stride, score_stride
 
 
@@ -184,6 +217,7 @@ def _check_grad(bits, grad, n_features, rows, out):
     _one_gpu(bits=bits, grad=grad, rows=rows, table_grad=table_grad, bias_grad=bias_grad)
     bits, row_stride = _packed(bits, n_features)
     grad, grad_stride = _rows(grad)
+    _apart({"out[0]": table_grad, "out[1]": bias_grad}, {"bits": bits, "grad": grad, "rows": rows})
     return bits, grad, rows, row_stride, grad_stride, stride
 
 
@@ -199,7 +233,7 @@ def row_scores_grad(bits, grad, n_features, *, scale=1.0, rows=None, out=None):
         if gpu >= 0 and grad.get_device() == gpu and bits.dim() == 2 and grad.dim() == 2 and bits.dtype in _BITS:
             (n, row_stride), (m, k) = bits.shape, grad.shape
             if (row_stride & 3 == 0 and k and m and 0 < n_features <= row_stride * 32 and (n == m if rows is None else _plain(rows, _I32, (m,), gpu))
-                    and (out is None or (_plain(out[0], _F32, (n_features, k), gpu) and _plain(out[1], _F32, (k,), gpu)))):
+                    and out is None):
                 kind = 0 if grad.dtype is _F32 else _TYPES.get(grad.dtype, -1)
                 grad_stride = stride = k
     if kind < 0:
@@ -248,6 +282,7 @@ def _check_loss(scores, label, siblings, weight, dtype, out):
         grad_stride = _out_rows("out[1]", grad, (m, k), dtype)
     _one_gpu(scores=scores, label=label, siblings=siblings, weight=weight, loss=loss, grad=grad)
     scores, score_stride = _rows(scores)
+    _apart({"out[0]": loss, "out[1]": grad}, {"scores": scores, "label": label, "siblings": siblings, "weight": weight})
     return scores, label, siblings, weight, score_stride, grad_stride
 
 
@@ -298,6 +333,7 @@ class AdamW:
     weight_decay, l1: a number, or one for each tensor.  state_bits 32 keeps the moments as floats; 8 keeps e4m3 codes with a
     power-of-two scale for each 256 values (m, m_scale: the first moment; v, v_scale: the ROOT of the second), 2.03 bytes
     a value instead of 8.  m, v and the scales are flat: tensor j's values begin at place state_at[j], a multiple of 256.
+    Addresses are taken once, so an AdamW is neither copied nor pickled: make another, and load_state() into it.
     The step count lives on the GPU, so a captured step() counts on when it is replayed; lr and the others are the values that
     step() was called with (attributes, may be changed between steps)."""
 
@@ -345,7 +381,7 @@ class AdamW:
                 k = int(bad[0]) + 1
                 before = max((int(end[q]), int(q)) for q, o in zip(order[:k], others[:k]) if o)[1]
                 raise ValueError("%s and %s share memory" % (name(before), name(int(order[k]))))
-        self.device, self.params, self.grads = device, params, grads
+        self._device, self._params, self._grads = device, tuple(params), tuple(grads)
         table = np.zeros(n, dtype=_TENSOR)
         padded = -(-counts // BLOCK) * BLOCK
         self.state_at = np.concatenate([[0], np.cumsum(padded)[:-1]]).tolist()
@@ -375,11 +411,15 @@ class AdamW:
         self._where = (self._tensors.data_ptr(), self._tiles.data_ptr(), self._n_tiles, state_bits, self._m.data_ptr(), self._v.data_ptr(), _ptr(self._m_scale),
                        _ptr(self._v_scale), self._step.data_ptr())
 
-    m, v, m_scale, v_scale = (property(lambda self, name=name: getattr(self, name)) for name in ("_m", "_v", "_m_scale", "_v_scale"))
+    device, params, grads, m, v, m_scale, v_scale = (
+        property(lambda self, name=name: getattr(self, name)) for name in ("_device", "_params", "_grads", "_m", "_v", "_m_scale", "_v_scale"))
+
+    def __reduce_ex__(self, protocol):
+        raise TypeError("an AdamW holds the addresses of its tensors: make another, and load_state() into it")
 
     def step(self):
         """One step with the gradients as they stand."""
-        gpu = self.device.index
+        gpu = self._device.index
         if gpu != _current():
             with torch.cuda.device(gpu):
                 return self.step()
@@ -417,15 +457,25 @@ def fit_siblings(bits, label, k, n_features, *, steps=200, batch=None, lr=0.05, 
     another value = a negative example for all.  l1 penalises coefficients (not the intercept) by l1 * |w| beside the mean loss
     of a row.  batch: rows a step (default all), drawn anew each pass by `seed`."""
     if isinstance(bits, np.ndarray):
+        if bits.dtype not in (np.uint32, np.int32):
+            raise TypeError("bits is %s: uint32 words are wanted" % bits.dtype)
         bits = torch.from_numpy(np.ascontiguousarray(bits).view(np.int32)).to(device or "cuda")
+    _is("bits", bits, _BITS, 2)
     device = bits.device
     n, k, n_features = bits.shape[0], int(k), int(n_features)
     _need(n >= 1, "no rows")
-    label = torch.as_tensor(label).to(device=device, dtype=torch.int32)
+    _need(k >= 1 and n_features >= 1, "no features (%d) or no classifiers (%d)", n_features, k)
+    _need(batch is None or int(batch) >= 1, "batch = %r", batch)
+    label = torch.as_tensor(label)
     _need(tuple(label.shape) == (n,), "label has shape %s: %s is wanted", tuple(label.shape), (n,))
+    if label.is_floating_point() or label.is_complex():
+        raise TypeError("label is %s: whole numbers are wanted" % label.dtype)
+    label = label.to(device=device, dtype=torch.int64)
+    label = torch.where((label >= 0) & (label < k), label, -1).to(torch.int32)       # before 64 bits become 32
     if weight is not None:
         weight = torch.as_tensor(weight).to(device=device, dtype=torch.float32)
-    batch = n if batch is None else max(1, min(int(batch), n))
+        _need(tuple(weight.shape) == (n,), "weight has shape %s: %s is wanted", tuple(weight.shape), (n,))
+    batch = n if batch is None else min(int(batch), n)
     table = torch.zeros((n_features, k), dtype=table_dtype, device=device)
     bias = torch.zeros(k, device=device)
     table_grad, bias_grad = torch.empty((n_features, k), device=device), torch.empty(k, device=device)

@@ -155,6 +155,33 @@ def test_infinities_reach_only_the_rows_that_have_the_token(n, k, n_features, dt
     assert np.array_equal(np.isnan(got[1].cpu().numpy()), np.isnan(near_bias)) and np.array_equal(np.isinf(got[1].cpu().numpy()), np.isinf(near_bias))
 
 
+@pytest.mark.parametrize("n, k, n_features", [(1, 4, 333), (40, 5, 333), (600, 70, 333), (1500, 200, 333), (2100, 400, 2500), (700, 20, 333)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_sums_near_the_largest_number_beside_infinities(n, k, n_features, dtype):
+    """2^127 fits 32 bits, its double does not; an infinity or NaN elsewhere in the batch changes nothing about it."""
+    rng = np.random.default_rng(2)
+    bits, x = packed(rng, n, n_features)
+    table = torch.from_numpy(rng.integers(-4, 5, (n_features, k)).astype(np.float32)).to(DEV).to(dtype)
+    table[33, 0] = table[34, k // 2] = 2.0 ** 127
+    table[17, 0], table[18, k - 1] = math.inf, math.nan
+    got = train.row_scores(bits, table, scale=0.5).double().cpu().numpy()
+    t = table.double().cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        want = 0.5 * np.stack([t[r > 0].sum(0) for r in x])
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isinf(got), np.isinf(want))
+    fine = np.isfinite(want)
+    near(got[fine], want[fine], U * np.abs(want[fine]))            # whole numbers: sums of small ones are exact, beside 2^127 they are nothing
+    grad = torch.from_numpy(rng.integers(-4, 5, (n, k)).astype(np.float32)).to(DEV).to(dtype)
+    grad[n // 3, 0], grad[n // 2, k - 1], grad[n - 1, 1] = 2.0 ** 127, 2.0 ** 127, math.inf
+    got = train.row_scores_grad(bits, grad, n_features)[0].double().cpu().numpy()
+    g = grad.double().cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        want = np.stack([g[c > 0].sum(0) for c in x.T])
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isinf(got), np.isinf(want))
+    fine = np.isfinite(want)
+    near(got[fine], want[fine], U * np.abs(want[fine]))
+
+
 @pytest.mark.parametrize("dtype, smallest", [(F16, 2.0 ** -24), (BF16, 2.0 ** -133), (F32, 2.0 ** -149)])
 @pytest.mark.parametrize("n, k", [(6, 8), (700, 24)])
 def test_values_below_the_normal_ones(n, k, dtype, smallest):
@@ -510,6 +537,19 @@ def test_adamw_takes_nan_and_infinities_one_by_one(bits):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_where_the_second_moment_overflows(bits):
+    """A finite gradient whose square is not: the value stands still with 32 bits, and is NaN from the second step on with 8."""
+    p, g = torch.ones(300, device=DEV), torch.ones(300, device=DEV)
+    g[7] = 1e30
+    opt = train.AdamW([p], [g], lr=0.125, state_bits=bits)
+    opt.step()
+    assert torch.isfinite(p).all() and p[7] == 1
+    opt.step()
+    assert p[7] == 1 if bits == 32 else torch.isnan(p[7])
+    assert torch.isfinite(p[:7]).all() and torch.isfinite(p[8:]).all() and torch.isinf(opt.v[7]) if bits == 32 else torch.isnan(opt.v.float()[7])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_adamw_at_odd_addresses(bits):
     """Tensors at addresses that no vector load may use, and what lies around them."""
     rng = np.random.default_rng(1)
@@ -539,6 +579,30 @@ def test_adamw_refuses_shared_memory():
         opt.load_state(0, opt.m, opt.v, opt.m, opt.v)
     with pytest.raises(ValueError, match="values: 256 are wanted"):
         opt.load_state(0, opt.m[:100], opt.v)
+
+
+def test_outputs_over_inputs_are_refused():
+    bits, _ = packed(np.random.default_rng(0), 50, 300)
+    buffer = torch.zeros(400, 40, device=DEV)
+    label = torch.zeros(50, dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError, match="out and table share memory"):
+        train.row_scores(bits, buffer[:300, :8], out=buffer[:50, 4:12])
+    with pytest.raises(ValueError, match=r"out\[1\] and scores share memory"):
+        train.sibling_loss(buffer[:50, :8], label, out=(torch.zeros(8, device=DEV), buffer[:50, :8]))
+    with pytest.raises(ValueError, match=r"out\[0\] and grad share memory"):
+        train.row_scores_grad(bits, buffer[:50, :8], 300, out=(buffer[:300, :8], torch.zeros(8, device=DEV)))
+    buffer[:, :8] = 1
+    scores = train.row_scores(bits, buffer[:300, :8], out=buffer[:50, 8:16])         # columns beside one another
+    assert torch.equal(scores, train.row_scores(bits, torch.ones(300, 8, device=DEV))) and (buffer[:, :8] == 1).all() and (buffer[:, 16:] == 0).all()
+
+
+def test_an_optimizer_keeps_its_tensors():
+    """Its addresses stay valid whatever the caller does to the lists it was made from."""
+    params, grads = [torch.ones(1000, device=DEV)], [torch.ones(1000, device=DEV)]
+    opt = train.AdamW(params, grads, lr=0.25)
+    del params[0], grads[0]
+    opt.step()
+    assert isinstance(opt.params, tuple) and (opt.params[0] - 0.75).abs().max() < 1e-6
 
 
 # ------------------------------------------------------------------------------------------------------ used together
@@ -662,6 +726,16 @@ def test_on_two_streams_at_once():
     for j in range(2):
         for a, b in got[j]:
             assert torch.equal(a, want[j][0]) and torch.equal(b, want[j][1])
+
+
+def test_labels_of_64_bits():
+    """A label that is no sibling stays none, also where 32 bits of it would be one; so is a row of uint32 words a tensor."""
+    bits, _, label = problem(np.random.default_rng(6))
+    label = label.astype(np.int64)
+    out = np.where(np.arange(400) % 3 == 0, label + 2**32, label)
+    want = train.fit_siblings(bits, np.where(np.arange(400) % 3 == 0, -1, label), 6, 300, steps=3)
+    assert np.array_equal(train.fit_siblings(bits, out, 6, 300, steps=3), want)
+    assert np.array_equal(train.fit_siblings(bits.cpu().numpy().view(np.uint32), out, 6, 300, steps=3, batch=1000), want)
 
 
 def test_fit_siblings_feeds_the_walk():

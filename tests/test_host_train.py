@@ -1,7 +1,9 @@
 """CPU-only checks of the training operators: libstag_train.so exports what include/stag_train.h declares, and both levels
 refuse what they cannot do before anything reaches a GPU."""
+import copy
 import ctypes
 import os
+import pickle
 import re
 
 import numpy as np
@@ -147,3 +149,59 @@ def test_too_narrow_and_unaligned_rows():
     bits, stride = train._packed(rows(6, 8)[:, :4], 100)
     assert stride == 8
     assert train._packed(rows(8, 8).t(), 100)[1] == 8       # copied to contiguous rows
+
+
+def test_rows_far_apart_are_copied_or_refused():
+    """A matrix whose rows lie more than 2^21 values apart: inputs are copied, outputs refused, and so is the stride at the C entry."""
+    wide = torch.empty(2, 2**21 + 8)[:, :3]
+    assert train._rows(wide)[1] == 3 and train._rows(torch.empty(2, 2**21)[:, :3])[1] == 2**21
+    with pytest.raises(ValueError, match="rows more than 2097152 values apart"):
+        train._out_rows("out", wide, (2, 3), torch.float32)
+    for args, which, name in ((SCORES, "table_stride", "d_table"), (SCORES, "score_stride", "d_scores")):
+        assert _lib.train_lib().stag_row_scores_dev(*{**args, which: 2**21 + 1}.values()) == -1
+        message = _lib.train_lib().stag_train_last_error().decode()
+        assert name in message and "is over 2097152" in message
+
+
+def test_outputs_that_share_memory():
+    """Only tensors that have a byte in common: columns of one buffer beside one another do not."""
+    buffer = torch.zeros(6, 20)
+    share = train._share
+    assert not share(buffer[:, :5], buffer[:, 5:9]) and not share(buffer[:, 5:9], buffer[:, :5]) and not share(buffer[:, 15:], buffer[:, :15])
+    assert share(buffer[:, :5], buffer[:, 4:9]) and share(buffer[:, 4:9], buffer[:, :5]) and share(buffer[:, 3:4], buffer)
+    assert not share(buffer[:3], buffer[3:]) and share(buffer[:3], buffer[2:])
+    assert share(buffer[2, 3:9], buffer[:, 8:10]) and not share(buffer[2, 3:8], buffer[:, 8:10]) and not share(buffer[0], buffer[1])
+    assert share(buffer.view(12, 10)[:, :3], buffer[:, 10:13]) and not share(buffer, buffer.clone()) and not share(buffer[:0], buffer)
+    assert share(buffer.view(torch.int32), buffer) and share(buffer.flatten(), buffer[:, 2:3])
+    with pytest.raises(ValueError, match=re.escape("out[1] and scores share memory")):
+        train._apart({"out[0]": torch.zeros(3), "out[1]": buffer}, {"label": None, "scores": buffer})
+    with pytest.raises(ValueError, match=re.escape("out[0] and out[1] share memory")):
+        train._apart({"out[0]": buffer[0], "out[1]": buffer}, {})
+
+
+def test_an_optimizer_is_not_copied():
+    """It holds addresses: a copy's would be those of the tensors copied from."""
+    opt = train.AdamW.__new__(train.AdamW)
+    for call in (copy.copy, copy.deepcopy, pickle.dumps):
+        with pytest.raises(TypeError, match="load_state"):
+            call(opt)
+    for name in ("params", "grads", "m", "v", "device"):
+        with pytest.raises(AttributeError):
+            setattr(opt, name, None)
+
+
+@pytest.mark.parametrize("change, error, message", [
+    (dict(bits=np.zeros((6, 16), np.uint8)), TypeError, "bits is uint8"),
+    (dict(bits=torch.zeros(6, dtype=torch.int32)), ValueError, "bits has 1 dimensions"),
+    (dict(bits=rows(0)), ValueError, "no rows"),
+    (dict(k=0), ValueError, "no classifiers (0)"),
+    (dict(n_features=0), ValueError, "no features (0)"),
+    (dict(label=np.zeros(6)), TypeError, "label is torch.float64"),
+    (dict(label=np.zeros(7, int)), ValueError, "label has shape (7,)"),
+    (dict(weight=np.ones(7)), ValueError, "weight has shape (7,)"),
+    (dict(batch=0), ValueError, "batch = 0"),
+    (dict(), ValueError, "on cpu"),
+])
+def test_fit_siblings_refusals(change, error, message):
+    with pytest.raises(error, match=re.escape(message)):
+        train.fit_siblings(**{**dict(bits=rows(), label=np.zeros(6, int), k=2, n_features=100), **change})
