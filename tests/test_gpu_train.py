@@ -581,6 +581,14 @@ def test_adamw_refuses_shared_memory():
         opt.load_state(0, opt.m[:100], opt.v)
 
 
+def test_an_empty_batch_of_a_large_table():
+    """More values than a launch has threads: a gradient of nothing is zeros everywhere."""
+    bits = torch.zeros((0, 2188), dtype=torch.int32, device=DEV)
+    out = torch.empty((70_000, 65_536), device=DEV).fill_(7.0), torch.full((65_536,), 7.0, device=DEV)
+    train.row_scores_grad(bits, torch.zeros((0, 65_536), device=DEV), 70_000, out=out)
+    assert not any(bool(out[0][i:i + 7_000].any()) for i in range(0, 70_000, 7_000)) and not out[1].any()
+
+
 def test_outputs_over_inputs_are_refused():
     bits, _ = packed(np.random.default_rng(0), 50, 300)
     buffer = torch.zeros(400, 40, device=DEV)
