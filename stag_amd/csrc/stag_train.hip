@@ -58,9 +58,9 @@ __device__ __forceinline__ const uint32_t *row_of(const uint32_t *bits, int64_t 
 // in 16 bits; a 32-bit coefficient is cut into three bf16 pieces of 8 bits each, which together are the coefficient,
 // and multiplied piece by piece into the same 32-bit sums.  16-bit coefficients go in as they are.
 //
-// What bounds them: the matrix cores for 32-bit coefficients (8,192 rows x 7,500 features x 1,000 columns: 237 us, 1.6 PFLOP/s of bf16
+// What bounds them: the matrix cores for 32-bit coefficients (8,192 rows x 7,500 features x 1,000 columns: 222 us, 1.7 PFLOP/s of bf16
 // operations counted densely; a library's bf16 product of 8,192^3 reaches 1.19 on the same card), the making of operands
-// beside them for 16-bit ones (that size's gradient in bf16: 119 us, 1.06 PFLOP/s), latency for one node's batch (4,096 x
+// beside them for 16-bit ones (that size's gradient in bf16: 108 us, 1.2 PFLOP/s), latency for one node's batch (4,096 x
 // 7,500 x 13: 10 us and 3 for adding up its parts).
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
@@ -109,6 +109,7 @@ template <typename raw_t> __device__ __forceinline__ uint32_t load_raw(__amdgpu_
         return __builtin_amdgcn_raw_buffer_load_b16(from, at, 0, 0);
 }
 
+__device__ __forceinline__ uint32_t low_halves(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x05040100u); }
 __device__ __forceinline__ uint32_t high_halves(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
 
 // the 8 operands of K-step part s: bits 4s .. 4s+3 and 4s+16 .. 4s+19 of x, as 2.0 or 0
@@ -154,23 +155,29 @@ constexpr int NOTES = 1024;      // groups of U K-steps
 // Why these tiles: 2 x 2 tiles a wave make 8 (or 24) matrix instructions of the 4 (or 6) operands loaded from LDS and two made
 // from bits, and 8 waves share what the workgroup cuts, at two waves a SIMD (150 to 190 registers).  Measured at the level's size, scores in
 // 32 bits and gradient in bf16, in us: 4 waves of 4 x 2 tiles with the sum in two parts 273 and 157; 8 of 2 x 2, one K-step a barrier 290
-// and 164, two 275 and 142, four 260 and 135; two buffers in LDS instead of one gained nothing.  One tile a wave where there are few.
-template <int TYPE, Source SRC, int MT, int NT>
+// and 164, two 275 and 142, four 260 and 135.  Then: operands, bits and loads in turns with the matrix instructions (in_turns) and WIDE
+// loads 242 -> 222 and 121 -> 108; what is left of it without the coefficients' way into LDS is 199 and 94.  Two buffers in LDS and one
+// barrier, with half of the waves cutting coefficients while the others multiply: 235 and 113, the matrix cores then run slower.
+// One tile a wave where there are few.
+//
+// WIDE: rows of coefficients that all begin at a multiple of 16 bytes (32-bit ones) or 8 are loaded four columns at a time.
+template <int TYPE, Source SRC, int MT, int NT, bool WIDE>
 __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
     typedef typename Raw<TYPE>::type raw_t;
     constexpr bool GRAD = SRC != ROWS;
     constexpr int P = TYPE == STAG_F32 ? 3 : 1, COLS = 32 * NT, U = SRC == TURN ? 2 : 4;
     // a thread's share of the 8 x COLS groups of 8 terms of U K-steps; PASSES of them are of one K-step
     constexpr int ITEMS = U * 8 * COLS / (64 * W), PASSES = 8 * COLS > 64 * W ? 8 * COLS / (64 * W) : 1;
-    static_assert(ITEMS >= 1, "a group for every thread");
+    static_assert(ITEMS >= 1 && (!WIDE || ITEMS == 4), "a group for every thread, or one of four columns");
+    constexpr int QUADS = COLS / 4, SUMS = WIDE ? 4 : 1;
     typedef __attribute__((ext_vector_type(MT))) uint32_t words_t;          // TURN: a lane loads the words of its wave's row tiles at once
     __shared__ u32x4 lds[U][P][8][COLS];
-    __shared__ float sums[GRAD ? 64 * W : 1];
+    __shared__ float sums[GRAD ? 64 * W * SUMS : 1];
     __shared__ int note[NOTES], noted, met, bad;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int64_t tile0 = ((int64_t)blockIdx.x * W + wave) * MT;           // this wave's first row tile
     const int64_t out_rows = GRAD ? a.n_features : a.m;
-    const int col = threadIdx.x % COLS, c0 = blockIdx.y * COLS, c = c0 + col;
+    const int col = WIDE ? 4 * (threadIdx.x % QUADS) : threadIdx.x % COLS, c0 = blockIdx.y * COLS, c = c0 + col;
     const bool c_ok = c < a.k;
     const int64_t limit = GRAD ? a.m : a.n_features;                       // terms of the sum
     constexpr int UNIT = SRC == TURN ? 1 : 4;                              // K-steps of a step of the plan
@@ -184,16 +191,18 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
     };
 
     f32x16 acc[MT][NT];
-    float column_sum;
+    float column_sum[SUMS];
     // An infinity or NaN that met a zero bit has made NaN of a sum that it has no part in.  If a sum is not finite after the first
     // sweep, a second one takes such coefficients for zeros and notes the K-steps that have them; they are added afterwards to
     // the sums whose rows have the bit.
     if (threadIdx.x == 0) noted = met = bad = 0;
 
-    // Buffer loads: one 32-bit offset a lane, and what lies behind the last term or column reads as zero.
-    uint32_t b[ITEMS][8];
-    auto step_of = [&](int i) { return PASSES * 64 * W == 8 * COLS ? i / PASSES : (i * 64 * W + wave * 64) / (8 * COLS); };      // the same for a whole wave
-    auto group_of = [&](int i) -> int { return (i * 64 * W + threadIdx.x) % (8 * COLS) / COLS; };
+    // Buffer loads: one 32-bit offset a lane, and what lies behind the last term or column reads as zero.  A thread's items: its
+    // column in ITEMS groups of terms, or (WIDE) four columns in one group, as they lie in memory.
+    constexpr int WORDS = WIDE && TYPE != STAG_F32 ? 2 : 4;
+    uint32_t b[WIDE ? 8 : ITEMS][WIDE ? WORDS : 8];
+    auto step_of = [&](int i) { return WIDE ? wave * 64 / (8 * QUADS) : PASSES * 64 * W == 8 * COLS ? i / PASSES : (i * 64 * W + wave * 64) / (8 * COLS); };      // the same for a whole wave
+    auto group_of = [&](int i) -> int { return WIDE ? threadIdx.x % (8 * QUADS) / QUADS : (i * 64 * W + threadIdx.x) % (8 * COLS) / COLS; };
     uint32_t at_b[PASSES];
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
@@ -201,50 +210,99 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
         at_b[i] = c_ok ? (uint32_t)((r0 * (int)a.mat_stride + c) * (int)sizeof(raw_t)) : NOWHERE;
     }
     const uint32_t row_b = (uint32_t)a.mat_stride * sizeof(raw_t);
-    auto load_b = [&](int ks) {
+    auto load_b = [&](int ks, bool there = true) {
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
+        for (int i = 0; i < (WIDE ? 1 : ITEMS); ++i) {
             const int64_t t0 = term(ks + step_of(i), 0);
-            const auto from = buffer((const raw_t *)a.mat + t0 * a.mat_stride, (limit - t0) * row_b);
+            const auto from = buffer((const raw_t *)a.mat + t0 * a.mat_stride, there ? (limit - t0) * row_b : 0);
 #pragma unroll
-            for (int q = 0; q < 8; ++q) b[i][q] = load_raw<raw_t>(from, at_b[i % PASSES] + ((q >> 1) + 16 * (q & 1)) * row_b);
+            for (int q = 0; q < 8; ++q) {
+                const uint32_t at = at_b[i % PASSES] + ((q >> 1) + 16 * (q & 1)) * row_b;
+                if constexpr (!WIDE) {
+                    b[i][q] = load_raw<raw_t>(from, at);
+                } else if constexpr (TYPE == STAG_F32) {
+                    const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0);
+                    b[q][0] = v[0], b[q][1] = v[1], b[q][2] = v[2], b[q][3] = v[3];
+                } else {
+                    const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(from, at, 0, 0);
+                    b[q][0] = v[0], b[q][1] = v[1];
+                }
+            }
         }
     };
+    // term q of item i, as its type's bits
+    auto raw_of = [&](int i, int q) -> uint32_t {
+        if constexpr (!WIDE) return b[i][q];
+        if constexpr (TYPE == STAG_F32) return b[q][i];
+        return i & 1 ? b[q][i >> 1] >> 16 : b[q][i >> 1] & 0xffffu;
+    };
+    auto clear = [&](int i, int q) {
+        if constexpr (!WIDE)
+            b[i][q] = 0;
+        else if constexpr (TYPE == STAG_F32)
+            b[q][i] = 0;
+        else
+            b[q][i >> 1] &= i & 1 ? 0xffffu : 0xffff0000u;
+    };
+    // Where a column's operands lie among the COLS of LDS: turned a little, so that neither four columns a thread nor one meet in a bank
+    auto place = [](int col) { return (col & ~7) | ((col + (col >> 3)) & 7); };
     // `real_at`: which of a K-step's rows are no padding (GRAD); the others are zeros, whatever the memory holds
     auto store_b = [&](auto careful, auto real_at) {
+        if constexpr (WIDE && GRAD) {
+            const uint64_t real = a.rows ? real_at(0) : ~0ull;
+            if (real != ~0ull) {
+                const uint32_t there = (uint32_t)(real >> (32 * (group_of(0) & 1) + 4 * (group_of(0) >> 1)));
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (!(there >> ((q >> 1) + 16 * (q & 1)) & 1u)) {
+#pragma unroll
+                        for (int j = 0; j < WORDS; ++j) b[q][j] = 0;
+                    }
+            }
+        }
+        if constexpr (WIDE) {
+            if (c + 4 > a.k) {      // what lies behind the last column
+#pragma unroll
+                for (int i = 1; i < ITEMS; ++i)
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        if (c + i >= a.k) clear(i, q);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             const int u = step_of(i), g = group_of(i);
-            uint32_t(&v)[8] = b[i];
-            if constexpr (GRAD) {
+            if constexpr (GRAD && !WIDE) {
                 const uint64_t real = SRC == TURN || a.rows ? real_at(u) : ~0ull;      // TURN: a part may end inside the U K-steps
                 if (real != ~0ull) {
                     const uint32_t there = (uint32_t)(real >> (32 * (g & 1) + 4 * (g >> 1)));
 #pragma unroll
                     for (int q = 0; q < 8; ++q)
-                        if (!(there >> ((q >> 1) + 16 * (q & 1)) & 1u)) v[q] = 0;
+                        if (!(there >> ((q >> 1) + 16 * (q & 1)) & 1u)) clear(i, q);
                 }
             }
             if constexpr (GRAD) {
                 if (blockIdx.x == 0) {
                     float s = 0.f;
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) s += value_of<TYPE>(v[q]);
-                    column_sum += s;
+                    for (int q = 0; q < 8; ++q) s += value_of<TYPE>(raw_of(i, q));
+                    column_sum[WIDE ? i : 0] += s;
                 }
             }
             if constexpr (careful.value) {
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
-                    if (not_finite<TYPE>(v[q])) {
+                    if (not_finite<TYPE>(raw_of(i, q))) {
                         met = 1;
-                        v[q] = 0;
+                        clear(i, q);
                     }
             }
+            const int to = place(WIDE ? col + i : col);
             if constexpr (TYPE == STAG_F32) {
-                uint32_t y[8], z[8];
+                uint32_t v[8], y[8], z[8];
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
+                    v[q] = raw_of(i, q);
                     const float left = __uint_as_float(v[q]) - __uint_as_float(v[q] & 0xffff0000u);        // exact: the low 16 bits
                     y[q] = __float_as_uint(left);
                     z[q] = __float_as_uint(left - __uint_as_float(y[q] & 0xffff0000u));                    // exact: the low 8 bits
@@ -256,22 +314,30 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
                     p1[j] = high_halves(y[2 * j], y[2 * j + 1]);
                     p2[j] = high_halves(z[2 * j], z[2 * j + 1]);
                 }
-                lds[u][0][g][col] = p0;
-                lds[u][P > 1 ? 1 : 0][g][col] = p1;
-                lds[u][P > 2 ? 2 : 0][g][col] = p2;
+                lds[u][0][g][to] = p0;
+                lds[u][P > 1 ? 1 : 0][g][to] = p1;
+                lds[u][P > 2 ? 2 : 0][g][to] = p2;
             } else {
                 u32x4 p0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    // Kept in registers of their own up to here: a load into the upper half of one that another load is to fill waits
-                    // for that load, and 32 loads one after the other took 236 us where these take 130.
-                    asm("" : "+v"(v[2 * j]), "+v"(v[2 * j + 1]));
-                    p0[j] = v[2 * j] | v[2 * j + 1] << 16;
+                    if constexpr (WIDE) {
+                        const uint32_t lo = b[2 * j][i >> 1], hi = b[2 * j + 1][i >> 1];
+                        p0[j] = i & 1 ? high_halves(lo, hi) : low_halves(lo, hi);
+                    } else {
+                        // Kept in registers of their own up to here: a load into the upper half of one that another load is to fill waits
+                        // for that load, and 32 loads one after the other took 236 us where these take 130.
+                        asm("" : "+v"(b[i][2 * j]), "+v"(b[i][2 * j + 1]));
+                        p0[j] = b[i][2 * j] | b[i][2 * j + 1] << 16;
+                    }
                 }
-                lds[u][0][g][col] = p0;
+                lds[u][0][g][to] = p0;
             }
         }
     };
+    int operand_at[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) operand_at[n] = place(32 * n + (lane & 31));
     auto multiply = [&](int u, const uint32_t *x) {
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
@@ -282,7 +348,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
             for (int p = P - 1; p >= 0; --p)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const u32x4 v = lds[u][p][2 * s + half][32 * n + (lane & 31)];
+                    const u32x4 v = lds[u][p][2 * s + half][operand_at[n]];
 #pragma unroll
                     for (int t = 0; t < MT; ++t) {
                         if constexpr (TYPE == STAG_F16)
@@ -294,8 +360,24 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
         }
     };
 
+    // The order that keeps the matrix cores fed: operands leave LDS AHEAD turns before their own, those of the bits are made and
+    // the next coefficients asked for in between.  Left to itself the compiler loads an operand where it is needed and waits.
+    auto in_turns = [&] {
+        constexpr int READS = U * 4 * P * NT, AHEAD = P == 1 ? 2 : 3;
+        __builtin_amdgcn_sched_group_barrier(0x2, 8 * MT, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+        for (int r = 0; r < READS; ++r) {
+            __builtin_amdgcn_sched_group_barrier(0x8, MT, 0);
+            if (r < READS - AHEAD) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x2, (8 * MT + P * NT - 1) / (P * NT) + 1, 0);
+            if (r % 3 == 0) __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
+        }
+    };
+
     auto sweep = [&](auto careful) -> bool {
-        column_sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < SUMS; ++i) column_sum[i] = 0.f;
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -326,14 +408,14 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
             auto load_real = [&](int sb) {
                 if constexpr (SRC == TURNED) {
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) real[q] = valid[sb * 8 + q];
+                    for (int q = 0; q < (WIDE ? 2 : 8); ++q) real[q] = valid[sb * 8 + (WIDE ? 4 * q + step_of(0) : q)];
                 }
             };
             auto real_at = [&](int u) -> uint64_t {
                 if constexpr (SRC != TURNED) return ~0ull;
-                uint32_t lo = real[0], hi = real[4];
+                uint32_t lo = real[0], hi = real[WIDE ? 1 : 4];
 #pragma unroll
-                for (int i = 1; i < U; ++i) lo = u == i ? real[i] : lo, hi = u == i ? real[4 + i] : hi;
+                for (int i = 1; i < (WIDE ? 1 : U); ++i) lo = u == i ? real[i] : lo, hi = u == i ? real[4 + i] : hi;
                 return (uint32_t)__builtin_amdgcn_readfirstlane(lo) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(hi) << 32;
             };
             u32x4 x[MT], next[MT];
@@ -353,8 +435,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
                 if (more) {
                     load_x((ks + U) >> 2, next);
                     load_real((ks + U) >> 2);
-                    load_b(ks + U);
                 }
+                load_b(ks + U, more);
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     uint32_t w[MT];
@@ -362,6 +444,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
                     for (int t = 0; t < MT; ++t) w[t] = x[t][u];
                     multiply(u, w);
                 }
+                in_turns();
                 __syncthreads();
 #pragma unroll
                 for (int t = 0; t < MT; ++t) x[t] = next[t];
@@ -493,16 +576,18 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
     }
     if constexpr (GRAD) {
         if (blockIdx.x == 0) {
-            sums[threadIdx.x] = column_sum;
+#pragma unroll
+            for (int i = 0; i < SUMS; ++i) sums[threadIdx.x * SUMS + i] = column_sum[i];
             __syncthreads();
-            if (threadIdx.x < COLS && c_ok) {
+            const int cc = c0 + threadIdx.x;
+            if (threadIdx.x < COLS && cc < a.k) {
                 float s = 0.f;
 #pragma unroll
-                for (int g = 0; g < 64 * W / COLS; ++g) s += sums[g * COLS + col];
+                for (int g = 0; g < 64 * W * SUMS / COLS; ++g) s += sums[g * COLS + threadIdx.x];
                 if (!whole)
-                    a.part[(int64_t)gridDim.z * out_rows * a.k + (int64_t)blockIdx.z * a.k + c] = s;
+                    a.part[(int64_t)gridDim.z * out_rows * a.k + (int64_t)blockIdx.z * a.k + cc] = s;
                 else if (a.bias_out)
-                    a.bias_out[c] = s;
+                    a.bias_out[cc] = s;
             }
         }
     }
@@ -1242,8 +1327,8 @@ Plan product_plan(bool grad, int64_t m, int32_t n_features, int32_t k, int type)
     p.mt = p.src == TURNED || (p.src == ROWS && p.nt == 2 && m > 512) ? 2 : 1;
     p.row_blocks = ceil_div(p.out_rows, 32 * W * p.mt);
     p.steps = (int)(p.src == ROWS ? ceil_div(n_features, 256) : p.src == TURN ? ceil_div(m, 64) : ceil_div(m, 256));
-    const int step = type == STAG_F32 ? (p.src == TURN ? (p.nt == 2 ? 1100 : 800) : p.nt == 1 ? 2200 : p.mt == 1 ? 4500 : 8500)
-                                      : (p.src == TURN ? (p.nt == 2 ? 700 : 500) : p.nt == 1 ? 1300 : p.mt == 1 ? 2200 : 3800);
+    const int step = type == STAG_F32 ? (p.src == TURN ? (p.nt == 2 ? 1100 : 800) : p.nt == 1 ? 2200 : p.mt == 1 ? 4300 : 7600)
+                                      : (p.src == TURN ? (p.nt == 2 ? 700 : 500) : p.nt == 1 ? 1300 : p.mt == 1 ? 2200 : 3300);
     const int64_t parts = best_parts(p.row_blocks * p.col_blocks, p.steps, step, p.src == TURN || p.nt == 1, p.out_rows * k);
     p.per_part = (int)ceil_div(p.steps, parts);
     p.parts = (int)ceil_div(p.steps, p.per_part);
@@ -1251,11 +1336,11 @@ Plan product_plan(bool grad, int64_t m, int32_t n_features, int32_t k, int type)
     return p;
 }
 
-// launches k_product<TYPE, SRC, MT, NT> if that is what the plan says
-template <int TYPE, Source SRC, int MT, int NT>
+// launches k_product<TYPE, SRC, MT, NT, WIDE> if that is what the plan says and the coefficients lie so
+template <int TYPE, Source SRC, int MT, int NT, bool WIDE>
 bool launched(const Plan &p, const ProductArgs &a, hipStream_t st) {
-    if (p.src != SRC || p.mt != MT || p.nt != NT) return false;
-    k_product<TYPE, SRC, MT, NT><<<dim3((unsigned)p.row_blocks, (unsigned)p.col_blocks, (unsigned)p.parts), 64 * W, 0, st>>>(a);
+    if (p.src != SRC || p.mt != MT || p.nt != NT || (WIDE && (a.mat_stride % 4 || !aligned(a.mat, 4 * type_bytes(TYPE))))) return false;
+    k_product<TYPE, SRC, MT, NT, WIDE><<<dim3((unsigned)p.row_blocks, (unsigned)p.col_blocks, (unsigned)p.parts), 64 * W, 0, st>>>(a);
     return true;
 }
 
@@ -1277,9 +1362,11 @@ int product(const Plan &p, ProductArgs a, void *work, hipStream_t st) {
                 REQUIRE(turns * 256 < MAX_THREADS, "%lld rows of %d features are too many", (long long)a.m, a.n_features);
                 k_turn<<<(unsigned)turns, 256, 0, st>>>(a, (uint32_t *)work, row_words, (int)word_blocks);
             }
-            done = launched<TYPE, TURNED, 2, 2>(p, a, st) || launched<TYPE, TURN, 1, 2>(p, a, st) || launched<TYPE, TURN, 1, 1>(p, a, st);
+            done = launched<TYPE, TURNED, 2, 2, true>(p, a, st) || launched<TYPE, TURNED, 2, 2, false>(p, a, st) || launched<TYPE, TURN, 1, 2, false>(p, a, st) ||
+                   launched<TYPE, TURN, 1, 1, false>(p, a, st);
         } else {
-            done = launched<TYPE, ROWS, 2, 2>(p, a, st) || launched<TYPE, ROWS, 1, 2>(p, a, st) || launched<TYPE, ROWS, 1, 1>(p, a, st);
+            done = launched<TYPE, ROWS, 2, 2, true>(p, a, st) || launched<TYPE, ROWS, 2, 2, false>(p, a, st) || launched<TYPE, ROWS, 1, 2, false>(p, a, st) ||
+                   launched<TYPE, ROWS, 1, 1, false>(p, a, st);
         }
         REQUIRE(done, "no kernel for %d x %d tiles", p.mt, p.nt);
         HIP_TRY(hipGetLastError());

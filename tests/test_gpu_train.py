@@ -279,6 +279,36 @@ def test_strided_tables_and_outputs(n, k):
     near(train.row_scores_grad(bits, one, n_features)[0].cpu(), x.T @ one.double().cpu().numpy(), (x.sum(0)[:, None] + 4) * U * x.sum(0)[:, None] * 5)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n, k, n_features", [(530, 66, 400), (600, 129, 300), (4200, 197, 2200)])
+@pytest.mark.parametrize("left, right", [(4, 4), (0, 0), (1, 2), (8, 5)])
+def test_values_between_the_rows_are_not_read(n, k, n_features, left, right, dtype):
+    """Tables and gradients inside larger buffers of NaN, at columns that fit wide loads and at others, with widths that end inside one; an infinity of
+    their own in the last column goes where it belongs."""
+    rng = np.random.default_rng(k)
+    width = -(-(left + k) // 4) * 4 + (right if right else 0) if right != 0 else left + k
+    bits, x = packed(rng, n, n_features)
+
+    def inside(rows):
+        big = torch.full((rows + 1, width), math.nan, device=DEV).to(dtype)
+        big[:rows, left:left + k] = torch.from_numpy(rng.normal(size=(rows, k)).astype(np.float32))
+        return big[:rows, left:left + k]
+
+    table, grad = inside(n_features), inside(n)
+    t, g = table.double().cpu().numpy(), grad.double().cpu().numpy()
+    near(train.row_scores(bits, table).cpu(), x @ t, (x.sum(1)[:, None] + 4) * U * (x @ np.abs(t)))
+    table_grad, bias_grad = train.row_scores_grad(bits, grad, n_features)
+    near(table_grad.cpu(), x.T @ g, (x.sum(0)[:, None] + 4) * U * (x.T @ np.abs(g)))
+    near(bias_grad.cpu(), g.sum(0), (n + 4) * U * np.abs(g).sum(0))
+    table[n_features - 1, k - 1] = math.inf
+    has = x[:, n_features - 1] > 0
+    got = train.row_scores(bits, table).double().cpu().numpy()
+    assert np.isinf(got[has, k - 1]).all()
+    t[n_features - 1, k - 1] = 0.0
+    got[has, k - 1] = (x @ t)[has, k - 1]
+    near(got, x @ t, (x.sum(1)[:, None] + 4) * U * (x @ np.abs(t)))
+
+
 def test_empty_batches():
     bits, _ = packed(np.random.default_rng(0), 5, 40)
     none = torch.empty(0, dtype=torch.int32, device=DEV)
