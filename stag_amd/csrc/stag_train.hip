@@ -1280,8 +1280,8 @@ struct Plan {
 
 // In how many parts the sum is cut, so that few result tiles still fill the card: of 1, 2, 3, 4, 6, 8, 12 .. 256 and those that fill it once,
 // the one whose time is the least by what was measured on the card, in ns -- `step` for each step of a workgroup that has its CU to
-// itself, half as much again where two share one (`shared`: they fit), and for more than one part 3,000 and the parts'
-// sums once out and once in at 4 TB/s.
+// itself, half as much again where two share one (`shared`: they fit), and for more than one part 5,000 for the second launch and the parts'
+// sums once out and once in at 4 TB/s.  (628 small and medium sizes: 3,000 instead 1.1 % slower on the mean, up to 4 us a pass; 7,000 0.4 %, up to 14.)
 struct Cut {
     int parts;
     double time;
@@ -1293,7 +1293,7 @@ Cut best_cut(int64_t blocks, int steps, int step, bool shared, int64_t values) {
         const int per = (steps + parts - 1) / parts;
         const double all = (double)blocks * ((steps + per - 1) / per);
         const double load = !shared ? std::ceil(all / 256) : all <= 256 ? 1.0 : 1.5 * std::ceil(all / 512);
-        const double time = per * (double)step * load + (parts > 1 ? 3000.0 + 8.0 * parts * (double)values / 4000.0 : 0.0);
+        const double time = per * (double)step * load + (parts > 1 ? 5000.0 + 8.0 * parts * (double)values / 4000.0 : 0.0);
         if (parts == 1 || time < best.time) best = {parts, time};
     };
     for (int parts = 1; parts <= 256; parts *= 2) {
@@ -1316,9 +1316,9 @@ Plan product_plan(bool grad, int64_t m, int32_t n_features, int32_t k, int type)
     if (p.lookup) return p;
     p.nt = k <= 32 ? 1 : 2;
     p.col_blocks = ceil_div(k, 32 * p.nt);
-    // Turning the bits beforehand pays when many column blocks would each turn them (7,500 features; 4,096 rows: 200 columns 53
-    // against 56 us, 1,000 columns 146 against 172, in bf16 73 against 102; 1,024 rows, 1,000 columns 47 against 49, 400 columns
-    // 38 against 36; 500 features, 4,096 rows, 1,000 columns 31 against 27)
+    // Turning the bits beforehand pays when many column blocks would each turn them (us beforehand against as they go, 32 bits and 7,500
+    // features: 3,000 rows x 400 columns 65 against 76, x 200 43 against 42, 1,800 x 1,000 75 against 81, 1,100 x 400 43 against 32; bf16 and
+    // 2,500 features: 3,000 x 1,000 36 against 52, x 400 26 against 26, x 200 24 against 20; 750 features, 5,000 x 1,000: 30 against 29)
     p.src = !grad ? ROWS : k > 128 && n_features >= 2048 && m * k >= 800000 ? TURNED : TURN;
     if (p.src == TURNED) {
         p.turned_words = 8 * ceil_div(m, 256);
