@@ -630,6 +630,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
 // The batch's bits by feature: turned[f][w], w < words = 8 * ceil(m / 256), with the words in the order in which k_product
 // takes them: word 8 s + 4 h + q holds batch rows 64 (4 s + q) + 32 h + (0..31).  Row n_features says which batch rows are no padding.
 // A wave turns 256 rows by 4 words of features; a lane loads 16 bytes of four rows and stores 16 bytes of four features.
+// 32 x 32 bits are turned in five exchanges between lanes.  8,192 rows of 7,500 features: 8 us, 1.9 TB/s in and out; latency bounds it.
 __global__ __launch_bounds__(256) void k_turn(ProductArgs a, uint32_t *turned, int row_words, int word_blocks) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int64_t s = blockIdx.x / word_blocks;
@@ -684,7 +685,8 @@ __global__ __launch_bounds__(256) void k_join(ProductArgs a, int parts, int64_t 
 }
 
 // Few rows: the lookups themselves.  A workgroup makes one row of scores, `cw` columns of it (a power of two up to 64): it
-// lists the row's tokens in LDS, 256 words at a time, and its 1024 / cw column groups take the tokens in turn.
+// lists the row's tokens in LDS, 256 words at a time, and its 1024 / cw column groups take the tokens in turn, four loads in flight.
+// Latency bounds it: the row, the list, the loads and the halving of the groups' sums take 4.2 us for a row of 7,500 features and 8 columns.
 constexpr int LOOKUP_WORDS = 256;
 template <typename T>
 __global__ __launch_bounds__(1024) void k_lookup(ProductArgs a, int cw_log) {
@@ -790,9 +792,25 @@ __device__ __forceinline__ void loss_of(float z, bool positive, float w, float &
     slope = positive ? -p : p;
 }
 
+// part[cv] = the sums of the rp threads of column cv, by halves (a single column's 1,024 one after the other took 6 us)
+template <int V> __device__ __forceinline__ void add_rows(float *part, const float *sum, int r, int rp, int cv, int ct) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) part[threadIdx.x * V + j] = sum[j];
+    for (int n = rp; n > 1;) {
+        const int half = (n + 1) / 2;
+        __syncthreads();
+        if (r + half < n) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) part[threadIdx.x * V + j] += part[(threadIdx.x + half * ct) * V + j];
+        }
+        n = half;
+    }
+}
+
 // A thread owns V neighbouring columns and goes down the rows of its workgroup, four at a time so that their loads are in
 // flight together; loss sums stay in its registers until the workgroup adds them up in a fixed order and stores one
-// partial row of K sums.  Scores are read only where the row trains.
+// partial row of K sums.  Scores are read only where the row trains.  Every score is read and every gradient written once: HBM bounds large
+// ones, the launch small ones (300 x 8 in 4.7 us).
 template <typename T, int V, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_loss(LossArgs a) {
     const float *const scores = a.scores, *const weight = a.weight;
@@ -859,15 +877,10 @@ __global__ __launch_bounds__(THREADS) void k_loss(LossArgs a) {
         }
     }
     if (!loss) return;
-#pragma unroll
-    for (int j = 0; j < V; ++j) part[threadIdx.x * V + j] = sum[j];
-    __syncthreads();
+    add_rows<V>(part, sum, r, rp, cv, ct);
     if (r == 0 && c0 < k) {
-        for (int j = 0; j < V; ++j) {
-            float s = 0.f;
-            for (int q = 0; q < rp; ++q) s += part[(q * ct + cv) * V + j];
-            loss[(int64_t)blockIdx.x * k + c0 + j] = s;
-        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) loss[(int64_t)blockIdx.x * k + c0 + j] = part[cv * V + j];
     }
 }
 
@@ -943,19 +956,14 @@ __global__ __launch_bounds__(256) void k_loss_siblings(LossArgs a) {
         __syncthreads();
     }
     if (!loss) return;
-#pragma unroll
-    for (int j = 0; j < V; ++j) part[threadIdx.x * V + j] = sum[j];
-    __syncthreads();
+    add_rows<V>(part, sum, r, rp, cv, ct);
     if (r == 0 && c0 < k) {
-        for (int j = 0; j < V; ++j) {
-            float s = 0.f;
-            for (int q = 0; q < rp; ++q) s += part[(q * ct + cv) * V + j];
-            loss[(int64_t)blockIdx.x * k + c0 + j] = s;
-        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) loss[(int64_t)blockIdx.x * k + c0 + j] = part[cv * V + j];
     }
 }
 
-// adds up the partial rows: 32 columns a workgroup, every 32nd row to a thread, then the 32 sums in order
+// adds up the partial rows: 32 columns a workgroup, every 32nd row to a thread, then the 32 sums in order (1,024 rows of 1,000: 4.4 us)
 __global__ __launch_bounds__(1024) void k_loss_join(const float *part, int n_parts, int k, float *loss) {
     __shared__ double sums[32][33];
     const int col = threadIdx.x & 31, g = threadIdx.x >> 5, c = blockIdx.x * 32 + col;
@@ -1105,7 +1113,8 @@ __device__ __forceinline__ void unpack_e4m3(uint32_t q, float *x) {
 }
 
 // A wave takes a tile of four blocks of 256 values, four neighbouring values a lane, and has the loads of GROUP blocks in
-// flight before it computes.  Everything is read once and written once; what bounds it is HBM.  m, v and the root are rounded after
+// flight before it computes.  Everything is read once and written once; what bounds it with 32-bit states is HBM (the 54 million
+// values of 1,600 tables in 32 bits, 1.5 GB: 266 us, 5.7 TB/s), with 8-bit ones the 30 instructions a value (as bf16: 142 us, 3.8 TB/s).  m, v and the root are rounded after
 // every operation (no fused multiply-add), so that the 8-bit codes are a function of the inputs that any other 32-bit
 // implementation can restate.
 template <int BITS>
