@@ -82,6 +82,7 @@ struct ProductArgs {
     const uint32_t *turned;     // TURNED: the bits by feature, see k_turn
     float *part;                // more than one part: their sums [parts][result rows][k], then column sums [parts][k]
     int32_t n_features, words, k;       // words of a row of bits (TURNED: of a turned row)
+    int32_t row_blocks, col_blocks, parts;
     int32_t steps, steps_per_part;      // in units of 4 K-steps (TURN: of 1)
     float scale;
 };
@@ -174,14 +175,19 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
     __shared__ u32x4 lds[U][P][8][COLS];
     __shared__ float sums[GRAD ? 64 * W * SUMS : 1];
     __shared__ int note[NOTES], noted, met, bad;
+    // Workgroups go round the card's 8 dies in turn; each die is given neighbours in row blocks of the same columns and terms, which share the
+    // coefficients in its L2.
+    const int per_die = gridDim.x / 8, tile = (int)(blockIdx.x % 8) * per_die + (int)(blockIdx.x / 8);
+    if (tile >= a.row_blocks * a.col_blocks * a.parts) return;
+    const int block_x = tile % a.row_blocks, block_y = tile / a.row_blocks % a.col_blocks, block_z = tile / a.row_blocks / a.col_blocks;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int64_t tile0 = ((int64_t)blockIdx.x * W + wave) * MT;           // this wave's first row tile
+    const int64_t tile0 = ((int64_t)block_x * W + wave) * MT;           // this wave's first row tile
     const int64_t out_rows = GRAD ? a.n_features : a.m;
-    const int col = WIDE ? 4 * (threadIdx.x % QUADS) : threadIdx.x % COLS, c0 = blockIdx.y * COLS, c = c0 + col;
+    const int col = WIDE ? 4 * (threadIdx.x % QUADS) : threadIdx.x % COLS, c0 = block_y * COLS, c = c0 + col;
     const bool c_ok = c < a.k;
     const int64_t limit = GRAD ? a.m : a.n_features;                       // terms of the sum
     constexpr int UNIT = SRC == TURN ? 1 : 4;                              // K-steps of a step of the plan
-    const int first = blockIdx.z * a.steps_per_part * UNIT, last = min((int)(blockIdx.z + 1) * a.steps_per_part, a.steps) * UNIT;
+    const int first = block_z * a.steps_per_part * UNIT, last = min((int)(block_z + 1) * a.steps_per_part, a.steps) * UNIT;
     uint32_t padding[MT] = {}, any_padding = 0;                             // ROWS: which rows of a tile are padding
 
     // the term that stands at place r (0..63) of K-step ks
@@ -282,7 +288,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
                 }
             }
             if constexpr (GRAD) {
-                if (blockIdx.x == 0) {
+                if (block_x == 0) {
                     float s = 0.f;
 #pragma unroll
                     for (int q = 0; q < 8; ++q) s += value_of<TYPE>(raw_of(i, q));
@@ -546,8 +552,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
             }
     }
 
-    const bool whole = gridDim.z == 1;
-    float *to = whole ? a.out : a.part + (int64_t)blockIdx.z * out_rows * a.k;
+    const bool whole = a.parts == 1;
+    float *to = whole ? a.out : a.part + (int64_t)block_z * out_rows * a.k;
     const int64_t stride = whole ? a.out_stride : a.k;
     const float scale = whole ? 0.5f * a.scale : 0.5f;
     const auto into = buffer(to + tile0 * 32 * stride, to ? (out_rows - tile0 * 32) * stride * 4 : 0);
@@ -575,7 +581,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
         }
     }
     if constexpr (GRAD) {
-        if (blockIdx.x == 0) {
+        if (block_x == 0) {
 #pragma unroll
             for (int i = 0; i < SUMS; ++i) sums[threadIdx.x * SUMS + i] = column_sum[i];
             __syncthreads();
@@ -585,7 +591,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
 #pragma unroll
                 for (int g = 0; g < 64 * W * SUMS / COLS; ++g) s += sums[g * COLS + threadIdx.x];
                 if (!whole)
-                    a.part[(int64_t)gridDim.z * out_rows * a.k + (int64_t)blockIdx.z * a.k + cc] = s;
+                    a.part[(int64_t)a.parts * out_rows * a.k + (int64_t)block_z * a.k + cc] = s;
                 else if (a.bias_out)
                     a.bias_out[cc] = s;
             }
@@ -1357,7 +1363,7 @@ Plan product_plan(bool grad, int64_t m, int32_t n_features, int32_t k, int type)
 template <int TYPE, Source SRC, int MT, int NT, bool WIDE>
 bool launched(const Plan &p, const ProductArgs &a, hipStream_t st) {
     if (p.src != SRC || p.mt != MT || p.nt != NT || (WIDE && (a.mat_stride % 4 || !aligned(a.mat, 4 * type_bytes(TYPE))))) return false;
-    k_product<TYPE, SRC, MT, NT, WIDE><<<dim3((unsigned)p.row_blocks, (unsigned)p.col_blocks, (unsigned)p.parts), 64 * W, 0, st>>>(a);
+    k_product<TYPE, SRC, MT, NT, WIDE><<<8 * (unsigned)ceil_div(p.row_blocks * p.col_blocks * p.parts, 8), 64 * W, 0, st>>>(a);
     return true;
 }
 
@@ -1367,7 +1373,10 @@ int product(const Plan &p, ProductArgs a, void *work, hipStream_t st) {
     a.steps = p.steps;
     a.steps_per_part = p.per_part;
     a.part = (float *)((char *)work + p.turned_bytes);
-    REQUIRE(p.row_blocks * 64 * W < MAX_THREADS, "%lld rows are too many", (long long)p.out_rows);
+    a.row_blocks = (int32_t)p.row_blocks;
+    a.col_blocks = (int32_t)p.col_blocks;
+    a.parts = p.parts;
+    REQUIRE((p.row_blocks * p.col_blocks * p.parts + 8) * 64 * W < MAX_THREADS, "%lld rows of %d columns are too many", (long long)p.out_rows, a.k);
     if (p.parts) {
         bool done;
         if constexpr (GRAD) {

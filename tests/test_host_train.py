@@ -52,7 +52,7 @@ SCORES = dict(bits=P, n=10, row_stride=4, n_features=100, rows=None, m=10, table
     (dict(bits=None), "d_bits"), (dict(bits=P + 4), "d_bits"), (dict(table=None), "d_table"), (dict(table=P + 2), "d_table"),
     (dict(table_stride=2), "d_table's stride"), (dict(scores=None), "d_scores"), (dict(score_stride=2), "d_scores's stride"), (dict(bias=P + 1), "d_bias"),
     (dict(rows=P + 2), "d_rows"), (dict(n=-1, rows=P), "n = -1"), (dict(m=1 << 31, rows=P), "m = "),
-    (dict(m=(1 << 31) - 1, rows=P), "2147483647 rows are too many"),
+    (dict(m=(1 << 31) - 1, rows=P), "2147483647 rows of 3 columns are too many"),
 ])
 def test_scores_refusals(change, message):
     rc = _lib.train_lib().stag_row_scores_dev(*{**SCORES, **change}.values())
