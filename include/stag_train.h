@@ -24,7 +24,8 @@
  * that a call takes.  Results do not depend on timing: equal inputs give equal bits.
  *
  * Sizes: 0 <= m < 2^31 rows of a batch, 1 <= k <= 2^20 classifiers, 1 <= n_features <= 2^27; the strides of tables, scores and
- * gradients are at least k and at most 2^21 values.  What is larger is refused.
+ * gradients are at least k and at most 2^21 values.  What is larger, or needs more workgroups than a launch has, is refused.
+ * Rows of tables and gradients that all begin at a multiple of 16 bytes (32-bit values) or 8 are read faster.
  */
 #ifndef STAG_TRAIN_H
 #define STAG_TRAIN_H

@@ -58,9 +58,9 @@ __device__ __forceinline__ const uint32_t *row_of(const uint32_t *bits, int64_t 
 // in 16 bits; a 32-bit coefficient is cut into three bf16 pieces of 8 bits each, which together are the coefficient,
 // and multiplied piece by piece into the same 32-bit sums.  16-bit coefficients go in as they are.
 //
-// What bounds them: the matrix cores for 32-bit coefficients (8,192 rows x 7,500 features x 1,000 columns: 222 us, 1.7 PFLOP/s of bf16
+// What bounds them: the matrix cores for 32-bit coefficients (8,192 rows x 7,500 features x 1,000 columns: 218 us, 1.7 PFLOP/s of bf16
 // operations counted densely; a library's bf16 product of 8,192^3 reaches 1.19 on the same card), the making of operands
-// beside them for 16-bit ones (that size's gradient in bf16: 108 us, 1.2 PFLOP/s), latency for one node's batch (4,096 x
+// beside them for 16-bit ones (that size's gradient in bf16: 105 us, 1.2 PFLOP/s), latency for one node's batch (4,096 x
 // 7,500 x 13: 10 us and 3 for adding up its parts).
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
@@ -176,7 +176,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
     __shared__ float sums[GRAD ? 64 * W * SUMS : 1];
     __shared__ int note[NOTES], noted, met, bad;
     // Workgroups go round the card's 8 dies in turn; each die is given neighbours in row blocks of the same columns and terms, which share the
-    // coefficients in its L2.
+    // coefficients in its L2 (HBM reads of the level's scores 248 -> 85 MB, of its gradient 193 -> 85; 221 -> 218 and 107.5 -> 104.7 us).
     const int per_die = gridDim.x / 8, tile = (int)(blockIdx.x % 8) * per_die + (int)(blockIdx.x / 8);
     if (tile >= a.row_blocks * a.col_blocks * a.parts) return;
     const int block_x = tile % a.row_blocks, block_y = tile / a.row_blocks % a.col_blocks, block_z = tile / a.row_blocks / a.col_blocks;
