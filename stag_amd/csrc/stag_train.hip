@@ -1580,10 +1580,12 @@ int stag_adamw_dev(const stag_adamw_tensor_t *d_tensors, const stag_adamw_tile_t
     REQUIRE(lr >= 0 && std::isfinite(lr), "lr = %g", lr);
     REQUIRE(beta1 > 0 && beta1 < 1 && beta2 > 0 && beta2 < 1, "beta1 = %g, beta2 = %g: not inside (0, 1)", beta1, beta2);
     REQUIRE(eps >= 0 && std::isfinite(eps), "eps = %g", eps);
-    if (n_tiles == 0) return STAG_OK;
-    REQUIRE(d_tensors && d_tiles && d_step && aligned(d_tensors, 8) && aligned(d_tiles, 8) && aligned(d_step, 4), "d_tensors, d_tiles or d_step is null or not aligned");
-    REQUIRE(d_m && d_v && aligned(d_m, 16) && aligned(d_v, 16), "d_m or d_v is null or not 16-byte aligned");
-    REQUIRE(state_bits == 32 || (d_m_scale && d_v_scale && aligned(d_m_scale, 4) && aligned(d_v_scale, 4)), "8-bit states have scales");
+    REQUIRE(d_step && aligned(d_step, 4), "d_step is null or not aligned");
+    if (n_tiles > 0) {
+        REQUIRE(d_tensors && d_tiles && aligned(d_tensors, 8) && aligned(d_tiles, 8), "d_tensors or d_tiles is null or not aligned");
+        REQUIRE(d_m && d_v && aligned(d_m, 16) && aligned(d_v, 16), "d_m or d_v is null or not 16-byte aligned");
+        REQUIRE(state_bits == 32 || (d_m_scale && d_v_scale && aligned(d_m_scale, 4) && aligned(d_v_scale, 4)), "8-bit states have scales");
+    }
     AdamwArgs a;
     a.tensors = d_tensors;
     a.tiles = d_tiles;
@@ -1603,7 +1605,7 @@ int stag_adamw_dev(const stag_adamw_tensor_t *d_tensors, const stag_adamw_tile_t
     a.eps = (float)eps;
     a.split = n_tiles <= 2048 ? 4 : 1;
     const int64_t waves = n_tiles * a.split;
-    const unsigned grid = (unsigned)(waves < 4 * 4096 ? ceil_div(waves, 4) : 4096);
+    const unsigned grid = (unsigned)(waves < 4 * 4096 ? ceil_div(waves + (waves == 0), 4) : 4096);      // a step of nothing is counted too
     if (state_bits == 32)
         k_adamw<32><<<grid, 256, 0, (hipStream_t)stream>>>(a);
     else

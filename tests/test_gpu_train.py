@@ -597,6 +597,33 @@ def test_adamw_at_odd_addresses(bits):
         assert buffers[0][0] == 7 and (buffers[0][2002:] == 7).all()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_counts_a_step_of_nothing(bits):
+    empty, one = torch.zeros((0, 5), device=DEV), torch.tensor(1.0, device=DEV)
+    opt = train.AdamW([empty], [empty.clone()], state_bits=bits)
+    opt.step(), opt.step()
+    assert opt.steps == 2
+    opt = train.AdamW([empty, one], [empty.clone(), torch.tensor(2.0, device=DEV)], lr=0.25, state_bits=bits)      # a tensor of no dimensions has one value
+    opt.step(), opt.step()
+    assert opt.steps == 2 and abs(float(one) - 0.5) < (1e-5 if bits == 32 else 0.25 / 4)      # the moments are off by 1/8 at most in the second step
+
+
+def test_parameters_and_unsigned_words():
+    """Parameters that require gradients are tensors like others (nothing is recorded), and so are rows of uint32 words."""
+    rng = np.random.default_rng(8)
+    for n in (1, 700):
+        bits, _ = packed(rng, n, 300)
+        table = torch.from_numpy(rng.normal(size=(300, 40)).astype(np.float32)).to(DEV)
+        bias = torch.ones(40, device=DEV)
+        want = train.row_scores(bits, table, bias)
+        got = train.row_scores(bits.view(torch.uint32), torch.nn.Parameter(table), torch.nn.Parameter(bias))
+        assert torch.equal(got, want) and not got.requires_grad
+        assert torch.equal(train.row_scores_grad(bits.view(torch.uint32), want, 300)[0], train.row_scores_grad(bits, want, 300)[0])
+    p = torch.nn.Parameter(torch.ones(10, device=DEV))
+    train.AdamW([p], [torch.ones(10, device=DEV)], lr=0.5).step()
+    assert (p - 0.5).abs().max() < 1e-5
+
+
 def test_adamw_refuses_shared_memory():
     x, y = torch.zeros(100, device=DEV), torch.zeros(100, device=DEV)
     with pytest.raises(ValueError, match=r"params\[0\] and params\[1\] share memory"):
