@@ -1060,9 +1060,11 @@ __device__ __forceinline__ void store4(void *p, int type, int64_t at, int64_t co
     }
 }
 
-// the largest of the wave's values (not negative), the same for every lane
-__device__ __forceinline__ int wave_max(int x) {
-#define STAG_MAX_DPP(CONTROL) x = max(x, __builtin_amdgcn_update_dpp(x, x, CONTROL, 0xf, 0xf, false));
+// the largest of the wave's x and of its y, the same for every lane; both at once, since a lane's neighbour can be read two instructions on
+__device__ __forceinline__ void wave_max(uint32_t &x, uint32_t &y) {
+#define STAG_MAX_DPP(CONTROL)                                                              \
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CONTROL, 0xf, 0xf, true)); \
+    y = max(y, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)y, CONTROL, 0xf, 0xf, true));
     STAG_MAX_DPP(0x111)      // row_shr 1, 2, 4, 8: the last lane of each 16 has their maximum
     STAG_MAX_DPP(0x112)
     STAG_MAX_DPP(0x114)
@@ -1070,26 +1072,30 @@ __device__ __forceinline__ int wave_max(int x) {
     STAG_MAX_DPP(0x142)      // row_bcast 15, 31: the last lane has all
     STAG_MAX_DPP(0x143)
 #undef STAG_MAX_DPP
-    return __builtin_amdgcn_readlane(x, 63);
+    x = (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+    y = (uint32_t)__builtin_amdgcn_readlane((int)y, 63);
 }
 
-// The exponent (biased) of the smallest power of two s with max|x| <= 448 s over the wave's 256 values; 448 = 1.75 * 2^8 is
-// the largest e4m3 value.  A power of two, so that dividing by it rounds nothing.  Infinities and NaN have no say.
-__device__ __forceinline__ int scale_exponent(const float *x) {
-    int top = 10 << 23;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) top = max(top, __float_as_int(x[j]) & 0x7fffffff);
-    top = wave_max(top);
-    if (top >= 0x7f800000) {
-        top = 10 << 23;
+// The exponents (biased) of the smallest powers of two s with max|x| <= 448 s over the wave's 256 values x, and y >= 0; 448 = 1.75 * 2^8
+// is the largest e4m3 value.  A power of two, so that dividing by it rounds nothing.  Infinities and NaN have no say.
+__device__ __forceinline__ void scale_exponents(const float *x, const float *y, int &x_exponent, int &y_exponent) {
+    constexpr float LEAST = 0x1p-117f;      // biased exponent 10
+    uint32_t top_x = __float_as_uint(fmaxf(fmaxf(fmaxf(LEAST, fabsf(x[0])), fmaxf(fabsf(x[1]), fabsf(x[2]))), fabsf(x[3])));
+    uint32_t top_y = __float_as_uint(fmaxf(fmaxf(fmaxf(LEAST, fabsf(y[0])), fmaxf(fabsf(y[1]), fabsf(y[2]))), fabsf(y[3])));
+    wave_max(top_x, top_y);
+    if (max(top_x, top_y) >= 0x7f800000u) {
+        asm volatile("");                   // seldom: not to be computed beforehand
+        top_x = top_y = __float_as_uint(LEAST);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int a = __float_as_int(x[j]) & 0x7fffffff;
-            top = max(top, a < 0x7f800000 ? a : 0);
+            const uint32_t a = __float_as_uint(x[j]) & 0x7fffffffu, b = __float_as_uint(y[j]) & 0x7fffffffu;
+            top_x = max(top_x, a < 0x7f800000u ? a : 0u);
+            top_y = max(top_y, b < 0x7f800000u ? b : 0u);
         }
-        top = wave_max(top);
+        wave_max(top_x, top_y);
     }
-    return (top >> 23) - 8 + ((top & 0x7fffff) > 0x600000);
+    x_exponent = (int)(top_x >> 23) - 8 + ((top_x & 0x7fffffu) > 0x600000u);
+    y_exponent = (int)(top_y >> 23) - 8 + ((top_y & 0x7fffffu) > 0x600000u);
 }
 
 // a = |x| / s as the value of an e4m3 code, up or down by `chance` (16 bits).  From 2^-6 on a code has 3 bits behind the
@@ -1120,7 +1126,7 @@ __device__ __forceinline__ void unpack_e4m3(uint32_t q, float *x) {
 
 // A wave takes a tile of four blocks of 256 values, four neighbouring values a lane, and has the loads of GROUP blocks in
 // flight before it computes.  Everything is read once and written once; what bounds it with 32-bit states is HBM (the 54 million
-// values of 1,600 tables in 32 bits, 1.5 GB: 266 us, 5.7 TB/s), with 8-bit ones the 30 instructions a value (as bf16: 142 us, 3.8 TB/s).  m, v and the root are rounded after
+// values of 1,600 tables in 32 bits, 1.5 GB: 266 us, 5.7 TB/s), with 8-bit ones the 75 instructions a value (as bf16: 138 us, 3.9 TB/s).  m, v and the root are rounded after
 // every operation (no fused multiply-add), so that the 8-bit codes are a function of the inputs that any other 32-bit
 // implementation can restate.
 template <int BITS>
@@ -1210,7 +1216,8 @@ __global__ __launch_bounds__(256) void k_adamw(AdamwArgs a) {
                     store4(a.m, STAG_F32, s, 0, true, m);
                     store4(a.v, STAG_F32, s, 0, true, v);
                 } else {
-                    const int me = scale_exponent(m), ve = scale_exponent(root);
+                    int me, ve;
+                    scale_exponents(m, root, me, ve);
                     const float mi = __int_as_float((254 - me) << 23), vi = __int_as_float((254 - ve) << 23);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
