@@ -1098,23 +1098,18 @@ __device__ __forceinline__ void scale_exponents(const float *x, const float *y, 
     y_exponent = (int)(top_y >> 23) - 8 + ((top_y & 0x7fffffu) > 0x600000u);
 }
 
-// a = |x| / s as the value of an e4m3 code, up or down by `chance` (16 bits).  From 2^-6 on a code has 3 bits behind the
-// leading one: adding 20 random bits below them and cutting them off goes up with the probability of what is cut.  Below
-// 2^-6 codes are 2^-9 apart, as they are from 2^-6 to 2^-5: such a value is moved there, rounded and moved back.
-__device__ __forceinline__ float rounded(float a, uint32_t chance) {
-    const float up = a < 0x1p-6f ? 0x1p-6f : 0.f;
-    return __uint_as_float((__float_as_uint(a + up) + (chance << 4 | 8u)) & 0xfff00000u) - up;
+// x's e4m3 code as byte J of `codes`, rounded up or down by `chance` (the upper 16 bits of it).  From 2^-6 on a code has 3 bits behind the
+// leading one: adding 20 random bits below them and cutting them off goes up with the probability of what is cut.  Below 2^-6
+// codes are 2^-9 apart, as they are from 2^-6 to 2^-5: such a value is moved there (what is below 2^-29 of it is dropped), rounded and moved back.
+// That is what the conversion instruction does; written out it took 9 instructions.
+template <int J> __device__ __forceinline__ uint32_t with_e4m3(float x, uint32_t chance, uint32_t codes) {
+    return (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(x, (int)((chance & 0xffff0000u) | 0x8000u), (int)codes, J);
 }
 
 // sqrt(x), x >= 0, from x / sqrt(x) and one step of Newton's method, which puts the rounding right
 __device__ __forceinline__ float root_of(float x) {
     const float s = __builtin_amdgcn_rsqf(x), y = x * s;
     return x == 0.f || x == INFINITY ? x : fmaf(fmaf(-y, y, x), 0.5f * s, y);
-}
-
-__device__ __forceinline__ uint32_t pack_e4m3(const float *x) {
-    int q = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], q, true);
 }
 
 __device__ __forceinline__ void unpack_e4m3(uint32_t q, float *x) {
@@ -1219,18 +1214,25 @@ __global__ __launch_bounds__(256) void k_adamw(AdamwArgs a) {
                     int me, ve;
                     scale_exponents(m, root, me, ve);
                     const float mi = __int_as_float((254 - me) << 23), vi = __int_as_float((254 - ve) << 23);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    uint32_t m_codes = 0, v_codes = 0;
+                    auto code = [&](auto place) {
+                        constexpr int j = place.value;
                         uint32_t x = (uint32_t)(s + j) ^ salt;
                         x = (x ^ x >> 16) * 0x7FEB352Du;
                         x = (x ^ x >> 15) * 0x846CA68Bu;
                         x ^= x >> 16;
-                        const float y = m[j] * mi, q = rounded(root[j] * vi, x & 0xffffu);
-                        m[j] = copysignf(rounded(fabsf(y), x >> 16), y);
-                        v[j] = root[j] > 0.f && q == 0.f ? 0x1p-9f : q;      // a root of zero would divide by eps alone: what is not zero stays so
-                    }
-                    __builtin_nontemporal_store(pack_e4m3(m), (uint32_t *)((uint8_t *)a.m + s));
-                    __builtin_nontemporal_store(pack_e4m3(v), (uint32_t *)((uint8_t *)a.v + s));
+                        // a root of zero would divide by eps alone: what is not zero stays so
+                        uint32_t q = __float_as_uint(root[j] * vi);
+                        if (q - 1u < 0x3b000000u - 1u) q = 0x3b000000u;      // 2^-9
+                        m_codes = with_e4m3<j>(m[j] * mi, x, m_codes);
+                        v_codes = with_e4m3<j>(__uint_as_float(q), x << 16, v_codes);
+                    };
+                    code(std::integral_constant<int, 0>());
+                    code(std::integral_constant<int, 1>());
+                    code(std::integral_constant<int, 2>());
+                    code(std::integral_constant<int, 3>());
+                    __builtin_nontemporal_store(m_codes, (uint32_t *)((uint8_t *)a.m + s));
+                    __builtin_nontemporal_store(v_codes, (uint32_t *)((uint8_t *)a.v + s));
                     if (lane == 0) {
                         a.m_scale[s >> 8] = __int_as_float(me << 23);
                         a.v_scale[s >> 8] = __int_as_float(ve << 23);

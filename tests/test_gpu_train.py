@@ -475,7 +475,8 @@ def test_adamw_32(which, t):
 def restated_rounding(x, scale, chance):
     y = (x / scale).astype(np.float32)
     a = np.abs(y)
-    up = np.where(a < 2.0 ** -6, np.float32(2.0 ** -6), np.float32(0))       # below 2^-6 codes are as far apart as above it
+    up = np.where(a < 2.0 ** -6, np.float32(2.0 ** -6), np.float32(0))       # below 2^-6 codes are as far apart as above it, and what is
+    a = np.where(a < 2.0 ** -6, np.floor(a * np.float32(2.0 ** 29)) * np.float32(2.0 ** -29), a)      # below 2^-29 is dropped
     bits = ((a + up).view(np.uint32) + (chance << 4 | 8).astype(np.uint32)) & np.uint32(0xfff00000)
     return np.copysign(bits.view(np.float32) - up, y)
 
