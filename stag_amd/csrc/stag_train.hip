@@ -1121,7 +1121,7 @@ __device__ __forceinline__ void unpack_e4m3(uint32_t q, float *x) {
 
 // A wave takes a tile of four blocks of 256 values, four neighbouring values a lane, and has the loads of GROUP blocks in
 // flight before it computes.  Everything is read once and written once; what bounds it with 32-bit states is HBM (the 54 million
-// values of 1,600 tables in 32 bits, 1.5 GB: 266 us, 5.7 TB/s), with 8-bit ones the 75 instructions a value (as bf16: 138 us, 3.9 TB/s).  m, v and the root are rounded after
+// values of 1,600 tables in 32 bits, 1.5 GB: 253 us, 6.0 TB/s), with 8-bit ones the 60 instructions a value (as bf16: 126 us, 4.3 TB/s).  m, v and the root are rounded after
 // every operation (no fused multiply-add), so that the 8-bit codes are a function of the inputs that any other 32-bit
 // implementation can restate.
 template <int BITS>
@@ -1614,7 +1614,10 @@ int stag_adamw_dev(const stag_adamw_tensor_t *d_tensors, const stag_adamw_tile_t
     a.eps = (float)eps;
     a.split = n_tiles <= 2048 ? 4 : 1;
     const int64_t waves = n_tiles * a.split;
-    const unsigned grid = (unsigned)(waves < 4 * 4096 ? ceil_div(waves + (waves == 0), 4) : 4096);      // a step of nothing is counted too
+    // A tile a wave with 32-bit states; with 8-bit ones a few, since a wave's start costs as much as half a tile's arithmetic (1,600
+    // tables, up to 4,096, 8,192, 16,384 workgroups: 270, 259, 254 us and 133, 125, 131).  A step of nothing is counted too.
+    const int64_t most = state_bits == 32 ? 1 << 20 : 8192;
+    const unsigned grid = (unsigned)(waves < 4 * most ? ceil_div(waves + (waves == 0), 4) : most);
     if (state_bits == 32)
         k_adamw<32><<<grid, 256, 0, (hipStream_t)stream>>>(a);
     else
