@@ -1429,7 +1429,7 @@ struct LossPlan {
     unsigned gx, gy;
 };
 
-LossPlan loss_plan(int64_t m, int32_t k, int v) {
+LossPlan loss_plan(int64_t m, int32_t k, int v, bool siblings) {
     LossPlan p;
     // few values: one workgroup a column tile, whose sums are the result without a second launch; the more threads, the
     // fewer values one after the other (300 x 8: 9.3 us with 256 threads of four columns, 4.7 with 1,024 of one)
@@ -1439,7 +1439,10 @@ LossPlan loss_plan(int64_t m, int32_t k, int v) {
     const int64_t cols = ceil_div(k, p.v);
     p.ct = (int)(cols < p.threads ? cols : p.threads);
     p.gy = (unsigned)ceil_div(cols, p.ct);
-    const int64_t passes = ceil_div(m, p.threads / p.ct), wanted = 1024 / p.gy > 0 ? 1024 / p.gy : 1;
+    // 1,024 workgroups, or 512 where each writes rows of siblings' gradients over nearly all of its threads (65,536 x 1,000 in 32 bits 60
+    // against 71 us, x 4,000 in bf16 97 against 112; over half of the threads, x 1,000 and x 520 in bf16, 52 against 36 and 47 against 30)
+    const unsigned all = siblings && p.ct >= 192 ? 512 : 1024;
+    const int64_t passes = ceil_div(m, p.threads / p.ct), wanted = all / p.gy > 0 ? all / p.gy : 1;
     p.gx = (unsigned)(few ? 1 : passes < wanted ? passes : wanted);
     return p;
 }
@@ -1543,7 +1546,7 @@ int64_t stag_sibling_loss_workspace(int64_t m, int32_t k) {
     REQUIRE(k >= 1 && k <= MAX_K, "k = %d is not in 1..%d", k, MAX_K);
     unsigned most = 1;
     for (int v : {1, 4, 8}) {
-        const unsigned gx = loss_plan(m, k, v).gx;
+        const unsigned gx = loss_plan(m, k, v, false).gx;      // siblings take no more
         if (gx > most) most = gx;
     }
     return most > 1 ? (int64_t)most * k * 4 : 0;
@@ -1567,7 +1570,7 @@ int stag_sibling_loss_dev(const float *d_scores, int64_t score_stride, int64_t m
     auto fits = [&](int v) {
         return k % v == 0 && score_stride % v == 0 && aligned(d_scores, 16) && (!d_grad || (grad_stride % v == 0 && aligned(d_grad, v * type_bytes(type))));
     };
-    const LossPlan p = loss_plan(m, k, type != STAG_F32 && fits(8) ? 8 : fits(4) ? 4 : 1);
+    const LossPlan p = loss_plan(m, k, type != STAG_F32 && fits(8) ? 8 : fits(4) ? 4 : 1, d_siblings != nullptr);
     LossArgs a = {};
     a.scores = d_scores, a.weight = d_weight, a.label = d_label, a.siblings = d_siblings, a.loss = d_loss, a.grad = d_grad;
     a.score_stride = score_stride, a.grad_stride = grad_stride, a.m = m, a.k = k, a.scale = scale;
