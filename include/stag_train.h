@@ -94,7 +94,8 @@ int stag_sibling_loss_dev(const float *d_scores, int64_t score_stride, int64_t m
  * One AdamW step over n tensors in one launch.  For every value, with t = *d_step + 1:
  *   m = beta1 m + (1 - beta1) g;   v = beta2 v + (1 - beta2) g^2;   d = sqrt(v / (1 - beta2^t)) + eps
  *   p = p (1 - lr weight_decay) - lr m / ((1 - beta1^t) d);   with l1 > 0 then  p = sign(p) max(|p| - lr l1 / d, 0)
- * and t is stored to *d_step.  Computed in 32 bits; p is rounded to its type at the end, to nearest.
+ * and t is stored to *d_step.  Computed in 32 bits, subnormal numbers included; p is rounded to its type at the end, to nearest.
+ * A square below 2^-149 is 0: with eps = 0 a value whose gradients were all under 2^-70 may become infinite or NaN.
  *
  * The last is the proximal step of l1 * |p| in the metric of the update, so that a point at rest has
  * |mean gradient| <= l1: the LASSO's condition.

@@ -1106,10 +1106,28 @@ template <int J> __device__ __forceinline__ uint32_t with_e4m3(float x, uint32_t
     return (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(x, (int)((chance & 0xffff0000u) | 0x8000u), (int)codes, J);
 }
 
-// sqrt(x), x >= 0, from x / sqrt(x) and one step of Newton's method, which puts the rounding right
-__device__ __forceinline__ float root_of(float x) {
-    const float s = __builtin_amdgcn_rsqf(x), y = x * s;
-    return x == 0.f || x == INFINITY ? x : fmaf(fmaf(-y, y, x), 0.5f * s, y);
+// The roots of four values >= 0.  32 bits: by the instruction.  8 bits: from x / sqrt(x) and one step of Newton's method, which puts the
+// rounding right.  The instructions take what is below 2^-126 for zero, and what Newton's step subtracts below 2^-96 is no normal
+// number; such values (zero among them) are multiplied by 2^64 first, in a branch that a wave seldom takes.
+template <int BITS> __device__ __forceinline__ void roots_of(const float *x, float *root) {
+    auto plain = [](float x) {
+        if constexpr (BITS == 32) return __builtin_amdgcn_sqrtf(x);
+        const float s = __builtin_amdgcn_rsqf(x), y = x * s;
+        return x == 0.f || x == INFINITY ? x : fmaf(fmaf(-y, y, x), 0.5f * s, y);
+    };
+    constexpr uint32_t SMALL = 0x0f800000u;      // 2^-96
+    const uint32_t least = min(min(__float_as_uint(x[0]), __float_as_uint(x[1])), min(__float_as_uint(x[2]), __float_as_uint(x[3])));
+    if (least >= SMALL) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) root[j] = plain(x[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool small = __float_as_uint(x[j]) < SMALL;
+            const float y = plain(small ? x[j] * 0x1p64f : x[j]);
+            root[j] = small ? y * 0x1p-32f : y;
+        }
+    }
 }
 
 __device__ __forceinline__ void unpack_e4m3(uint32_t q, float *x) {
@@ -1195,8 +1213,8 @@ __global__ __launch_bounds__(256) void k_adamw(AdamwArgs a) {
                 for (int j = 0; j < 4; ++j) {
                     m[j] = m[j] * a.beta1 + g[j] * a.one_minus_beta1;
                     v[j] = v[j] * a.beta2 + (g[j] * g[j]) * a.one_minus_beta2;
-                    root[j] = BITS == 32 ? __builtin_amdgcn_sqrtf(v[j]) : root_of(v[j]);
                 }
+                roots_of<BITS>(v, root);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float r = __builtin_amdgcn_rcpf(fmaf(root[j], c2, a.eps));

@@ -580,6 +580,74 @@ def test_adamw_where_the_second_moment_overflows(bits):
     assert torch.isfinite(p[:7]).all() and torch.isfinite(p[8:]).all() and torch.isinf(opt.v[7]) if bits == 32 else torch.isnan(opt.v.float()[7])
 
 
+def small_gradients(rng, n_blocks=14):
+    """Blocks of 256 gradients of about 1e-23, 3e-23 .. 3e-17, and one block of all of these sizes."""
+    size = np.repeat(10.0 ** (-23 + 0.5 * np.arange(n_blocks - 1)), 256)
+    size = np.concatenate([size, rng.permutation(size)[:256]])
+    return (size * rng.uniform(0.3, 1, size.size) * rng.choice([-1.0, 1.0], size.size)).astype(np.float32)
+
+
+def root_range(v, operations):
+    """Between what the root lies of v made in 32 bits by this many operations: each is off by U of v, or by 2^-150 where it has less than 24 bits."""
+    off = operations * (U * v + 2.0 ** -150)
+    return np.sqrt(np.maximum(v - off, 0)) * (1 - 2 * U), np.sqrt(v + off) * (1 + 2 * U)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_where_the_second_moment_is_below_the_normal_numbers(bits):
+    """Second moments of 1e-49 to 1e-37, where numbers of 32 bits end at 1.4e-45 and have all their bits from 1.2e-38 on: two steps."""
+    rng = np.random.default_rng(23)
+    g = small_gradients(rng)
+    d_g, p = torch.from_numpy(g).to(DEV), torch.zeros(g.size, device=DEV)
+    opt = train.AdamW([p], [d_g], lr=0.1, eps=1e-8, state_bits=bits)
+
+    def held():
+        if bits == 32:
+            return opt.m.double().cpu().numpy(), opt.v.double().sqrt().cpu().numpy()
+        return tuple((x.double().view(-1, 256) * s.double().unsqueeze(1)).flatten().cpu().numpy() for x, s in ((opt.m, opt.m_scale), (opt.v, opt.v_scale)))
+
+    g = g.astype(np.float64)
+    for t in (1, 2):
+        before, start = held(), p.double().cpu().numpy()
+        opt.step()
+        if t == 1:
+            d_g.mul_(0.5)
+        m, v = before[0] * 0.9 + g * 0.1, before[1] ** 2 * 0.999 + g * g * 0.001
+        lo, hi = root_range(v, 6)
+        # roots are off by sqrt(6 * 2^-150) = 7e-23 at most, which makes 2e-13 of d; 16 operations and constants of 32 bits
+        want = start - 0.1 * m / ((1 - 0.9 ** t) * (np.sqrt(v / (1 - 0.999 ** t)) + 1e-8))
+        near(p.cpu(), want, 16 * U * (np.abs(start) + np.abs(want - start)) + 1e-12 * np.abs(want - start))
+        after = held()
+        if bits == 32:
+            near(after[0], m, 4 * U * (np.abs(before[0]) + np.abs(g)))
+            assert (after[1] >= lo).all() and (after[1] <= hi).all()
+        else:      # a code is off by less than one step of its own: 2^-3 of it, 2^-9 scales at least
+            for got, low, high, scale in ((np.abs(after[0]), np.abs(m) * (1 - 4 * U), np.abs(m) * (1 + 4 * U), opt.m_scale), (after[1], lo, hi, opt.v_scale)):
+                s = np.repeat(scale.double().cpu().numpy(), 256)
+                assert (got >= low - np.maximum(low / 8, s / 512)).all() and (got <= high + np.maximum(high / 8, s / 512)).all()
+        g = g * 0.5
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_steps_by_lr_where_the_second_moment_is_below_the_normal_numbers(bits):
+    """A first step without eps moves a value by lr, however small its gradient."""
+    rng = np.random.default_rng(24)
+    g = (10.0 ** rng.uniform(-20, -17, 3000) * rng.choice([-1.0, 1.0], 3000)).astype(np.float32)
+    p = torch.zeros(3000, device=DEV)
+    train.AdamW([p], [torch.from_numpy(g).to(DEV)], lr=0.125, eps=0.0, state_bits=bits).step()
+    v = g.astype(np.float64) ** 2 * 0.001
+    lo, hi = root_range(v, 4)
+    near(p.cpu(), -0.125 * np.sign(g), 0.125 * (np.maximum(np.sqrt(v) / lo, hi / np.sqrt(v)) - 1 + 16 * U))
+
+
+def test_a_fit_with_8_bit_states_stays_finite():
+    """Rows scored far from 0 leave tokens that they meet first with gradients of 1e-21 to 1e-18."""
+    rng = np.random.default_rng(25)
+    bits, _, label = problem(rng, n=1024, ncol=1500, k=8)
+    for steps, k, batch in ((8, 8, 256), (40, 4, 64)):
+        assert np.isfinite(train.fit_siblings(bits, label, k, 7500, steps=steps, batch=batch, l1=1e-4, state_bits=8)).all()
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_adamw_at_odd_addresses(bits):
     """Tensors at addresses that no vector load may use, and what lies around them."""
