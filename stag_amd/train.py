@@ -18,6 +18,7 @@ they take no part in autograd.  With their outputs given (``out=``) or allocated
 HIP graph.  Inputs whose rows are not contiguous (or lie more than 2^21 values apart) are copied first; outputs have to be as
 documented and may share memory with nothing else that the call takes.
 """
+import ctypes
 import functools
 import math
 
@@ -38,6 +39,7 @@ _BITS = (torch.int32, torch.uint32)
 _empty = torch.empty_strided
 _raw_stream = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream(i).cuda_stream without the objects
 _current = torch._C._cuda_getDevice
+_address, _size = _Tensor.data_ptr, torch._C.StorageBase.nbytes
 _MAX_STRIDE = 1 << 21                                # values from one row of a matrix to the next
 
 
@@ -325,17 +327,24 @@ def sibling_loss(scores, label, *, siblings=None, weight=None, scale=1.0, grad_d
     return loss, grad
 
 
+def _fixed(t):
+    """t's memory as a tensor whose storage cannot be resized."""
+    return None if t is None else torch.utils.dlpack.from_dlpack(torch.utils.dlpack.to_dlpack(t.view(torch.uint8))).view(t.dtype)
+
+
 class AdamW:
     """AdamW over a list of tensors, one launch a step, with an optional L1 shrinkage (stag_adamw_dev).
 
     params, grads: lists of contiguous tensors (float32, bfloat16 or float16) on one GPU, a gradient as large as its parameter.  The
-    optimizer holds THESE tensors: it reads the gradients from them and updates the parameters in place, at every step.
+    optimizer holds THESE tensors: it reads the gradients from them and updates the parameters in place, at every step.  They keep
+    the memory they had when it was made: after ``.data = ...``, ``set_``, a ``resize_`` that moves one or a module's ``.to(dtype)``, step() raises
+    ValueError.  (Of views that share a storage it looks at one; another that is given other memory is not followed: step() goes on with the old.)
     weight_decay, l1: a number, or one for each tensor.  state_bits 32 keeps the moments as floats; 8 keeps e4m3 codes with a
     power-of-two scale for each 256 values (m, m_scale: the first moment; v, v_scale: the ROOT of the second), 2.03 bytes
     a value instead of 8.  m, v and the scales are flat: tensor j's values begin at place state_at[j], a multiple of 256.
     Addresses are taken once, so an AdamW is neither copied nor pickled: make another, and load_state() into it.
-    The step count lives on the GPU, so a captured step() counts on when it is replayed; lr and the others are the values that
-    step() was called with (attributes, may be changed between steps)."""
+    The step count lives on the GPU, so a captured step() counts on when it is replayed (a graph holds none of this memory: the AdamW
+    has to live as long); lr and the others are the values that step() was called with (attributes, may be changed between steps)."""
 
     def __init__(self, params, grads, *, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, l1=0.0, state_bits=32):
         params, grads = list(params), list(grads)
@@ -408,24 +417,43 @@ class AdamW:
         if state_bits == 8:
             self._m_scale = torch.ones(size // BLOCK, dtype=torch.float32, device=device)
             self._v_scale = torch.ones(size // BLOCK, dtype=torch.float32, device=device)
-        self._where = (self._tensors.data_ptr(), self._tiles.data_ptr(), self._n_tiles, state_bits, self._m.data_ptr(), self._v.data_ptr(), _ptr(self._m_scale),
-                       _ptr(self._v_scale), self._step.data_ptr())
+        # What the kernel reads and writes stays allocated while its address is held: a storage for each memory, and a tensor whose address shows
+        # whether it moved.  The states are given out as tensors that cannot be resized.
+        memory = {}
+        for x in both:
+            storage = x.untyped_storage()
+            memory.setdefault(storage._cdata, (x, storage))
+        self._watched, self._storages = [list(x) for x in zip(*memory.values())]
+        self._addresses, self._sizes = [*map(_address, self._watched)], [*map(_size, self._storages)]
+        pointer = lambda x: None if x is None else ctypes.c_void_p(x.data_ptr())      # noqa: E731
+        self._where = (pointer(self._tensors), pointer(self._tiles), self._n_tiles, state_bits, pointer(self._m), pointer(self._v), pointer(self._m_scale),
+                       pointer(self._v_scale), pointer(self._step))
+        self._given_m, self._given_v, self._given_m_scale, self._given_v_scale = (_fixed(x) for x in (self._m, self._v, self._m_scale, self._v_scale))
+        self._gpu, self._launch = device.index, _lib.train_lib().stag_adamw_dev
 
     device, params, grads, m, v, m_scale, v_scale = (
-        property(lambda self, name=name: getattr(self, name)) for name in ("_device", "_params", "_grads", "_m", "_v", "_m_scale", "_v_scale"))
+        property(lambda self, name=name: getattr(self, name)) for name in ("_device", "_params", "_grads", "_given_m", "_given_v", "_given_m_scale", "_given_v_scale"))
 
     def __reduce_ex__(self, protocol):
         raise TypeError("an AdamW holds the addresses of its tensors: make another, and load_state() into it")
 
     def step(self):
         """One step with the gradients as they stand."""
-        gpu = self._device.index
+        gpu = self._gpu
         if gpu != _current():
             with torch.cuda.device(gpu):
                 return self.step()
-        rc = _lib.train_lib().stag_adamw_dev(*self._where, self.lr, *self.betas, self.eps, _raw_stream(gpu))
+        if [*map(_address, self._watched)] != self._addresses or [*map(_size, self._storages)] != self._sizes:
+            self._moved()
+        rc = self._launch(*self._where, self.lr, *self.betas, self.eps, _raw_stream(gpu))
         if rc:
             _lib.check_train(rc)
+
+    def _moved(self):
+        for x, at, storage, size in zip(self._watched, self._addresses, self._storages, self._sizes):
+            if x.data_ptr() != at or _size(storage) != size:
+                name = next("%s[%d]" % (kind, j) for kind, held in (("params", self._params), ("grads", self._grads)) for j, y in enumerate(held) if y is x)
+                raise ValueError("%s has other memory than when this AdamW was made: make another" % name)
 
     @property
     def steps(self):
@@ -437,14 +465,14 @@ class AdamW:
         _need(0 <= int(steps) < 2**31 - 1, "steps = %r", steps)
         given = {"m": m, "v": v, "m_scale": m_scale, "v_scale": v_scale}
         for name, t in given.items():
-            mine = getattr(self, name)
+            mine = getattr(self, "_" + name)
             _need((t is None) == (mine is None), "%s: %s", name, "missing" if t is None else "states of 32 bits have none")
             if mine is not None:
                 _is(name, t, mine.dtype, 1)
                 _need(t.shape == mine.shape, "%s has %d values: %d are wanted", name, t.shape[0], mine.shape[0])
         for name, t in given.items():
             if t is not None:
-                getattr(self, name).copy_(t)
+                getattr(self, "_" + name).copy_(t)
         self._step[0] = int(steps)
 
 

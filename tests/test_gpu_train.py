@@ -739,6 +739,52 @@ def test_an_optimizer_keeps_its_tensors():
     assert isinstance(opt.params, tuple) and (opt.params[0] - 0.75).abs().max() < 1e-6
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("move", [
+    lambda x: setattr(x, "data", torch.ones(1000, device=DEV)), lambda x: x.set_(torch.ones(1000, device=DEV)), lambda x: x.resize_(100_000),
+    lambda x: x.untyped_storage().resize_(0), lambda x: setattr(x, "data", x.data.to(BF16))])
+def test_an_optimizer_whose_tensors_moved_does_not_step(move, bits):
+    """Memory that was given back may be another tensor's."""
+    for which in range(4):
+        params, grads = [torch.ones(1000, device=DEV) for _ in range(2)], [torch.ones(1000, device=DEV) for _ in range(2)]
+        opt = train.AdamW(params, grads, lr=0.25, state_bits=bits)
+        opt.step()
+        steps = opt.steps
+        move((params + grads)[which])
+        with pytest.raises(ValueError, match=r"%s\[%d\] has other memory" % ("params" if which < 2 else "grads", which % 2)):
+            opt.step()
+        assert opt.steps == steps
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_states_are_not_taken_away(bits):
+    p, q = torch.ones(1000, device=DEV), torch.ones(1000, device=DEV)
+    opt, other = (train.AdamW([x], [torch.ones(1000, device=DEV)], lr=0.25, state_bits=bits) for x in (p, q))
+    for name in ("m", "v") + (("m_scale", "v_scale") if bits == 8 else ()):
+        with pytest.raises(RuntimeError, match="not resizable"):
+            getattr(opt, name).untyped_storage().resize_(0)
+    opt.step(), other.step()
+    assert all(torch.equal(getattr(opt, x).view(torch.uint8), getattr(other, x).view(torch.uint8)) for x in ("m", "v"))
+    assert (opt.m[:1000].float() != 0).all()
+    opt.m.data = zeros = torch.zeros_like(opt.m)
+    opt.step(), other.step()
+    assert torch.equal(p, q) and not zeros.float().any()
+
+
+def test_an_optimizer_keeps_the_memory_of_views():
+    """A view that is given other memory is not followed; the memory it had stays the optimizer's while that lives."""
+    flat, grad = torch.ones(2000, device=DEV), torch.ones(2000, device=DEV)
+    views = [flat[:1000], flat[1000:]]
+    opt = train.AdamW(views, [grad[:1000], grad[1000:]], lr=0.25)
+    at = flat.data_ptr()
+    views[1].data = new = torch.ones(1000, device=DEV)
+    del flat
+    others = [torch.ones(2000, device=DEV) for _ in range(50)]
+    opt.step()
+    assert views[0].data_ptr() == at and (views[0] - 0.75).abs().max() < 1e-6
+    assert (new == 1).all() and all(x.data_ptr() != at and (x == 1).all() for x in others)
+
+
 # ------------------------------------------------------------------------------------------------------ used together
 def problem(rng, n=400, ncol=60, k=6):
     consensus = rng.integers(1, 5, (k, ncol))
