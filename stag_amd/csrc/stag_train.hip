@@ -146,7 +146,7 @@ enum Source { ROWS, TURN, TURNED };
 typedef const uint32_t __attribute__((address_space(4))) *const_words;      // read through the scalar cache
 
 constexpr int W = 8;      // waves of a workgroup
-constexpr int NOTES = 1024;      // groups of U K-steps
+constexpr int NOTES = 1024;      // words of the notes of k_product
 
 // A workgroup of W waves makes W MT x 32 rows of the result by NT x 32 columns; a wave its own MT row tiles.  A K-step
 // is 64 terms of the sum: two words of bits, one for each half of the wave (the matrix instruction takes 8 terms from
@@ -174,7 +174,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
     typedef __attribute__((ext_vector_type(MT))) uint32_t words_t;          // TURN: a lane loads the words of its wave's row tiles at once
     __shared__ u32x4 lds[U][P][8][COLS];
     __shared__ float sums[GRAD ? 64 * W * SUMS : 1];
-    __shared__ int note[NOTES], noted, met, bad;
+    __shared__ uint32_t note[NOTES];
+    __shared__ int met, bad;
     // Workgroups go round the card's 8 dies in turn; each die is given neighbours in row blocks of the same columns and terms, which share the
     // coefficients in its L2 (HBM reads of the level's scores 248 -> 85 MB, of its gradient 193 -> 85; 221 -> 218 and 107.5 -> 104.7 us).
     const int per_die = gridDim.x / 8, tile = (int)(blockIdx.x % 8) * per_die + (int)(blockIdx.x / 8);
@@ -199,9 +200,10 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
     f32x16 acc[MT][NT];
     float column_sum[SUMS];
     // An infinity or NaN that met a zero bit has made NaN of a sum that it has no part in.  If a sum is not finite after the first
-    // sweep, a second one takes such coefficients for zeros and notes the K-steps that have them; they are added afterwards to
-    // the sums whose rows have the bit.
-    if (threadIdx.x == 0) noted = met = bad = 0;
+    // sweep, a second one takes such coefficients for zeros and notes the groups of U K-steps that have them (a bit for one group, or for 2, 4, 8 ..
+    // of sums that are very long); afterwards it is found out there which sums have them.
+    if (threadIdx.x == 0) met = bad = 0;
+    int note_shift = 0;
 
     // Buffer loads: one 32-bit offset a lane, and what lies behind the last term or column reads as zero.  A thread's items: its
     // column in ITEMS groups of terms, or (WIDE) four columns in one group, as they lie in memory.
@@ -434,8 +436,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
                 store_b(careful, real_at);
                 __syncthreads();
                 if (careful.value && threadIdx.x == 0 && met) {
-                    if (noted < NOTES) note[noted] = ks;
-                    ++noted;
+                    const int at = ((ks - first) / U) >> note_shift;
+                    note[at >> 5] |= 1u << (at & 31);
                     met = 0;
                 }
                 if (more) {
@@ -487,8 +489,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
                 store_b(careful, real_at);
                 __syncthreads();
                 if (careful.value && threadIdx.x == 0 && met) {
-                    if (noted < NOTES) note[noted] = ks;
-                    ++noted;
+                    const int at = ((ks - first) / U) >> note_shift;
+                    note[at >> 5] |= 1u << (at & 31);
                     met = 0;
                 }
                 words_t now[U];
@@ -526,30 +528,71 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
     const bool careful = bad;
     bool overflowed = false;
     if (careful) {
+        const int groups = (last - first + U - 1) / U;
+        while (((groups - 1) >> note_shift) >= 32 * NOTES) ++note_shift;
+        for (int i = threadIdx.x; i < NOTES; i += 64 * W) note[i] = 0;
         overflowed = !sweep(std::true_type());
         __syncthreads();
-        for (int e = 0; e < min(noted, NOTES); ++e)
-            for (int q = 0; q < 64 * U; ++q) {
-                const int64_t at = term(note[e] + q / 64, q % 64);
-                if (note[e] + q / 64 >= last || at >= limit) continue;
-                const uint32_t *words = GRAD ? row_of(a.bits, a.n, a.row_stride, a.rows, at) : nullptr;
-                if (GRAD && !words) continue;
+        // Which of a tile's 32 rows of sums have a term that takes them up (+infinity or NaN) or down (-infinity or NaN), a bit each; a lane looks
+        // at its column; both make NaN, in whatever order.  A level's scores in 32 bits and gradient in bf16 take 0.6 and 0.3 ms with one row of
+        // infinities, 2.3 and 2.1 ms when all is NaN.
+        uint32_t up[MT][NT] = {}, down[MT][NT] = {};
+        for (int noted = 0; noted < groups; noted += 1 << note_shift) {
+            const int n_at = noted >> note_shift;
+            if (!(note[n_at >> 5] >> (n_at & 31) & 1u)) continue;
+            for (int h = 2 * (first + noted * U); h < 2 * min(last, first + (noted + (1 << note_shift)) * U); ++h) {
+                // 32 terms; lane j (or j + 32) finds out which of the rows have term j
+                const int64_t t0 = term(h >> 1, 32 * (h & 1));
+                uint32_t has[MT];
+                if constexpr (GRAD) {
+                    const int64_t at = t0 + (lane & 31);
+                    const uint32_t *words = at < limit ? row_of(a.bits, a.n, a.row_stride, a.rows, at) : nullptr;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const int cc = c0 + 32 * n + (lane & 31);
-                    const uint32_t v = cc < a.k ? ((const raw_t *)a.mat)[at * a.mat_stride + cc] : 0;
-                    if (!not_finite<TYPE>(v)) continue;
+                    for (int t = 0; t < MT; ++t) has[t] = words && (tile0 + t) * 32 < out_rows ? words[tile0 + t] : 0u;
+                } else {
 #pragma unroll
-                    for (int t = 0; t < MT; ++t)
+                    for (int t = 0; t < MT; ++t) {
+                        const int64_t r = (tile0 + t) * 32 + (lane & 31);
+                        const uint32_t *words = r < out_rows && t0 < limit ? row_of(a.bits, a.n, a.row_stride, a.rows, r) : nullptr;
+                        has[t] = transposed(words ? words[t0 >> 5] : 0u, lane);
+                    }
+                }
+#pragma unroll 1
+                for (int j0 = 0; j0 < 32; j0 += 8) {
+                    uint32_t v[8][NT];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int64_t r = (tile0 + t) * 32 + 8 * (i >> 2) + 4 * half + (i & 3), bit = GRAD ? r : at;
-                            if (r >= out_rows) continue;
-                            const uint32_t *of = GRAD ? words : row_of(a.bits, a.n, a.row_stride, a.rows, r);
-                            if (of && (of[bit >> 5] >> (bit & 31) & 1u)) acc[t][n][i] += value_of<TYPE>(v);
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            const int cc = c0 + 32 * n + (lane & 31);
+                            v[j][n] = cc < a.k && t0 + j0 + j < limit ? ((const raw_t *)a.mat)[(t0 + j0 + j) * a.mat_stride + cc] : 0u;
+                        }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int t = 0; t < MT; ++t) {
+                            const uint32_t rows = __builtin_amdgcn_readlane(has[t], j0 + j);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+                                if (not_finite<TYPE>(v[j][n])) {
+                                    const float x = value_of<TYPE>(v[j][n]);
+                                    up[t][n] |= x != -INFINITY ? rows : 0u;
+                                    down[t][n] |= x != INFINITY ? rows : 0u;
+                                }
                         }
                 }
             }
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int r = 8 * (i >> 2) + 4 * half + (i & 3);
+                    const bool u = up[t][n] >> r & 1u, d = down[t][n] >> r & 1u;
+                    if (u || d) acc[t][n][i] = !d ? INFINITY : !u ? -INFINITY : NAN;
+                }
     }
 
     const bool whole = a.parts == 1;
@@ -597,9 +640,9 @@ __global__ __launch_bounds__(64 * W, 2) void k_product(ProductArgs a) {
             }
         }
     }
-    // Not finite without the infinities and NaN (or with more K-steps of those than could be noted): twice the sum, which is what the
-    // matrix cores make, may be too large where the sum is not.  Added up term by term.
-    if (!to || (!overflowed && (!careful || noted <= NOTES))) return;
+    // Not finite without the infinities and NaN: twice the sum, which is what the matrix cores make, may be too large where the sum is
+    // not.  Added up term by term.
+    if (!to || !overflowed) return;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int cc = c0 + 32 * n + (lane & 31);

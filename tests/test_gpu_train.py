@@ -155,6 +155,163 @@ def test_infinities_reach_only_the_rows_that_have_the_token(n, k, n_features, dt
     assert np.array_equal(np.isnan(got[1].cpu().numpy()), np.isnan(near_bias)) and np.array_equal(np.isinf(got[1].cpu().numpy()), np.isinf(near_bias))
 
 
+def with_special(finite, has, special):
+    """finite + the infinities and NaN of `special` [terms, k] that each sum has: has [sums, terms] of 0 and 1."""
+    up, down, nan = (has @ x.astype(np.float64) > 0 for x in (special == np.inf, special == -np.inf, np.isnan(special)))
+    return np.where(nan | (up & down), np.nan, np.where(up, np.inf, np.where(down, -np.inf, finite)))
+
+
+@pytest.mark.parametrize("share", [0.002, 0.2, 1.0])
+@pytest.mark.parametrize("n, k, n_features", [(3, 5, 700), (700, 20, 333), (900, 40, 700), (600, 70, 700), (4300, 129, 600), (2100, 400, 2500)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_many_infinities_and_nan(n, k, n_features, dtype, share):
+    """A share of all values, up to each, are infinities of both signs and NaN; a few rows and features have nothing; some of the batch is padding."""
+    rng = np.random.default_rng(n + k)
+    bits, x = packed(rng, n, n_features, density=0.03)
+    bits[5::100] = 0
+    x[5::100] = 0
+    rows, d_rows = batch(rng, n, n)
+    xb, real = picked(x, rows)
+
+    def values(shape):
+        v = rng.normal(size=shape).astype(np.float32)
+        kind = rng.random(shape)
+        special = (rng.random(shape) < share) & (rng.random(shape[1]) < 0.7)          # some columns have none
+        v[special] = np.where(kind < 0.45, np.inf, np.where(kind < 0.9, -np.inf, np.nan))[special]
+        t = torch.from_numpy(v).to(DEV).to(dtype)
+        v = t.double().cpu().numpy()
+        return t, np.where(np.isfinite(v), v, 0.0), np.where(np.isfinite(v), 0.0, v)
+
+    def check(got, want, tol):
+        got = got.double().cpu().numpy()
+        fine = np.isfinite(want)
+        assert ((got == want) | (np.isnan(got) & np.isnan(want)))[~fine].all()
+        near(got[fine], want[fine], tol[fine])
+
+    table, finite, special = values((n_features, k))
+    bias = torch.from_numpy(rng.normal(size=k).astype(np.float32)).to(DEV)
+    b = bias.double().cpu().numpy()
+    want = np.where(real[:, None], with_special(0.37 * (xb @ finite) + b, xb, special), 0.0)
+    check(train.row_scores(bits, table, bias, scale=0.37, rows=d_rows), want, (xb.sum(1)[:, None] + 4) * U * (0.37 * (xb @ np.abs(finite)) + np.abs(b)))
+    grad, finite, special = values((n, k))
+    table_grad, bias_grad = train.row_scores_grad(bits, grad, n_features, scale=0.37, rows=d_rows)
+    check(table_grad, with_special(0.37 * (xb.T @ finite), xb.T, special), (xb.sum(0)[:, None] + 4) * U * 0.37 * (xb.T @ np.abs(finite)))
+    r = real[None].astype(np.float64)
+    check(bias_grad[None], with_special(r @ finite, r, special), (real.sum() + 4) * U * (r @ np.abs(finite)))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_scores_of_a_long_sum_with_nan_all_along_it(dtype):
+    """One column has a NaN in each 256 features of a sum that one workgroup adds up; others have single infinities near its end."""
+    rng = np.random.default_rng(31)
+    n, m, n_features, k = 40, 131_072, 270_000, 64
+    assert train._workspace("stag_row_scores_workspace", m, n_features, k, train._TYPES[dtype]) == 0        # not cut into parts
+    x = rng.random((n, n_features)) < 0.02
+    nan_at = np.arange(200, n_features, 256)
+    x[:, nan_at] = False
+    x[3, nan_at[1]] = True
+    x[4, nan_at[-1]] = True
+    x[[7, 8], [269_990, 269_990]] = True
+    bits = torch.from_numpy(np.packbits(np.pad(x, ((0, 0), (0, -n_features % 128))), axis=1, bitorder="little").view(np.int32).reshape(n, -1).copy()).to(DEV)
+    table = torch.randn((n_features, k), generator=torch.Generator(device=DEV).manual_seed(1), device=DEV)
+    table[torch.from_numpy(nan_at).to(DEV), 0] = math.nan
+    table[269_990, 7], table[269_000, 40], table[268_001, 40] = math.inf, -math.inf, math.inf
+    table = table.to(dtype)
+    rows = rng.integers(0, n, m).astype(np.int32)
+    rows[rng.random(m) < 0.05] = -1
+    got = train.row_scores(bits, table, rows=torch.from_numpy(rows).to(DEV)).cpu().numpy()
+    t = table.double().cpu().numpy()
+    has, finite = x.astype(np.float64), np.where(np.isfinite(t), t, 0.0)
+    want = with_special(has @ finite, has, np.where(np.isfinite(t), 0.0, t))
+    tol = (has.sum(1)[:, None] + 4) * U * (has @ np.abs(finite))
+    for r in range(n):
+        mine = got[rows == r]
+        assert (mine == mine[0]).all() or np.array_equal(mine, np.broadcast_to(mine[0], mine.shape), equal_nan=True)
+        fine = np.isfinite(want[r])
+        assert np.array_equal(mine[0][~fine], want[r][~fine], equal_nan=True), r
+        near(mine[0][fine], want[r][fine], tol[r][fine])
+    assert np.isinf(want[7, 7]) and np.isnan(want[3, 0]) and np.isfinite(want[5, 0]) and (got[rows < 0] == 0).all()
+
+
+@pytest.mark.parametrize("n_features, k, m, dtype", [(61_440, 128, 140_000, F32), (61_440, 128, 140_000, F16), (7_500, 1000, 270_000, BF16)])
+def test_grad_of_a_long_batch_with_nan_all_along_it(n_features, k, m, dtype):
+    """The same for a batch that one workgroup adds up: NaN in one column every 100 rows, single infinities near the end."""
+    rng = np.random.default_rng(32)
+    n = 50
+    bits, x = packed(rng, n, n_features, density=0.05)
+    rows = rng.integers(0, n, m)
+    nan_at = np.arange(50, m, 100)
+    rows[nan_at] = 3
+    x[3, :] = 0                                                     # the row that NaN goes with has few features
+    x[3, [5, 77, n_features - 1]] = 1
+    bits[3] = torch.from_numpy(np.packbits(np.pad(x[3].astype(bool), (0, bits.shape[1] * 32 - n_features)), bitorder="little").view(np.int32)).to(DEV)
+    rows[rng.random(m) < 0.05] = -1
+    rows[[m - 40, m - 30, m - 20, m - 10]] = 7, 8, 7, -1
+    d_rows = torch.from_numpy(rows.astype(np.int32)).to(DEV)
+    grad = torch.randn((m, k), generator=torch.Generator(device=DEV).manual_seed(2), device=DEV)
+    grad[torch.from_numpy(nan_at).to(DEV), 0] = math.nan
+    grad[m - 40, 7], grad[m - 30, 100], grad[m - 20, 100], grad[m - 10, 50] = math.inf, math.inf, -math.inf, math.nan          # the last is padding
+    grad = grad.to(dtype)
+    table_grad, bias_grad = (t.double().cpu().numpy() for t in train.row_scores_grad(bits, grad, n_features, rows=d_rows))
+    # what each held row is picked for, summed in 64 bits
+    real, at = d_rows >= 0, d_rows.clamp(min=0).long()
+    g = torch.where(real[:, None], grad.double(), 0.0)
+    fine, special = torch.where(torch.isfinite(g), g, 0.0), torch.where(torch.isfinite(g), 0.0, g)
+    per_row, size = (torch.zeros((n, k), dtype=torch.float64, device=DEV).index_add_(0, at, y).cpu().numpy() for y in (fine, fine.abs()))
+    marks = torch.zeros((n, k), dtype=torch.float64, device=DEV).index_add_(0, at, special).cpu().numpy()
+    count = np.bincount(rows[rows >= 0], minlength=n)
+    want = with_special(x.T @ per_row, x.T, marks)
+    tol = ((x.T @ count)[:, None] + 4) * U * (x.T @ size)
+    fine = np.isfinite(want)
+    assert np.array_equal(table_grad[~fine], want[~fine], equal_nan=True) and (~fine[:, 7]).any() and (~fine[:, 100]).any() and fine[:, 50].all() and fine[1, 0]
+    near(table_grad[fine], want[fine], tol[fine])
+    one = np.ones((1, n))
+    want = with_special(one @ per_row, one, marks)[0]
+    fine = np.isfinite(want)
+    assert np.array_equal(bias_grad[~fine], want[~fine], equal_nan=True) and (~fine).sum() == 3
+    near(bias_grad[fine], want[fine], ((rows >= 0).sum() + 4) * U * size.sum(0)[fine])
+
+
+def test_infinities_in_sums_of_millions_of_terms():
+    """Sums that one workgroup adds up in more than 32,768 groups of terms: 8.6 million features, 4.3 million rows."""
+    rng = np.random.default_rng(33)
+    m, f, k = 131_072, 8_600_000, 64
+    assert train._workspace("stag_row_scores_workspace", m, f, k, 1) == 0
+    table = torch.randn((f, k), generator=torch.Generator(device=DEV).manual_seed(3), device=DEV).to(BF16)
+    bits = np.zeros((4, -(-f // 128) * 4), np.uint32)
+    token = [np.unique(rng.integers(0, f - 100, 20_000)) for _ in range(4)]
+    for r, t in enumerate(token):
+        token[r] = np.append(t, f - 1 - r)
+        np.bitwise_or.at(bits[r], token[r] >> 5, np.uint32(1) << (token[r] & 31).astype(np.uint32))
+    table[f - 1, 3], table[f - 2, 40], table[int(token[2][10]), 5], table[int(token[2][10_000]), 5], table[f - 90, 6] = math.inf, -math.inf, math.inf, -math.inf, math.nan
+    rows = torch.arange(m, device=DEV, dtype=torch.int32) % 4
+    got = train.row_scores(torch.from_numpy(bits.view(np.int32)).to(DEV), table, rows=rows)
+    for r in range(4):
+        mine, terms = got[r::4], table[torch.from_numpy(token[r]).to(DEV)].double()
+        want, size = terms.sum(0).cpu().numpy(), terms.abs().sum(0).cpu().numpy()
+        assert torch.equal(mine.nan_to_num(7e30), mine[:1].expand_as(mine).nan_to_num(7e30))
+        fine = np.isfinite(want)
+        assert (~fine).sum() == (1 if r < 3 else 0) and np.array_equal(mine[0].cpu().numpy()[~fine], want[~fine], equal_nan=True)
+        near(mine[0].cpu().numpy()[fine], want[fine], (len(token[r]) + 4) * U * size[fine])
+    del table, got
+    n, m, f, k = 50, 4_300_000, 61_440, 128
+    bits, x = packed(rng, n, f, density=0.05)
+    rows = rng.integers(0, n, m).astype(np.int32)
+    rows[[m - 1, m - 2, 5]] = 7, 8, 9
+    d_rows = torch.from_numpy(rows).to(DEV)
+    grad = torch.randn((m, k), generator=torch.Generator(device=DEV).manual_seed(4), device=DEV).to(BF16)
+    grad[m - 1, 3], grad[m - 2, 40], grad[5, 40] = math.inf, math.inf, math.nan
+    got = train.row_scores_grad(bits, grad, f, rows=d_rows)[0].double().cpu().numpy()
+    g = grad.double()
+    sums = [torch.zeros((n, k), dtype=torch.float64, device=DEV).index_add_(0, d_rows.long(), y).cpu().numpy()
+            for y in (torch.where(torch.isfinite(g), g, 0.0), torch.where(torch.isfinite(g), g.abs(), 0.0), torch.where(torch.isfinite(g), 0.0, g))]
+    want = with_special(x.T @ sums[0], x.T, sums[2])
+    fine = np.isfinite(want)
+    assert np.array_equal(got[~fine], want[~fine], equal_nan=True) and (~fine).any(0).nonzero()[0].tolist() == [3, 40]
+    terms = (x.T @ np.bincount(rows, minlength=n))[:, None]
+    near(got[fine], want[fine], ((terms + 4) * U * (x.T @ sums[1]))[fine])
+
+
 @pytest.mark.parametrize("n, k, n_features", [(1, 4, 333), (40, 5, 333), (600, 70, 333), (1500, 200, 333), (2100, 400, 2500), (700, 20, 333)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_sums_near_the_largest_number_beside_infinities(n, k, n_features, dtype):
