@@ -137,8 +137,9 @@ def _ptr(t):
 
 
 @functools.lru_cache(maxsize=65536)
-def _workspace(name, *sizes):
-    nbytes = getattr(_lib.train_lib(), name)(*sizes)
+def _workspace(name, m, *sizes):
+    _need(max(sizes) < 2**31, "sizes of 2^31 and more: %s", sizes)          # the C ABI has 32 bits for all but m
+    nbytes = getattr(_lib.train_lib(), name)(m, *sizes)
     if nbytes < 0:
         _lib.check_train(int(nbytes))
     return nbytes
@@ -189,9 +190,9 @@ def row_scores(bits, table, bias=None, *, scale=1.0, rows=None, out=None):
     n = bits.shape[0]
     n_features, k = table.shape
     m = n if rows is None else rows.shape[0]
+    need = _workspace("stag_row_scores_workspace", m, n_features, k, kind)
     if out is None:
         out = _empty((m, k), (k, 1), dtype=_F32, device=bits.device)
-    need = _workspace("stag_row_scores_workspace", m, n_features, k, kind)
     work = _empty((need,), (1,), dtype=torch.uint8, device=bits.device) if need else None
     rc = _lib.train_lib().stag_row_scores_dev(bits.data_ptr(), n, row_stride, n_features, None if rows is None else rows.data_ptr(), m, table.data_ptr(), kind,
                                               table_stride, None if bias is None else bias.data_ptr(), k, float(scale), out.data_ptr(), score_stride,
@@ -245,12 +246,12 @@ def row_scores_grad(bits, grad, n_features, *, scale=1.0, rows=None, out=None):
         with torch.cuda.device(gpu):
             return row_scores_grad(bits, grad, n_features, scale=scale, rows=rows, out=out)
     m, k = grad.shape
+    need = _workspace("stag_row_scores_grad_workspace", m, n_features, k, kind)
     if out is None:
         table_grad = _empty((n_features, k), (k, 1), dtype=_F32, device=bits.device)
         bias_grad = _empty((k,), (1,), dtype=_F32, device=bits.device)
     else:
         table_grad, bias_grad = out
-    need = _workspace("stag_row_scores_grad_workspace", m, n_features, k, kind)
     work = _empty((need,), (1,), dtype=torch.uint8, device=bits.device) if need else None
     rc = _lib.train_lib().stag_row_scores_grad_dev(bits.data_ptr(), bits.shape[0], row_stride, n_features, None if rows is None else rows.data_ptr(), m, grad.data_ptr(),
                                                    kind, grad_stride, k, float(scale), table_grad.data_ptr(), stride, bias_grad.data_ptr(),
@@ -312,12 +313,12 @@ def sibling_loss(scores, label, *, siblings=None, weight=None, scale=1.0, grad_d
         with torch.cuda.device(gpu):
             return sibling_loss(scores, label, siblings=siblings, weight=weight, scale=scale, grad_dtype=dtype, out=out)
     m, k = scores.shape
+    need = _workspace("stag_sibling_loss_workspace", m, k)
     if out is None:
         loss = _empty((k,), (1,), dtype=_F32, device=scores.device)
         grad = _empty((m, k), (k, 1), dtype=dtype, device=scores.device)
     else:
         loss, grad = out
-    need = _workspace("stag_sibling_loss_workspace", m, k)
     work = _empty((need,), (1,), dtype=torch.uint8, device=scores.device) if need else None
     rc = _lib.train_lib().stag_sibling_loss_dev(scores.data_ptr(), score_stride, m, k, label.data_ptr(), None if siblings is None else siblings.data_ptr(),
                                                 None if weight is None else weight.data_ptr(), float(scale), loss.data_ptr(), grad.data_ptr(), _TYPES[dtype], grad_stride,

@@ -872,6 +872,15 @@ def test_an_empty_batch_of_a_large_table():
     assert not any(bool(out[0][i:i + 7_000].any()) for i in range(0, 70_000, 7_000)) and not out[1].any()
 
 
+def test_more_features_than_32_bits_count_are_refused():
+    """2^32 + 5 features, which is 5 in 32 bits."""
+    bits = torch.zeros((1, 2**27 + 4), dtype=torch.int32, device=DEV)
+    held = torch.cuda.memory_allocated()
+    with pytest.raises(ValueError, match="sizes of 2"):
+        train.row_scores_grad(bits, torch.ones((1, 1), device=DEV), 2**32 + 5)
+    assert torch.cuda.memory_allocated() < held + 2**20
+
+
 def test_outputs_over_inputs_are_refused():
     bits, _ = packed(np.random.default_rng(0), 50, 300)
     buffer = torch.zeros(400, 40, device=DEV)

@@ -152,6 +152,15 @@ def test_too_narrow_and_unaligned_rows():
     assert train._packed(rows(8, 8).t(), 100)[1] == 8       # copied to contiguous rows
 
 
+def test_sizes_that_32_bits_would_wrap_are_refused():
+    for name, *sizes in (("stag_row_scores_workspace", 1, 2**32 + 5, 3, 0), ("stag_row_scores_workspace", 1, 5, 2**32 + 3, 0),
+                         ("stag_row_scores_grad_workspace", 1, 2**32 + 5, 3, 0), ("stag_sibling_loss_workspace", 1, 2**32 + 3)):
+        with pytest.raises(ValueError, match="sizes of 2"):
+            train._workspace(name, *sizes)
+    with pytest.raises(_lib.StagError, match="m = 4294967301"):
+        train._workspace("stag_sibling_loss_workspace", 2**32 + 5, 3)
+
+
 def test_rows_far_apart_are_copied_or_refused():
     """A matrix whose rows lie more than 2^21 values apart: inputs are copied, outputs refused, and so is the stride at the C entry."""
     wide = torch.empty(2, 2**21 + 8)[:, :3]
