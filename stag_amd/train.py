@@ -177,7 +177,7 @@ def row_scores(bits, table, bias=None, *, scale=1.0, rows=None, out=None):
         gpu = bits.get_device()
         if gpu >= 0 and table.get_device() == gpu and bits.dim() == 2 and table.dim() == 2 and bits.dtype in _BITS:
             row_stride, (n_features, k) = bits.shape[1], table.shape
-            if (row_stride & 3 == 0 and k and 0 < n_features <= row_stride * 32 and (bias is None or _plain(bias, _F32, (k,), gpu))
+            if (row_stride & 3 == 0 and bits.data_ptr() & 15 == 0 and k and 0 < n_features <= row_stride * 32 and (bias is None or _plain(bias, _F32, (k,), gpu))
                     and (rows is None or (type(rows) is _Tensor and rows.dim() == 1 and _plain(rows, _I32, rows.shape, gpu)))):
                 kind = 0 if table.dtype is _F32 else _TYPES.get(table.dtype, -1)
                 table_stride = score_stride = k
@@ -235,7 +235,7 @@ def row_scores_grad(bits, grad, n_features, *, scale=1.0, rows=None, out=None):
         gpu = bits.get_device()
         if gpu >= 0 and grad.get_device() == gpu and bits.dim() == 2 and grad.dim() == 2 and bits.dtype in _BITS:
             (n, row_stride), (m, k) = bits.shape, grad.shape
-            if (row_stride & 3 == 0 and k and m and 0 < n_features <= row_stride * 32 and (n == m if rows is None else _plain(rows, _I32, (m,), gpu))
+            if (row_stride & 3 == 0 and bits.data_ptr() & 15 == 0 and k and m and 0 < n_features <= row_stride * 32 and (n == m if rows is None else _plain(rows, _I32, (m,), gpu))
                     and out is None):
                 kind = 0 if grad.dtype is _F32 else _TYPES.get(grad.dtype, -1)
                 grad_stride = stride = k

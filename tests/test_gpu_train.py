@@ -881,6 +881,16 @@ def test_more_features_than_32_bits_count_are_refused():
     assert torch.cuda.memory_allocated() < held + 2**20
 
 
+def test_contiguous_rows_at_odd_addresses_are_refused():
+    """With the same error as rows that are not contiguous."""
+    flat = torch.zeros(41, dtype=torch.int32, device=DEV)
+    for bits in (flat[1:].view(10, 4), flat[1:33].view(4, 8)[:, :4]):
+        with pytest.raises(ValueError, match="aligned 16-byte units"):
+            train.row_scores(bits, torch.ones((100, 3), device=DEV))
+        with pytest.raises(ValueError, match="aligned 16-byte units"):
+            train.row_scores_grad(bits, torch.ones((bits.shape[0], 3), device=DEV), 100)
+
+
 def test_outputs_over_inputs_are_refused():
     bits, _ = packed(np.random.default_rng(0), 50, 300)
     buffer = torch.zeros(400, 40, device=DEV)
