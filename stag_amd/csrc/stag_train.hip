@@ -55,8 +55,9 @@ __device__ __forceinline__ const uint32_t *row_of(const uint32_t *bits, int64_t 
 // and run on the matrix cores although four of five bits are 0: 1,500 additions a score fed from LDS or L2 one by one take longer than
 // 7,500 multiply-adds at the matrix cores' rate.  A bit becomes a 16-bit operand by one shift and one mask: bit 14 alone is 2.0, in bf16
 // and in f16, and a mask of two such bits makes a pair; the factor 2 is taken out of the result.  A zero or one is exact
-// in 16 bits; a 32-bit coefficient is cut into three bf16 pieces of 8 bits each, which together are the coefficient,
-// and multiplied piece by piece into the same 32-bit sums.  16-bit coefficients go in as they are.
+// in 16 bits; a 32-bit coefficient is cut into three bf16 pieces of 8 bits each, which together are the coefficient (to 2^-133, the
+// smallest step of bf16: below 2^-110 that is less than 24 bits), and multiplied piece by piece into the same 32-bit sums.  16-bit
+// coefficients go in as they are.
 //
 // What bounds them: the matrix cores for 32-bit coefficients (8,192 rows x 7,500 features x 1,000 columns: 218 us, 1.7 PFLOP/s of bf16
 // operations counted densely; a library's bf16 product of 8,192^3 reaches 1.19 on the same card), the making of operands
@@ -740,7 +741,7 @@ constexpr int LOOKUP_WORDS = 256;
 template <typename T>
 __global__ __launch_bounds__(1024) void k_lookup(ProductArgs a, int cw_log) {
     __shared__ uint16_t token[LOOKUP_WORDS * 32];
-    __shared__ int before[5];
+    __shared__ int before[4];
     __shared__ float part[1024];
     const int64_t i = blockIdx.x;
     const int cw = 1 << cw_log, c = blockIdx.y * cw + (threadIdx.x & (cw - 1)), slot = threadIdx.x >> cw_log, slots = 1024 >> cw_log;
@@ -1278,6 +1279,8 @@ __global__ __launch_bounds__(256) void k_adamw(AdamwArgs a) {
                     uint32_t m_codes = 0, v_codes = 0;
                     auto code = [&](auto place) {
                         constexpr int j = place.value;
+                        // Two rounds of shift, exclusive or and multiply, with the constants that C. Wellons published ("Prospecting for Hash
+                        // Functions", 2018)
                         uint32_t x = (uint32_t)(s + j) ^ salt;
                         x = (x ^ x >> 16) * 0x7FEB352Du;
                         x = (x ^ x >> 15) * 0x846CA68Bu;
@@ -1501,7 +1504,8 @@ LossPlan loss_plan(int64_t m, int32_t k, int v, bool siblings) {
     p.ct = (int)(cols < p.threads ? cols : p.threads);
     p.gy = (unsigned)ceil_div(cols, p.ct);
     // 1,024 workgroups, or 512 where each writes rows of siblings' gradients over nearly all of its threads (65,536 x 1,000 in 32 bits 60
-    // against 71 us, x 4,000 in bf16 97 against 112; over half of the threads, x 1,000 and x 520 in bf16, 52 against 36 and 47 against 30)
+    // against 71 us, x 4,000 in bf16 97 against 112; over half of the threads, x 1,000 and x 520 in bf16, 52 against 36 and 47 against 30).
+    // A last tile of few columns takes as many workgroups as a full one, which costs most just above one tile (x 256 24 us, x 257 69).
     const unsigned all = siblings && p.ct >= 192 ? 512 : 1024;
     const int64_t passes = ceil_div(m, p.threads / p.ct), wanted = all / p.gy > 0 ? all / p.gy : 1;
     p.gx = (unsigned)(few ? 1 : passes < wanted ? passes : wanted);
