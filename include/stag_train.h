@@ -61,8 +61,8 @@ int64_t stag_row_scores_grad_workspace(int64_t m, int32_t n_features, int32_t k,
  * r_i = d_rows[i], or i when d_rows is NULL (then m <= n).  The same row may be named more than once; an index outside
  * 0..n-1 marks padding, whose scores are 0.  table[f][c] = d_table[f * table_stride + c], of `type`; d_bias (k values)
  * may be NULL; scores[i][c] = d_scores[i * score_stride + c], 32-bit.
- * Sums are held in 32 bits; 32-bit coefficients count with their 24 bits, or to 2^-133 where that is coarser.  Only the coefficients of features that a row has
- * enter its score, so infinities and NaN elsewhere in the table do not reach it.
+ * Sums are held in 32 bits; 32-bit coefficients count with their 24 bits, or to 2^-133 where that is coarser.  Only the
+ * coefficients of features that a row has enter its score, so infinities and NaN elsewhere in the table do not reach it.
  */
 int stag_row_scores_dev(const uint32_t *d_bits, int64_t n, int64_t row_stride, int32_t n_features, const int32_t *d_rows,
                         int64_t m, const void *d_table, int32_t type, int64_t table_stride, const float *d_bias, int32_t k,

@@ -15,8 +15,8 @@ these steps for the children of one node and returns coefficients in the form ``
 
 All functions take torch tensors on one GPU, enqueue their work on that GPU's current stream and return without waiting;
 they take no part in autograd.  With their outputs given (``out=``: fixed buffers, at the price of more checks on the host) or allocated
-under capture they can be recorded into a HIP graph.  Inputs whose rows are not contiguous (or lie more than 2^21 values apart) are copied first; outputs have to be as
-documented and may share memory with nothing else that the call takes.
+under capture they can be recorded into a HIP graph.  Inputs whose rows are not contiguous (or lie more than 2^21 values apart) are copied
+first; outputs have to be as documented and may share memory with nothing else that the call takes.
 """
 import ctypes
 import functools
